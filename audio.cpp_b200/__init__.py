@@ -22,6 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libb200diff.so")
 
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_BF16 = 0, 1, 8, 30
+TYPE_I8, TYPE_E4M3 = 24, 256  # paged cache elements
 EPI_F32, EPI_CT, EPI_SWIGLU, EPI_RESID = 0, 1, 2, 3
 
 STATUS = {0: "ok", -1: "EINVAL", -2: "ECUDA", -3: "ENOMEM", -4: "ESTATE", -5: "ENONFINITE", -6: "ETIMEOUT",
@@ -33,7 +34,9 @@ EXPORTED = ["b2d_create", "b2d_destroy", "b2d_last_error", "b2d_sync", "b2d_vers
             "b2d_sa3_load", "b2d_sa3_sample", "b2d_sa3_sample_device", "b2d_oobleck_load", "b2d_oobleck_decode",
             "b2d_oobleck_decode_device", "b2d_vvdec_load", "b2d_vvdec_decode", "b2d_vvdec_decode_device",
             "b2d_saocond_load", "b2d_saocond_encode", "b2d_saocond_encode_device",
-            "b2d_vvlm_load", "b2d_vvlm_prefill", "b2d_vvlm_step", "b2d_vvlm_prefill_device", "b2d_vvlm_step_device"]
+            "b2d_vvlm_load", "b2d_vvlm_prefill", "b2d_vvlm_step", "b2d_vvlm_prefill_device", "b2d_vvlm_step_device",
+            "b2d_kv_check", "b2d_kv_append", "b2d_kv_gather", "b2d_paged_attention_workspace", "b2d_paged_attention",
+            "b2d_sample_tokens"]
 
 
 class B2DError(RuntimeError):
@@ -114,6 +117,25 @@ class VvlmConfig(C.Structure):
                 ("eps", C.c_float), ("rope_theta", C.c_float)]
 
 
+class KvCacheDesc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int64), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p)]
+
+
+class KvBatchDesc(C.Structure):
+    _fields_ = [("seqs", C.c_int32), ("max_new", C.c_int32), ("max_context", C.c_int32), ("rows", C.c_int64),
+                ("row_start", C.c_void_p), ("context", C.c_void_p), ("page_table", C.c_void_p),
+                ("table_stride", C.c_int64)]
+
+
+class SampleRequest(C.Structure):
+    _fields_ = [("logits_type", C.c_int32), ("rows", C.c_int64), ("vocab", C.c_int64), ("row_stride", C.c_int64),
+                ("logits", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
+                ("min_p", C.c_void_p), ("uniform", C.c_void_p), ("tokens", C.c_void_p), ("probs", C.c_void_p)]
+
+
 SA3_SAMPLERS = {"": 0, "pingpong": 0, "euler": 1}
 
 SAMPLERS = {"dpmpp-2m": 0, "dpmpp-3m-sde": 1, "": 2, "euler": 2, "pingpong": 2}
@@ -177,6 +199,14 @@ def lib() -> C.CDLL:
         L.b2d_vvlm_step.argtypes = [P, P, P, P, P]
         L.b2d_vvlm_prefill_device.argtypes = [P, P, I64, P, P, P]
         L.b2d_vvlm_step_device.argtypes = [P, P, P, P, P]
+        L.b2d_kv_check.argtypes = [C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), I32, C.c_char_p, C.c_size_t]
+        L.b2d_kv_append.argtypes = [P, C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), I32, P, P, I64, P]
+        L.b2d_kv_gather.argtypes = [P, C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), I32, P, P, I64, P]
+        L.b2d_paged_attention_workspace.argtypes = [P, C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), I32]
+        L.b2d_paged_attention_workspace.restype = C.c_size_t
+        L.b2d_paged_attention.argtypes = [P, C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), I32, P, I64, P, I64, I32, F,
+                                          I32, P, C.c_size_t, P]
+        L.b2d_sample_tokens.argtypes = [P, C.POINTER(SampleRequest), P]
         _lib = L
     return _lib
 
@@ -225,6 +255,87 @@ def _ptr(a) -> int:
     if hasattr(a, "data_ptr"):
         return a.data_ptr()
     return a.ctypes.data
+
+
+# torch dtypes by name (this layer does not import torch)
+_TENSOR_TYPES = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16,
+                 "torch.int8": TYPE_I8, "torch.float8_e4m3fn": TYPE_E4M3}
+
+
+def _tensor_type(t, allowed, what: str) -> int:
+    got = _TENSOR_TYPES.get(str(t.dtype))
+    if got not in allowed:
+        raise B2DError(-1, "%s of type %s" % (what, t.dtype))
+    return got
+
+
+def _want(t, what: str, shape, dtype: str, device=None):
+    """A contiguous tensor of this shape and type (on this device), or a refusal."""
+    if tuple(t.shape) != tuple(shape) or str(t.dtype) != dtype or not t.is_contiguous():
+        raise B2DError(-1, "%s must be a contiguous %s tensor of shape %s" % (what, dtype, tuple(shape)))
+    if device is not None and t.device != device:
+        raise B2DError(-1, "%s is on %s, not on %s" % (what, t.device, device))
+    return t
+
+
+class PagedCache:
+    """One layer's paged keys and values (b2d_kv_cache) over the caller's torch tensors.
+
+    ``k``, ``v``: [pages, kv_heads, page_size, head_dim] views of any page / head / slot strides (the last dimension
+    contiguous), float16, bfloat16, int8 or float8_e4m3fn; the 8-bit types also need ``k_scale`` / ``v_scale``, contiguous
+    float32 [pages, kv_heads, page_size].  The tensors stay the caller's; this object keeps them alive."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        kind = _tensor_type(k, (TYPE_F16, TYPE_BF16, TYPE_I8, TYPE_E4M3), "paged cache")
+        if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device or v.stride() != k.stride():
+            raise B2DError(-1, "paged cache k and v must be 4-d and alike in shape, strides, type and device")
+        if k.stride(3) != 1:
+            raise B2DError(-1, "paged cache head_dim must be contiguous")
+        if kind in (TYPE_I8, TYPE_E4M3):
+            if k_scale is None or v_scale is None:
+                raise B2DError(-1, "an 8-bit paged cache needs its scales")
+            _want(k_scale, "k_scale", k.shape[:3], "torch.float32", k.device)
+            _want(v_scale, "v_scale", k.shape[:3], "torch.float32", k.device)
+        else:
+            k_scale = v_scale = None
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.type, self.device = kind, k.device
+        pages, kv_heads, page_size, head_dim = k.shape
+        self.desc = KvCacheDesc(kind, page_size, pages, kv_heads, head_dim, k.stride(0), k.stride(1), k.stride(2),
+                                k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
+                                v_scale.data_ptr() if v_scale is not None else None)
+
+
+class PagedBatch:
+    """The new tokens of some sequences (b2d_kv_batch): int32 device tensors ``row_start`` [seqs + 1], ``context`` [seqs]
+    and ``page_table`` [seqs, pages], with the bounds that hold for this call and every replay of it."""
+
+    def __init__(self, row_start, context, page_table, rows: int, max_new: int, max_context: int):
+        seqs = context.shape[0]
+        _want(context, "context", (seqs,), "torch.int32")
+        _want(row_start, "row_start", (seqs + 1,), "torch.int32", context.device)
+        if page_table.dim() != 2 or page_table.shape[0] != seqs or str(page_table.dtype) != "torch.int32" or \
+                (page_table.numel() and page_table.stride(1) != 1) or page_table.device != context.device:
+            raise B2DError(-1, "page_table must be an int32 tensor [seqs, pages] with contiguous rows")
+        self.row_start, self.context, self.page_table = row_start, context, page_table
+        self.rows, self.device = rows, context.device
+        stride = page_table.stride(0) if seqs > 1 else page_table.shape[1]
+        if stride < page_table.shape[1]:
+            raise B2DError(-1, "page_table rows overlap")
+        self.table_pages = page_table.shape[1]
+        self.desc = KvBatchDesc(seqs, max_new, max_context, rows, row_start.data_ptr(), context.data_ptr(),
+                                page_table.data_ptr(), stride)
+
+
+def check_paged(cache: PagedCache, batch: PagedBatch, heads: int = 0) -> None:
+    """The checks that the calls make of a cache, a batch and (unless 0) the query heads; needs no GPU."""
+    if batch.desc.seqs and -(-batch.desc.max_context // cache.desc.page_size) > batch.table_pages:
+        raise B2DError(-1, "page_table rows of %d pages do not hold max_context %d"
+                       % (batch.table_pages, batch.desc.max_context))
+    err = C.create_string_buffer(256)
+    st = lib().b2d_kv_check(C.byref(cache.desc), C.byref(batch.desc), heads, err, 256)
+    if st != 0:
+        raise B2DError(st, err.value.decode())
 
 
 class Context:
@@ -298,6 +409,84 @@ class Context:
                                          epilogue, bn, split, C.c_void_p(bias or None), C.c_void_p(out or None), ldo,
                                          C.c_void_p(resid or None), ldr, C.c_void_p(gate or None), ldg,
                                          C.c_void_p(stream)))
+
+    # ------------------------------------------------------- serving operators
+    def _on_device(self, *tensors) -> None:
+        for t in tensors:
+            if t is not None and (t.device.type != "cuda" or t.device.index != self.device):
+                raise B2DError(-1, "tensor on %s; this context's device is cuda:%d" % (t.device, self.device))
+
+    def _cache_rows(self, cache: PagedCache, batch: PagedBatch, k, v):
+        """(element type, row stride) of k / v rows [rows, kv_heads, head_dim] whose last two dimensions are packed."""
+        check_paged(cache, batch)
+        kind = _tensor_type(k, (TYPE_F32, TYPE_F16, TYPE_BF16), "cache rows")
+        shape = (batch.rows, cache.desc.kv_heads, cache.desc.head_dim)
+        for t in (k, v):
+            if tuple(t.shape) != shape or t.dtype != k.dtype or t.stride(2) != 1 or t.stride(1) != shape[2] or \
+                    t.stride(0) != k.stride(0):
+                raise B2DError(-1, "cache rows must be alike, [rows, kv_heads, head_dim] = %s, heads packed" % (shape,))
+        self._on_device(cache.k, batch.context, k, v)
+        return kind, k.stride(0) if batch.rows > 1 else shape[1] * shape[2]
+
+    def kv_append(self, cache: PagedCache, batch: PagedBatch, k, v, stream: int = 0) -> None:
+        """Writes the batch's rows into the cache, quantising them to its type (b2d_kv_append)."""
+        kind, stride = self._cache_rows(cache, batch, k, v)
+        self.check(lib().b2d_kv_append(self._h, C.byref(cache.desc), C.byref(batch.desc), kind, _ptr(k), _ptr(v), stride,
+                                       C.c_void_p(stream)))
+
+    def kv_gather(self, cache: PagedCache, batch: PagedBatch, k_out, v_out, stream: int = 0) -> None:
+        """Reads the batch's rows back as the values they stand for (b2d_kv_gather)."""
+        kind, stride = self._cache_rows(cache, batch, k_out, v_out)
+        self.check(lib().b2d_kv_gather(self._h, C.byref(cache.desc), C.byref(batch.desc), kind, _ptr(k_out), _ptr(v_out),
+                                       stride, C.c_void_p(stream)))
+
+    def paged_attention_workspace(self, cache: PagedCache, batch: PagedBatch, heads: int) -> int:
+        """Bytes of workspace paged_attention needs for batches of these bounds."""
+        check_paged(cache, batch, heads)
+        return lib().b2d_paged_attention_workspace(self._h, C.byref(cache.desc), C.byref(batch.desc), heads)
+
+    def paged_attention(self, q, cache: PagedCache, batch: PagedBatch, out, scale: Optional[float] = None,
+                        window: int = 0, workspace=None, stream: int = 0) -> None:
+        """Causal attention of the batch's rows over the cache (b2d_paged_attention): q, out [rows, heads, head_dim]
+        float16 or bfloat16 with packed heads; scale defaults to head_dim ** -0.5; workspace: a uint8 tensor of
+        paged_attention_workspace bytes (calls that may overlap need one each)."""
+        hd = cache.desc.head_dim
+        if q.dim() != 3 or q.shape[0] != batch.rows or q.shape[2] != hd:
+            raise B2DError(-1, "paged attention queries must be [rows, heads, head_dim]")
+        heads = q.shape[1]
+        check_paged(cache, batch, heads)
+        kind = _tensor_type(q, (TYPE_F16, TYPE_BF16), "paged attention queries")
+        for t in (q, out):
+            if t.shape != q.shape or t.dtype != q.dtype or t.stride(2) != 1 or t.stride(1) != hd:
+                raise B2DError(-1, "paged attention q and out must be alike with packed heads")
+        self._on_device(cache.k, batch.context, q, out, workspace)
+        rows = [t.stride(0) if batch.rows > 1 else heads * hd for t in (q, out)]
+        self.check(lib().b2d_paged_attention(
+            self._h, C.byref(cache.desc), C.byref(batch.desc), int(kind == TYPE_BF16), _ptr(q), rows[0], _ptr(out),
+            rows[1], heads, float(hd ** -0.5 if scale is None else scale), window,
+            _ptr(workspace) if workspace is not None else None, workspace.numel() if workspace is not None else 0,
+            C.c_void_p(stream)))
+
+    def sample_tokens(self, logits, temperature, top_k, top_p, min_p, uniform, tokens, probs=None,
+                      stream: int = 0) -> None:
+        """The next token of each row of logits [rows, vocab] (b2d_sample_tokens); top_k, top_p, min_p and probs may be
+        None.  temperature, top_p, min_p, uniform, probs: float32 [rows]; top_k, tokens: int32 [rows]."""
+        if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1):
+            raise B2DError(-1, "logits must be [rows, vocab] with contiguous rows")
+        kind = _tensor_type(logits, (TYPE_F32, TYPE_F16, TYPE_BF16), "logits")
+        rows, vocab = logits.shape
+        for name, t, dtype in (("temperature", temperature, "torch.float32"), ("top_k", top_k, "torch.int32"),
+                               ("top_p", top_p, "torch.float32"), ("min_p", min_p, "torch.float32"),
+                               ("uniform", uniform, "torch.float32"), ("tokens", tokens, "torch.int32"),
+                               ("probs", probs, "torch.float32")):
+            if t is not None:
+                _want(t, name, (rows,), dtype)
+        self._on_device(logits, temperature, top_k, top_p, min_p, uniform, tokens, probs)
+        rq = SampleRequest(kind, rows, vocab, logits.stride(0) if rows > 1 else vocab, _ptr(logits), _ptr(temperature),
+                           _ptr(top_k) if top_k is not None else None, _ptr(top_p) if top_p is not None else None,
+                           _ptr(min_p) if min_p is not None else None, _ptr(uniform), _ptr(tokens),
+                           _ptr(probs) if probs is not None else None)
+        self.check(lib().b2d_sample_tokens(self._h, C.byref(rq), C.c_void_p(stream)))
 
 
 WeightSpec = Tuple[str, int, Tuple[int, ...], np.ndarray]  # (name, ggml type, dims, raw payload)

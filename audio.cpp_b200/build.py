@@ -2,8 +2,9 @@
 
     python audio.cpp_b200/build.py
 
-Sources: csrc/api.cu (C ABI + runtimes), csrc/schedule.cpp (host scheduler),
-headers csrc/*.cuh and include/b200diff.h.  No torch, no JIT cache: the .so
+Sources: csrc/api.cu (C ABI + runtimes), csrc/serve.cu (the language model's serving operators), csrc/noalloc.cu,
+csrc/schedule.cpp (host scheduler), csrc/storage.cpp; headers csrc/*.cuh and include/b200diff.h.  Each source is
+compiled to an object under build/ (in parallel, and again only when it or a header it includes changed).  No torch, no JIT cache: the .so
 lands next to this file so it travels with the repository snapshot.
 """
 from __future__ import annotations
@@ -11,16 +12,19 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libb200diff.so")
-SOURCES = [os.path.join(HERE, "csrc", "api.cu"), os.path.join(HERE, "csrc", "noalloc.cu"),
+SOURCES = [os.path.join(HERE, "csrc", "api.cu"), os.path.join(HERE, "csrc", "serve.cu"),
+           os.path.join(HERE, "csrc", "noalloc.cu"),
            os.path.join(HERE, "csrc", "schedule.cpp"), os.path.join(HERE, "csrc", "storage.cpp")]
 DEPS = SOURCES + [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc"))] + [
     os.path.join(os.path.dirname(HERE), "include", "b200diff.h")]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-              "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-shared"]
+              "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
+OBJECTS = os.path.join(HERE, "build")
 
 
 def nvcc() -> str:
@@ -35,6 +39,24 @@ def up_to_date() -> bool:
         return False
     t = os.path.getmtime(LIB)
     return all(os.path.getmtime(p) <= t for p in DEPS if os.path.exists(p))
+
+
+def compile_object(source: str, force: bool, verbose: bool) -> str:
+    """One source as an object; nvcc's own dependency list (-MD) says whether the object still stands."""
+    obj = os.path.join(OBJECTS, os.path.basename(source) + ".o")
+    deps = obj + ".d"
+    if not force and os.path.exists(obj) and os.path.exists(deps):
+        with open(deps) as f:
+            paths = f.read().split(":", 1)[1].replace("\\\n", " ").split()
+        paths.append(os.path.abspath(__file__))
+        if all(os.path.exists(p) and os.path.getmtime(p) <= os.path.getmtime(obj) for p in paths):
+            return obj
+    cmd = [nvcc()] + NVCC_FLAGS + ["-MD", "-MF", deps, "-c", "-o", obj + ".tmp.o", source]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(obj + ".tmp.o", obj)
+    return obj
 
 
 ENGINE_LIB = os.path.join(HERE, "libb2d_engine.so")
@@ -62,7 +84,10 @@ def build_host(force: bool = False, verbose: bool = False) -> None:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if force or not up_to_date():
-        cmd = [nvcc()] + NVCC_FLAGS + ["-o", LIB + ".tmp"] + SOURCES
+        os.makedirs(OBJECTS, exist_ok=True)
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            objects = list(pool.map(lambda source: compile_object(source, force, verbose), SOURCES))
+        cmd = [nvcc()] + NVCC_FLAGS + ["-shared", "-o", LIB + ".tmp"] + objects
         if verbose:
             print(" ".join(cmd))
         subprocess.run(cmd, check=True)

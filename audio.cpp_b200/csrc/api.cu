@@ -18,6 +18,8 @@
 #include <vector>
 
 #include "../../include/b200diff.h"
+#include "host.cuh"
+#include "serve.h"
 #include "attention_tc.cuh"
 #include "dit_kernels.cuh"
 #include "sa3_kernels.cuh"
@@ -31,27 +33,6 @@
 using namespace b2d;
 
 namespace {
-
-// ------------------------------------------------------------ error plumbing
-struct Fail {
-    b2d_status code;
-    std::string msg;
-};
-
-[[noreturn]] void fail(b2d_status code, const char* fmt, ...) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    throw Fail{code, buf};
-}
-
-#define CK(call)                                                                                   \
-    do {                                                                                           \
-        cudaError_t e_ = (call);                                                                   \
-        if (e_ != cudaSuccess) fail(B2D_ECUDA, "%s failed: %s", #call, cudaGetErrorString(e_));    \
-    } while (0)
 
 // ----------------------------------------------------------- device buffers
 struct DevBuf {
@@ -85,82 +66,6 @@ struct DevBuf {
     template <typename T>
     T* as() const { return static_cast<T*>(p); }
 };
-
-// ------------------------------------------------------ kernel launches
-// Launches inside a PdlScope carry the programmatic-stream-serialization attribute: the next kernel may start
-// its prologue (and its constant-weight loads) while this one finishes; every kernel launched this way calls
-// pdl_wait before touching data of its predecessors.  Per host thread, so concurrent contexts do not interact.
-thread_local bool tl_pdl = false;
-
-struct PdlScope {
-    bool prev;
-    PdlScope() : prev(tl_pdl) { tl_pdl = true; }
-    ~PdlScope() { tl_pdl = prev; }
-};
-
-template <typename... KArgs, typename... Args>
-void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster_x,
-              Args&&... args) {
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    if (cluster_x > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = unsigned(cluster_x);
-        attr[n].val.clusterDim.y = 1;
-        attr[n].val.clusterDim.z = 1;
-        ++n;
-    }
-    if (tl_pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = unsigned(n);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-    if (e != cudaSuccess) fail(B2D_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
-}
-
-// ---------------------------------------------------------- TMA descriptors
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-std::mutex g_host_mutex;  // guards the process-wide lookups below
-
-EncodeTiledFn encode_fn() {
-    static std::atomic<EncodeTiledFn> fn{nullptr};
-    EncodeTiledFn f = fn.load(std::memory_order_acquire);
-    if (!f) {
-        std::lock_guard<std::mutex> lock(g_host_mutex);
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
-        if (q != cudaDriverEntryPointSuccess || !p) fail(B2D_ECUDA, "cuTensorMapEncodeTiled unavailable");
-        f = reinterpret_cast<EncodeTiledFn>(p);
-        fn.store(f, std::memory_order_release);
-    }
-    return f;
-}
-
-// A kernel's dynamic shared-memory limit is an attribute of the function in the CURRENT device's context, so it
-// is set once per (kernel, device): a second context on another device in the same process sets its own.
-template <typename K>
-void set_smem_limit(K* kernel, int bytes) {
-    static std::set<std::pair<const void*, int>> done;
-    int dev = 0;
-    CK(cudaGetDevice(&dev));
-    const auto key = std::make_pair(reinterpret_cast<const void*>(kernel), dev);
-    std::lock_guard<std::mutex> lock(g_host_mutex);
-    if (done.count(key)) return;
-    CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done.insert(key);
-}
 
 // 2-D K-major operand [rows, k] of 16-bit elements, boxes of 64 (K) x box_rows, 128B swizzle.
 CUtensorMap make_tmap(const void* base, bool bf16, uint64_t rows, uint64_t k, uint32_t box_rows) {
@@ -479,6 +384,8 @@ void check_status_word(b2d_ctx* ctx, cudaStream_t st) {
         CK(cudaMemsetAsync(ctx->status.p, 0, sizeof(int), st));
         CK(cudaStreamSynchronize(st));
         if (s == kErrNonFinite) fail(B2D_ENONFINITE, "VibeVoice diffusion sampler produced non-finite latent");
+        if (s == kErrCacheBatch)
+            fail(B2D_EINVAL, "paged cache batch names a page, rows or a context outside the call's bounds");
         fail(B2D_ETIMEOUT, "a device-side wait expired (code %d); the kernel unwound", s);
     }
 }
@@ -1666,6 +1573,52 @@ b2d_status b2d_vvlm_step_device(b2d_ctx* ctx, const float* embedding, float* log
         if (ctx->lm->pos == 0) fail(B2D_ESTATE, "VibeVoice decoder cached step before prefill");
         lm_forward<__half>(ctx, embedding, 1, logits, last_hidden, static_cast<cudaStream_t>(stream), true);
     });
+}
+
+// --------------------------------------------------------------- serving operators (serve.cu)
+static ServeDevice serve_device(const b2d_ctx* ctx) { return {ctx->num_sms, ctx->status.as<int>()}; }
+
+b2d_status b2d_kv_check(const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t heads, char* err, size_t err_len) {
+    try {
+        kv_check(cache, batch, heads);
+        return B2D_OK;
+    } catch (const Fail& e) {
+        if (err && err_len) std::snprintf(err, err_len, "%s", e.msg.c_str());
+        return e.code;
+    }
+}
+
+b2d_status b2d_kv_append(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t src_type,
+                         const void* k, const void* v, int64_t row_stride, void* stream) {
+    return guarded(ctx, [&] {
+        kv_append(serve_device(ctx), cache, batch, src_type, k, v, row_stride, static_cast<cudaStream_t>(stream));
+    });
+}
+
+b2d_status b2d_kv_gather(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t dst_type, void* k,
+                         void* v, int64_t row_stride, void* stream) {
+    return guarded(ctx, [&] {
+        kv_gather(serve_device(ctx), cache, batch, dst_type, k, v, row_stride, static_cast<cudaStream_t>(stream));
+    });
+}
+
+size_t b2d_paged_attention_workspace(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t heads) {
+    size_t bytes = 0;
+    guarded(ctx, [&] { bytes = paged_attention_workspace(serve_device(ctx), cache, batch, heads); });
+    return bytes;
+}
+
+b2d_status b2d_paged_attention(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t bf16,
+                               const void* q, int64_t q_row, void* o, int64_t o_row, int32_t heads, float scale,
+                               int32_t window, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded(ctx, [&] {
+        paged_attention(serve_device(ctx), cache, batch, bf16 != 0, q, q_row, o, o_row, heads, scale, window, workspace,
+                        workspace_bytes, static_cast<cudaStream_t>(stream));
+    });
+}
+
+b2d_status b2d_sample_tokens(b2d_ctx* ctx, const b2d_sample_request* request, void* stream) {
+    return guarded(ctx, [&] { sample_tokens(serve_device(ctx), request, static_cast<cudaStream_t>(stream)); });
 }
 
 }  // extern "C"

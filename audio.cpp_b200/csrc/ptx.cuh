@@ -22,6 +22,7 @@ enum DeviceError : int {
     kErrTimeoutMma = 2,
     kErrTimeoutEpilogue = 3,
     kErrNonFinite = 4,
+    kErrCacheBatch = 5,
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -53,6 +53,9 @@ enum {
 
 /* ggml type ids accepted in tensor views (external/ggml/include/ggml.h enum ggml_type). */
 enum { B2D_TYPE_F32 = 0, B2D_TYPE_F16 = 1, B2D_TYPE_Q8_0 = 8, B2D_TYPE_BF16 = 30 };
+/* Element types of a paged cache besides F16 / BF16: ggml's id for bare int8, and (no ggml id) 8-bit floats with 4
+ * exponent and 3 mantissa bits, largest value 448. */
+enum { B2D_TYPE_I8 = 24, B2D_TYPE_E4M3 = 256 };
 
 /* One named weight tensor as stored in GGUF / safetensors (raw bytes, host memory).
  * dims are in the reference's metadata order ([out, in] for linears).
@@ -413,6 +416,109 @@ B2D_API b2d_status b2d_vvlm_prefill_device(b2d_ctx* ctx, const float* embeddings
                                            float* last_hidden, void* stream);
 B2D_API b2d_status b2d_vvlm_step_device(b2d_ctx* ctx, const float* embedding, float* logits, float* last_hidden,
                                         void* stream);
+
+/* --------------------------------------------- serving the language model: paged cache */
+/* No counterpart in the reference, which keeps one dense cache for one sequence.  All pointers are device memory;
+ * every call below is asynchronous on `stream`, allocates nothing and can be captured into a CUDA graph.
+ *
+ * One layer's keys and values, in pages that sequences own in any order (several may share a page they only read).
+ * Element (page, head, slot, j) of K sits at k + page * page_stride + head * head_stride + slot * token_stride + j
+ * (strides in elements, multiples of 16 bytes), likewise V.  8-bit types hold code x scale, with one fp32 scale
+ * per (page, head, slot) at k_scale[(page * kv_heads + head) * page_size + slot], likewise v_scale. */
+typedef struct {
+    int32_t type;        /* B2D_TYPE_F16, B2D_TYPE_BF16, B2D_TYPE_I8 or B2D_TYPE_E4M3 */
+    int32_t page_size;   /* slots of a page: 16, 32, 64 or 128 */
+    int64_t pages;
+    int32_t kv_heads;
+    int32_t head_dim;    /* 32, 64 or 128 */
+    int64_t page_stride, head_stride, token_stride;
+    void* k;
+    void* v;
+    float* k_scale;      /* 8-bit types; else unused */
+    float* v_scale;
+} b2d_kv_cache;
+
+/* The new tokens of some sequences, rows packed one sequence after the other: sequence s has rows row_start[s] ..
+ * row_start[s + 1] - 1, and context[s] tokens with them, so its row i sits at position context[s] - n + i, in slot
+ * position % page_size of page page_table[s * table_stride + position / page_size].  A row at a negative position has
+ * no place.  Rows before the first or behind the last sequence are left as they are.
+ * The arrays are read on the device and may change between replays of a captured graph, within the bounds given
+ * here.  An index outside its bound (a page outside the cache, rows that overlap or exceed max_new or rows, a context
+ * above max_context) is not followed; b2d_sync then returns B2D_EINVAL. */
+typedef struct {
+    int32_t seqs;                /* 0 to 8192 */
+    int32_t max_new;             /* no sequence has more new rows */
+    int32_t max_context;         /* no context is longer; table_stride pages hold it */
+    int64_t rows;                /* rows of the packed buffers */
+    const int32_t* row_start;    /* [seqs + 1] */
+    const int32_t* context;      /* [seqs] */
+    const int32_t* page_table;   /* [seqs, table_stride] */
+    int64_t table_stride;
+} b2d_kv_batch;
+
+/* Host only (no context, no GPU): the checks that the calls below make of a cache, a batch and, unless heads is 0, the
+ * query heads.  err / err_len (may be NULL / 0) receive the message of a refusal. */
+B2D_API b2d_status b2d_kv_check(const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t heads, char* err,
+                                size_t err_len);
+
+/* Writes the batch's rows k, v [rows, kv_heads, head_dim] (src_type F32, F16 or BF16, row stride in elements, rows
+ * 16-byte aligned) into the cache.  16-bit caches round to nearest.  8-bit caches hold each head of each row with
+ * scale = max|x| / 127 (I8) or / 448 (E4M3), rounded to fp32, and codes x / scale rounded to nearest even from the
+ * exact quotient; a head whose scale would be below 2^-100 is held as zeros, one with an infinity or a NaN reads back
+ * as NaN.  A slot may be written once in a call. */
+B2D_API b2d_status b2d_kv_append(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t src_type,
+                                 const void* k, const void* v, int64_t row_stride, void* stream);
+
+/* Reads the batch's rows back, as the values they stand for (code x scale in fp32, rounded once to dst_type F32, F16
+ * or BF16), into k, v laid out as b2d_kv_append takes them.  A row without a place reads as zeros.  A batch whose
+ * sequences have as many new rows as context reads whole contexts. */
+B2D_API b2d_status b2d_kv_gather(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t dst_type,
+                                 void* k, void* v, int64_t row_stride, void* stream);
+
+/* Bytes of workspace b2d_paged_attention needs for batches of these bounds (seqs, max_new, max_context, rows; the
+ * arrays are not read).  0 when an argument is refused (the message is b2d_last_error's). */
+B2D_API size_t b2d_paged_attention_workspace(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch,
+                                             int32_t heads);
+
+/* Causal attention of the batch's rows over the cache (their own keys and values already appended): head h of the row
+ * at position p reads kv head h / (heads / kv_heads) and
+ *   o = sum_j softmax_j(scale q . k_j) v_j  over the positions j <= p, with window > 0 only those above p - window.
+ * q, o: [rows, heads, head_dim] fp16 (bf16 = 0) or bf16 (bf16 = 1), row strides q_row / o_row in elements, 16-byte
+ * aligned; a 16-bit cache has the queries' type.  heads is 1 to 128 times kv_heads.  A row that sees no key gives
+ * zeros.  Keys and values at the positions of a context that a new row may see must be finite (what lies behind a
+ * context, in its last page, may be anything).  Scores, softmax sums and the output's sums are fp32; probabilities,
+ * and the values of an 8-bit cache, enter the second product rounded to the queries' type.  The same batch gives the same bits whenever it runs.
+ * workspace: 16-byte aligned, contents neither read nor kept; calls that may overlap (two streams, two graphs) need
+ * one each. */
+B2D_API b2d_status b2d_paged_attention(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t bf16,
+                                       const void* q, int64_t q_row, void* o, int64_t o_row, int32_t heads, float scale,
+                                       int32_t window, void* workspace, size_t workspace_bytes, void* stream);
+
+/* --------------------------------------------------- serving the language model: sampling */
+/* The next token of each row of logits (the reference samples on the host, src/framework/sampling).  With m the
+ * row's largest logit and w_i = exp((x_i - m) / temperature), entries ordered by (logit descending, index ascending):
+ *   top_k > 0 keeps the first top_k; top_p < 1 keeps an entry while the mass before it is below top_p times the mass
+ *   top-k left (the best entry always stays); min_p > 0 keeps those with w_i >= min(min_p, 1);
+ *   the token is the first index whose running sum of kept weights, in index order, exceeds uniform times their sum.
+ * temperature <= 0 takes the best entry.  A NaN logit counts as -infinity, +infinity as certain; a row without an
+ * entry above -infinity gives token -1.  Weights are computed in fp64 and summed exactly in units of 2^-45 of the
+ * largest, so the token depends on nothing but the arguments. */
+typedef struct {
+    int32_t logits_type;        /* B2D_TYPE_F32, B2D_TYPE_F16 or B2D_TYPE_BF16 */
+    int64_t rows, vocab;        /* vocab 1 to 262144 */
+    int64_t row_stride;         /* elements */
+    const void* logits;         /* [rows, vocab] */
+    const float* temperature;   /* [rows] */
+    const int32_t* top_k;       /* [rows], or NULL: off.  <= 0 or >= vocab: off for the row */
+    const float* top_p;         /* [rows], or NULL: off */
+    const float* min_p;         /* [rows], or NULL: off */
+    const float* uniform;       /* [rows], in [0, 1); values outside are brought to its ends */
+    int32_t* tokens;            /* [rows] out */
+    float* probs;               /* [rows] out, or NULL: w_token / sum of kept w (1 for the best entry at temperature <= 0,
+                                 * 0 for token -1) */
+} b2d_sample_request;
+
+B2D_API b2d_status b2d_sample_tokens(b2d_ctx* ctx, const b2d_sample_request* request, void* stream);
 
 /* ------------------------------------------------------ kernel-level entries */
 /* Q8_0 rows (GGUF bytes, dev) -> fp32 (dev), bit-exact with dequantize_row_q8_0

@@ -1,0 +1,83 @@
+"""CPU tests of the serving operators' argument checks (the paged cache, its batches, attention heads) through
+b2d_kv_check and the Python layer: what a call would refuse is refused before any device work."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+def _cache(b2d, dtype=torch.float16, pages=4, heads=2, page=16, dim=64, scales=True):
+    k = torch.zeros(pages, heads, page, dim).to(dtype)
+    s = torch.zeros(pages, heads, page) if scales else None
+    return b2d.PagedCache(k, k.clone(), s, s.clone() if scales else None)
+
+
+def _batch(b2d, seqs=2, pages=3, rows=4, max_new=2, max_context=48):
+    i = torch.int32
+    return b2d.PagedBatch(torch.zeros(seqs + 1, dtype=i), torch.zeros(seqs, dtype=i),
+                          torch.zeros(seqs, pages, dtype=i), rows, max_new, max_context)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn])
+def test_good_descriptions_pass(b2d, dtype):
+    b2d.check_paged(_cache(b2d, dtype), _batch(b2d), heads=6)
+    b2d.check_paged(_cache(b2d, dtype, dim=128, page=128), _batch(b2d, seqs=0, pages=0, rows=0, max_new=0, max_context=0))
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(type=0), "type"), (dict(type=8), "type"), (dict(page_size=24), "page_size"), (dict(page_size=256), "page_size"),
+    (dict(head_dim=80), "head_dim"), (dict(pages=0), "positive"), (dict(kv_heads=0), "positive"), (dict(k=None), "aligned"),
+    (dict(token_stride=60), "strides"), (dict(token_stride=32), "below head_dim"), (dict(page_stride=0), "strides"),
+    (dict(head_stride=-64), "strides"),
+])
+def test_bad_caches_are_refused(b2d, change, text):
+    cache, batch = _cache(b2d), _batch(b2d)
+    for name, value in change.items():
+        setattr(cache.desc, name, value)
+    with pytest.raises(b2d.B2DError, match=text):
+        b2d.check_paged(cache, batch)
+
+
+def test_eight_bit_cache_needs_scales(b2d):
+    with pytest.raises(b2d.B2DError, match="scales"):
+        _cache(b2d, torch.int8, scales=False)
+    cache = _cache(b2d, torch.int8)
+    cache.desc.v_scale = None
+    with pytest.raises(b2d.B2DError, match="scales"):
+        b2d.check_paged(cache, _batch(b2d))
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(seqs=-1), "sequences"), (dict(seqs=8193), "sequences"), (dict(rows=-1), "sizes"), (dict(rows=1 << 31), "sizes"),
+    (dict(max_new=-1), "sizes"), (dict(max_context=-1), "sizes"), (dict(max_context=49), "max_context"),
+    (dict(table_stride=2), "max_context"), (dict(context=None), "needs row_start"), (dict(page_table=None), "needs row_start"),
+])
+def test_bad_batches_are_refused(b2d, change, text):
+    cache, batch = _cache(b2d), _batch(b2d)
+    for name, value in change.items():
+        setattr(batch.desc, name, value)
+    batch.table_pages = 100  # leave the check to the library
+    with pytest.raises(b2d.B2DError, match=text):
+        b2d.check_paged(cache, batch)
+
+
+@pytest.mark.parametrize("heads", [-2, 3, 2 * 129])
+def test_bad_heads_are_refused(b2d, heads):
+    with pytest.raises(b2d.B2DError, match="heads"):
+        b2d.check_paged(_cache(b2d), _batch(b2d), heads)
+
+
+def test_python_layer_refuses_mismatched_tensors(b2d):
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
+    for v in (k.float(), k[:3], k.transpose(1, 2)):
+        with pytest.raises(b2d.B2DError):
+            b2d.PagedCache(k, v)
+    with pytest.raises(b2d.B2DError):
+        b2d.PagedCache(k.transpose(2, 3), k.transpose(2, 3))
+    i = torch.int32
+    start, context, table = torch.zeros(3, dtype=i), torch.zeros(2, dtype=i), torch.zeros(2, 3, dtype=i)
+    for bad in ((start[:2], context, table), (start, context.long(), table), (start, context, table.long()),
+                (start, context, table[:1]), (start, context, table[:1].expand(2, 3))):
+        with pytest.raises(b2d.B2DError):
+            b2d.PagedBatch(*bad, rows=2, max_new=1, max_context=16)
+    with pytest.raises(b2d.B2DError, match="max_context"):
+        b2d.check_paged(_cache(b2d), b2d.PagedBatch(start, context, table, rows=2, max_new=1, max_context=49))
