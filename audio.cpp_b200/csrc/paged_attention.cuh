@@ -11,10 +11,13 @@
 // key rows (K: lanes of a quad side by side; V: eight quads side by side) and no shared memory or ldmatrix is needed.
 // K of the next step is requested as soon as this step's S is issued, V as soon as its P V is.
 //
-// 8-bit pools: K's codes are exact in fp16, so S uses an fp16 MMA on the bare codes and the key's scale multiplies
-// the finished score; bf16 queries are brought to fp16 by a power of two per row that makes their largest entry lie
-// in [1, 2) (entries below 2^-14 of it lose bits far under the bf16 rounding of the others).  V is expanded to
-// 16 bits as round(code x scale), one rounding of the kind the 16-bit cache would hold.  P is rounded to 16 bits.
+// 8-bit pools: codes are exact in fp16, so both products run on bare codes in fp16 and nothing is rounded but P.  The
+// key's scale multiplies the finished score; bf16 queries are brought to fp16 by a power of two per row that makes
+// their largest entry lie in [1, 2) (entries below 2^-14 of it lose bits far under the bf16 rounding of the others).
+// The value's scale multiplies the probability, t = p vs, before it is rounded to fp16; the running maximum is that
+// of s + log2 vs, so the largest t of a row is near 1 whatever the scales are and what fp16 flushes is below 2^-24
+// of it.  (Expanding V to round(code x scale) instead doubled the error against 64 bits, 0.0029 to 0.0017 of the
+// output at bf16, and took 3.75 instructions an element in place of 1.5.)
 //
 // The keys of all units form one list of 64-key tiles, cut into equal runs, one per CTA: ragged batches load every
 // SM alike whatever the lengths.  A run that holds only part of a unit leaves (O, m, l) in the workspace and
@@ -137,22 +140,6 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
             : "r"(w));
     }
 }
-// Four codes of a word as fp32 values (exact).
-template <int POOL>
-__device__ __forceinline__ void codes_to_f32(uint32_t w, float (&x)[4]) {
-    if constexpr (POOL == kPoolI8) {
-        const uint32_t u = w ^ 0x80808080u;  // 2^23 + (code + 128), minus 2^23 + 128
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
-    } else {
-        uint32_t lo, hi;
-        codes_to_f16<POOL>(w, lo, hi);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-    }
-}
-
 // W words of a row, in pieces of min(W, 4) words that lie `step` bytes apart.
 template <int W>
 __device__ __forceinline__ void load_words(const uint8_t* p, int step, uint32_t (&w)[W]) {
@@ -179,7 +166,8 @@ struct PagedShape {
     static constexpr int kVw = HD / 8 * kElem / 4;  // words of a value a lane holds for P V (eight quads share it)
     static constexpr int kKPiece = (kKw < 4 ? kKw : 4) * 4;  // bytes of one load
     static constexpr int kVPiece = (kVw < 4 ? kVw : 4) * 4;
-    static constexpr int kMinBlocks = kWide ? 3 : 4;
+    // CTAs an SM holds: what the registers allow without spilling (the O accumulators of 16 rows of 128 take 64)
+    static constexpr int kMinBlocks = (kWide ? 3 : 4) - (HD == 128 && NT == 2 ? 1 : 0);
     static constexpr size_t kSmem = size_t(kPaWarps) * kRows * (HD + 2) * 4;
 };
 
@@ -189,6 +177,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
     using Sh = PagedShape<CT, POOL, HD, NT>;
     constexpr bool kWide = Sh::kWide;
     constexpr int ROWS = Sh::kRows, KW = Sh::kKw, VW = Sh::kVw, MT = HD / 16;
+    using MT16 = typename std::conditional<kWide, CT, __half>::type;  // the products' 16-bit type
     extern __shared__ float pa_sm[];  // [warp][row][HD] O, then [warp][row] (m, l)
     __shared__ int64_t red[kPaWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -308,7 +297,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
         step += (warp - step) & (kPaWarps - 1);
         const int step_end = min((u.key0 + k1) * kPaWarps, (any_hi >> 4) + 1);
         uint32_t kr[2][KW], vr[4][VW];
-        float ksc[2], vsc[4];
+        float ksc[2], vsc[2];
         const int* table = a.b.table + int64_t(seq) * a.b.table_stride;
         auto fetch_page = [&](int st) -> int {
             return st < step_end ? __ldg(table + ((st << 4) >> a.kv.page_shift)) : 0;
@@ -337,11 +326,9 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
             load_words<VW>(base + 8 * a.kv.token_stride, 8 * Sh::kVPiece, vr[2]);
             load_words<VW>(base + 9 * a.kv.token_stride, 8 * Sh::kVPiece, vr[3]);
             if constexpr (!kWide) {
-                const float* s = a.kv.vs + scale_index(a.kv, p, head, (st << 4) + 2 * c);
+                const float* s = a.kv.vs + scale_index(a.kv, p, head, (st << 4) + g);
                 vsc[0] = __ldg(s);
-                vsc[1] = __ldg(s + 1);
-                vsc[2] = __ldg(s + 8);
-                vsc[3] = __ldg(s + 9);
+                vsc[1] = __ldg(s + 8);
             }
         };
         int page = -1, next_page = 0;
@@ -370,10 +357,9 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
                     codes_to_f16<POOL>(kr[0][ks], a0, a2);
                     codes_to_f16<POOL>(kr[1][ks], a1, a3);
                 }
-                using ST = typename std::conditional<kWide, CT, __half>::type;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                    mma_16816(s[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], ST{});
+                    mma_16816(s[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], MT16{});
             }
             const float ks0 = kWide ? 1.f : ksc[0], ks1 = kWide ? 1.f : ksc[1];
             const int this_page = page;
@@ -393,18 +379,27 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
                     if (!whole && (key < lo[nt][j] || key > hi[nt][j] || this_page < 0)) x = -INFINITY;
                     s[nt][e] = x;
                 }
-            // ---- running maximum, raised only when a score exceeds it by 2^8 (p stays below 256 otherwise)
+            // ---- running maximum, raised only when a score exceeds it by 2^8 (p, or t, stays below 256 otherwise)
+            float lv[2] = {0.f, 0.f};
+            if constexpr (!kWide) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int key = pos + g + 8 * i;
+                    if (key < any_lo || key > any_hi || this_page < 0) vsc[i] = 0.f;  // a slot no row sees
+                    lv[i] = fmaxf(__log2f(vsc[i]), -101.f);  // held scales are 0 or at least 2^-100
+                }
+            }
             bool exceed = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) exceed = exceed || s[nt][e] > m[nt][e & 1] + 8.f;
+                for (int e = 0; e < 4; ++e) exceed = exceed || s[nt][e] + lv[e >> 1] > m[nt][e & 1] + 8.f;
             if (__any_sync(0xffffffffu, exceed)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float x = fmaxf(s[nt][j], s[nt][j + 2]);
+                        float x = fmaxf(s[nt][j] + lv[0], s[nt][j + 2] + lv[1]);
 #pragma unroll
                         for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
                         x = fmaxf(x, m[nt][j]);
@@ -424,9 +419,10 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
                     const float base = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
                     p[e] = ex2_approx(s[nt][e] - base);
                     l[nt][e & 1] += p[e];
+                    if constexpr (!kWide) p[e] *= vsc[e >> 1];
                 }
-                pf[nt][0] = transpose_8x8(pack_16<CT>(p[0], p[1]));
-                pf[nt][1] = transpose_8x8(pack_16<CT>(p[2], p[3]));
+                pf[nt][0] = transpose_8x8(pack_16<MT16>(p[0], p[1]));
+                pf[nt][1] = transpose_8x8(pack_16<MT16>(p[2], p[3]));
             }
             // ---- values that no row sees (behind the context, before the window, on a bad page) count as zero: what
             // lies there may be anything, NaN included
@@ -437,7 +433,6 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
                     if (key < any_lo || key > any_hi || this_page < 0) {
 #pragma unroll
                         for (int w = 0; w < VW; ++w) vr[i][w] = 0u;
-                        vsc[i] = 0.f;
                     }
                 }
             }
@@ -450,27 +445,21 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
                     const uint32_t a2 = __byte_perm(vr[2][w], vr[3][w], 0x5410);
                     const uint32_t a3 = __byte_perm(vr[2][w], vr[3][w], 0x7632);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][w], a0, a1, a2, a3, pf[nt][0], pf[nt][1], CT{});
+                    for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][w], a0, a1, a2, a3, pf[nt][0], pf[nt][1], MT16{});
                 }
             } else {
 #pragma unroll
                 for (int w = 0; w < VW; ++w) {
-                    float x[4][4];
+                    // the same dimension of two keys side by side, then to fp16
+                    uint32_t lo0[2], lo1[2], hi0[2], hi1[2];
+                    codes_to_f16<POOL>(__byte_perm(vr[0][w], vr[1][w], 0x5140), lo0[0], lo0[1]);
+                    codes_to_f16<POOL>(__byte_perm(vr[0][w], vr[1][w], 0x7362), lo1[0], lo1[1]);
+                    codes_to_f16<POOL>(__byte_perm(vr[2][w], vr[3][w], 0x5140), hi0[0], hi0[1]);
+                    codes_to_f16<POOL>(__byte_perm(vr[2][w], vr[3][w], 0x7362), hi1[0], hi1[1]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        codes_to_f32<POOL>(vr[i][w], x[i]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[i][e] *= vsc[i];
-                    }
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const uint32_t a0 = pack_16<CT>(x[0][2 * t], x[1][2 * t]);
-                        const uint32_t a1 = pack_16<CT>(x[0][2 * t + 1], x[1][2 * t + 1]);
-                        const uint32_t a2 = pack_16<CT>(x[2][2 * t], x[3][2 * t]);
-                        const uint32_t a3 = pack_16<CT>(x[2][2 * t + 1], x[3][2 * t + 1]);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            mma_16816(o[nt][2 * w + t], a0, a1, a2, a3, pf[nt][0], pf[nt][1], CT{});
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_16816(o[nt][2 * w], lo0[0], lo0[1], hi0[0], hi0[1], pf[nt][0], pf[nt][1], MT16{});
+                        mma_16816(o[nt][2 * w + 1], lo1[0], lo1[1], hi1[0], hi1[1], pf[nt][0], pf[nt][1], MT16{});
                     }
                 }
             }

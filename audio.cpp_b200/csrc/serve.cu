@@ -183,11 +183,12 @@ namespace {
 // Rows of the stream kernel's tiles: 8 when no sequence packs more than 8 rows, else 16.
 int stream_rows(const BatchView& b, int group) { return int64_t(b.max_new) * group <= 8 ? 8 : 16; }
 
-int stream_runs_per_sm(int kind) { return kind == kPoolF16 || kind == kPoolBf16 ? 3 : 4; }
+constexpr int kMaxRunsPerSm = 4;
 
 template <typename CT, int POOL, int HD, int NT>
 void launch_stream(const PagedArgs& a, int num_sms, int row_tiles, cudaStream_t st) {
     using Sh = PagedShape<CT, POOL, HD, NT>;
+    static_assert(Sh::kMinBlocks <= kMaxRunsPerSm, "the workspace holds two slots a run");
     auto kernel = paged_stream_kernel<CT, POOL, HD, NT>;
     set_smem_limit(kernel, int(Sh::kSmem));
     const int runs = num_sms * Sh::kMinBlocks;
@@ -213,7 +214,7 @@ void launch_stream_dim(int rows, const PagedArgs& a, int num_sms, int row_tiles,
     }
 }
 
-size_t stream_slots(int kind, int num_sms) { return size_t(2) * num_sms * stream_runs_per_sm(kind); }
+size_t stream_slots(int num_sms) { return size_t(2) * num_sms * kMaxRunsPerSm; }
 
 }  // namespace
 
@@ -221,7 +222,7 @@ size_t paged_attention_workspace(const ServeDevice& dev, const b2d_kv_cache* cac
     const KvView kv = cache_view(cache);
     const BatchView b = batch_view(batch, cache, dev.status);
     const int group = check_heads(kv, heads);
-    return stream_slots(pool_kind(cache->type), dev.num_sms) * stream_rows(b, group) * (size_t(kv.head_dim) + 2) * 4;
+    return stream_slots(dev.num_sms) * stream_rows(b, group) * (size_t(kv.head_dim) + 2) * 4;
 }
 
 void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2d_kv_batch* batch, bool bf16,
@@ -251,7 +252,7 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
     a.scale_log2 = scale * 1.4426950408889634f;
     a.min_rows = 0x7fffffff;
     const int rows = stream_rows(a.b, a.group);
-    const size_t slots = stream_slots(kind, dev.num_sms);
+    const size_t slots = stream_slots(dev.num_sms);
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * rows * a.kv.head_dim);
     const int64_t packed = int64_t(std::min<int64_t>(a.b.max_new, a.b.rows)) * a.group;
