@@ -1,0 +1,580 @@
+// Attention of a chunk of new rows over the paged cache on the 5th-generation tensor cores (tcgen05 + TMEM), head_dim
+// 64 or 128.  Same contract as paged_stream_kernel (paged_attention.cuh), which keeps the sequences of few rows.
+//
+// A CTA takes two 128-row query tiles of one (sequence, kv head): the rows are (token, query head of the group) pairs
+// in that order, packed without gaps, so the heads that share a kv head share its K / V stream.  Keys come in 128-key
+// blocks.  Bound by the exponentials and the tensor pipe alike (128 x 128 scores of 128-dim heads: 1024 clocks of each
+// on an SM); two tiles alternate so that one tile's softmax runs under the other's products:
+//   warps 0-3, 4-7  softmax of tile 0 / 1, one thread = one query row = one TMEM lane.  S (fp32, TMEM) -> p = 2^(s - m)
+//                   -> P (16 bits, TMEM, over the first half of S), row sum.  m is raised only when a block's sum of p
+//                   exceeds 2^8 (no p can be above it otherwise), then the row's sum and O are scaled down.
+//   warp 8          issues, per block and tile, O += P V of the block before and S = Q K^T (P from TMEM; K K-major, V
+//                   MN-major in shared memory).  The tensor pipe runs them in order, so S may overwrite P.
+//   16-bit caches:  warp 9 loads K / V pages with TMA, one box per page and 64-dim panel (128-byte swizzle)
+//   8-bit caches:   warps 9-12 read the codes and write them as fp16 (exact) in the same layout; key scales multiply
+//                   the scores and value scales the probabilities, as in paged_stream_kernel
+// K and V have a ring of two blocks each.  TMEM (512 columns): S_t (and P_t) at 128 t, O_t at 256 + 128 t.
+// Few units are spread over more CTAs by cutting the key range into `splits`; paged_join_kernel joins the parts.
+#pragma once
+
+#include "paged_attention.cuh"
+
+namespace b2d {
+
+constexpr int kPtStages = 2;
+constexpr int kPtScaleSlots = 4;
+
+struct PagedTcArgs {
+    PagedArgs a;
+    int splits;
+    int pairs;       // bound on the tile pairs of all sequences: grid.x
+    float* part_o;   // [split][pair][kv head][256][head_dim]
+    float2* part_ml; // [split][pair][kv head][256]
+};
+
+template <int POOL, int HD>
+struct PagedTcShape {
+    static constexpr bool kWide = POOL == kPoolF16 || POOL == kPoolBf16;
+    static constexpr int kThreads = kWide ? 320 : 416;
+    static constexpr uint32_t kPanel = 128 * 64 * 2;             // 128 rows of 64 dims
+    static constexpr uint32_t kTile = kPanel * (HD / 64);
+    static constexpr uint32_t kK = 2 * kTile;                    // after the two Q tiles
+    static constexpr uint32_t kV = kK + kPtStages * kTile;
+    static constexpr uint32_t kScale = kV + kPtStages * kTile;   // [slot][key scale | value scale | its log2][128]
+    static constexpr uint32_t kBar = kScale + (kWide ? 0u : kPtScaleSlots * 3u * 128u * 4u);
+    // at least half of an SM's: two CTAs must not share an SM, each takes all of its TMEM
+    static constexpr uint32_t kNeed = kBar + 256 + 1024;
+    static constexpr uint32_t kSmem = kNeed > 120u * 1024u ? kNeed : 120u * 1024u;
+};
+
+// The tile pair `pair` of the list over all sequences that this kernel takes (those of more than min_rows packed rows; last
+// tiles first, they see the most keys): sequence, its span, the pair's first row.  False behind the last.
+struct PairPlace {
+    int seq, row0;
+    SeqSpan s;
+};
+__device__ __forceinline__ bool find_pair(const PagedArgs& a, int pair, PairPlace& at, bool report) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int s0 = 0; s0 < a.b.seqs; s0 += 32) {
+        const int s = s0 + lane;
+        SeqSpan v{0, 0, 0};
+        int n = 0;
+        if (s < a.b.seqs) {
+            v = seq_span(a.b, s, report);
+            const int rows = v.n * a.group;
+            n = rows > a.min_rows ? (rows + 255) / 256 : 0;
+        }
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > pair);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            at.seq = s0 + l;
+            at.s.first = __shfl_sync(0xffffffffu, v.first, l);
+            at.s.n = __shfl_sync(0xffffffffu, v.n, l);
+            at.s.context = __shfl_sync(0xffffffffu, v.context, l);
+            const int tiles = __shfl_sync(0xffffffffu, n, l);
+            const int start = before + __shfl_sync(0xffffffffu, upto, l) - tiles;
+            at.row0 = (tiles - 1 - (pair - start)) * 256;
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
+// A bounded wait of a whole warp: all lanes get the same answer, so a warp that gives up does so together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status, code)) != 0;
+}
+
+template <typename CT, int POOL, int HD>
+__global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
+    paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const PagedTcArgs ta) {
+    using Sh = PagedTcShape<POOL, HD>;
+    constexpr bool kWide = Sh::kWide;
+    using MT16 = typename std::conditional<kWide, CT, __half>::type;  // the products' 16-bit type
+    const PagedArgs& a = ta.a;
+    extern __shared__ uint8_t pt_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::kBar);
+    uint64_t* q_full = bars;                       // [tile]
+    uint64_t* k_full = bars + 2;                   // [stage]
+    uint64_t* k_empty = k_full + kPtStages;
+    uint64_t* v_full = k_empty + kPtStages;
+    uint64_t* v_empty = v_full + kPtStages;
+    uint64_t* s_full = v_empty + kPtStages;        // [tile]
+    uint64_t* p_full = s_full + 2;                 // [tile]
+    uint64_t* o_full = p_full + 2;                 // [tile]
+    uint64_t* v_tail = o_full + 2;
+    uint64_t* scale_full = v_tail + 1;             // [slot]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scale_full + kPtScaleSlots);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    PairPlace at;
+    if (!find_pair(a, int(blockIdx.x), at, blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && warp == 0)) return;
+    const int head = int(blockIdx.y), split = int(blockIdx.z);
+    const int seq_rows = at.s.n * a.group;
+    const int p_base = at.s.context - at.s.n;  // position of the sequence's first new token
+
+    // key blocks each tile sees, cut to this split's share of the pair's range
+    int lo[2], hi[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int r0 = at.row0 + t * 128, r1 = min(r0 + 128, seq_rows) - 1;
+        lo[t] = 0;
+        hi[t] = 0;
+        if (r0 <= r1) {
+            const int p0 = p_base + r0 / a.group, p1 = p_base + r1 / a.group;
+            if (p1 >= 0) {
+                lo[t] = a.window > 0 ? max(0, p0 - a.window + 1) >> 7 : 0;
+                hi[t] = (p1 >> 7) + 1;
+            }
+        }
+    }
+    int jb = lo[0], je = hi[0];
+    if (hi[1] > lo[1]) {
+        if (je > jb) jb = min(jb, lo[1]), je = max(je, hi[1]);
+        else jb = lo[1], je = hi[1];
+    }
+    if (ta.splits > 1) {
+        const int n = je - jb, b0 = jb;
+        jb = b0 + int(int64_t(n) * split / ta.splits);
+        je = b0 + int(int64_t(n) * (split + 1) / ta.splits);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        lo[t] = max(lo[t], jb);
+        hi[t] = min(hi[t], je);
+    }
+
+    if (threadIdx.x == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_full[t], 4);
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 4);
+            mbar_init(&o_full[t], 1);
+        }
+        for (int s = 0; s < kPtStages; ++s) {
+            mbar_init(&k_full[s], kWide ? 1 : 4);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], kWide ? 1 : 4);
+            mbar_init(&v_empty[s], 1);
+        }
+        mbar_init(v_tail, 1);
+        for (int s = 0; s < kPtScaleSlots; ++s) mbar_init(&scale_full[s], 4);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int* table = a.b.table + int64_t(at.seq) * a.b.table_stride;
+
+    if (warp < 8) {
+        // ------------------------------------------------------------------------------------ softmax
+        const int t = warp >> 2, wq = warp & 3, row = wq * 32 + lane;
+        const int r = at.row0 + t * 128 + row;
+        const bool live = r < seq_rows;
+        const int token = live ? r / a.group : 0, hq = head * a.group + (live ? r % a.group : 0);
+        float rf = kWide ? a.scale_log2 : 1.f;  // what a raw score is multiplied by
+        {
+            // this row of Q into its tile (128-byte swizzle); for 8-bit caches as fp16, scaled by a power of two
+            uint4 w[HD / 8];
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const CT*>(a.q) +
+                                                              int64_t(at.s.first + token) * a.q_row + int64_t(hq) * HD);
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) w[c] = live ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (!kWide && std::is_same<CT, __nv_bfloat16>::value) {
+                uint32_t* u = reinterpret_cast<uint32_t*>(w);
+                float big = 0.f;
+#pragma unroll
+                for (int i = 0; i < HD / 2; ++i) {
+                    big = fmaxf(big, fabsf(__uint_as_float(u[i] << 16)));
+                    big = fmaxf(big, fabsf(__uint_as_float(u[i] & 0xffff0000u)));
+                }
+                const int ex = min(max(int(__float_as_uint(big) >> 23) - 127, -125), 125);
+                const float f = big > 0.f ? __uint_as_float(uint32_t(127 - ex) << 23) : 1.f;
+                rf = big > 0.f ? __uint_as_float(uint32_t(127 + ex) << 23) : 1.f;
+#pragma unroll
+                for (int i = 0; i < HD / 2; ++i)
+                    u[i] = pack_16<__half>(__uint_as_float(u[i] << 16) * f, __uint_as_float(u[i] & 0xffff0000u) * f);
+            }
+            uint8_t* dst = smem + t * Sh::kTile + row * 128;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c)
+                *reinterpret_cast<uint4*>(dst + (c >> 3) * Sh::kPanel + (((c & 7) ^ (row & 7)) << 4)) = w[c];
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[t]);
+
+        const uint32_t lane_off = uint32_t(wq * 32) << 16;
+        const uint32_t tS = tmem + lane_off + uint32_t(t * 128), tO = tmem + lane_off + 256u + uint32_t(t * 128);
+        const int p_row = live ? p_base + token : 0x3fffffff;  // a lane without a row sees every key (of a zero query)
+        const int key_hi = p_row, key_lo = live && a.window > 0 ? p_row - a.window + 1 : 0;
+        // keys that every row of the warp sees
+        const int all_hi = __reduce_min_sync(0xffffffffu, key_hi), all_lo = __reduce_max_sync(0xffffffffu, key_lo);
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = lo[t]; j < hi[t]; ++j) {
+            const int i = j - lo[t], key0 = j << 7;
+            const bool whole = key0 >= all_lo && key0 + 127 <= all_hi;
+            const int slot = (j - jb) % kPtScaleSlots;
+            const float* ks = reinterpret_cast<const float*>(smem + Sh::kScale) + slot * 384;
+            if constexpr (!kWide) {
+                if (!(ok = warp_wait(&scale_full[slot], uint32_t((j - jb) / kPtScaleSlots) & 1u, abort_flag, a.b.status,
+                                     kErrTimeoutEpilogue)))
+                    break;
+            }
+            if (!(ok = warp_wait(&s_full[t], uint32_t(i) & 1u, abort_flag, a.b.status, kErrTimeoutEpilogue))) break;
+            tc_fence_after();
+            // 32 of the row's scores (times rf they are in log2 units), -inf where the row does not see the key
+            auto load_chunk = [&](int c, float (&x)[32]) {
+                tmem_ld_32x32b_x32(tS + uint32_t(c * 32), x);
+                tmem_ld_wait();
+                if constexpr (!kWide) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4*>(ks + c * 32 + e);
+                        x[e] *= k4.x, x[e + 1] *= k4.y, x[e + 2] *= k4.z, x[e + 3] *= k4.w;
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int key = key0 + c * 32 + e;
+                        if (key < key_lo || key > key_hi) x[e] = -INFINITY;
+                    }
+                }
+            };
+            auto row_max = [&]() -> float {
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x[32];
+                    load_chunk(c, x);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float y = x[e] * rf;
+                        mx[e & 3] = fmaxf(mx[e & 3], kWide ? y : y + ks[256 + c * 32 + e]);
+                    }
+                }
+                return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            };
+            uint32_t p[64];
+            // P of the row (packed) and its sums: of p, and of what is rounded to 16 bits (t = p x value scale)
+            auto exp_pass = [&](float& sum_t) -> float {
+                const float base = m == -INFINITY ? 0.f : -m;
+                float sp[4] = {0.f, 0.f, 0.f, 0.f}, st[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x[32];
+                    load_chunk(c, x);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        x[e] = ex2_approx(fmaf(x[e], rf, base));
+                        sp[e & 3] += x[e];
+                    }
+                    if constexpr (!kWide) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 v4 = *reinterpret_cast<const float4*>(ks + 128 + c * 32 + e);
+                            x[e] *= v4.x, x[e + 1] *= v4.y, x[e + 2] *= v4.z, x[e + 3] *= v4.w;
+                            st[0] += x[e], st[1] += x[e + 1], st[2] += x[e + 2], st[3] += x[e + 3];
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) p[c * 16 + e] = pack_16<MT16>(x[2 * e], x[2 * e + 1]);
+                }
+                const float sum = (sp[0] + sp[1]) + (sp[2] + sp[3]);
+                sum_t = kWide ? sum : (st[0] + st[1]) + (st[2] + st[3]);
+                return sum;
+            };
+            float sum = 0.f, sum_t = 0.f;
+            bool raise = m == -INFINITY;
+            if (!__any_sync(0xffffffffu, raise)) {
+                sum = exp_pass(sum_t);
+                raise = sum_t > 256.f;
+            }
+            if (__any_sync(0xffffffffu, raise)) {
+                const float top = fmaxf(row_max(), m);
+                const float f = !raise || m == top ? 1.f : ex2_approx(m - top);
+                if (raise) m = top;
+                l *= f;
+                if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+                    // S of this block is complete, and with it P V of the block before: O may be changed
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        float o[32];
+                        tmem_ld_32x32b_x32(tO + uint32_t(c * 32), o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= f;
+                        tmem_st_32x32b_x32(tO + uint32_t(c * 32), o);
+                    }
+                }
+                sum = exp_pass(sum_t);
+            }
+            l += sum;
+            tmem_st_32x32b_x32(tS, reinterpret_cast<const float(&)[32]>(p[0]));
+            tmem_st_32x32b_x32(tS + 32u, reinterpret_cast<const float(&)[32]>(p[32]));
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[t]);
+        }
+        const bool any = hi[t] > lo[t];
+        if (any && ok) ok = warp_wait(&o_full[t], 0u, abort_flag, a.b.status, kErrTimeoutEpilogue);
+        if (ok) {
+            tc_fence_after();
+            const bool part = ta.splits > 1;
+            const float inv = part ? 1.f : (l == 0.f ? 0.f : 1.f / l);  // no visible key: zeros
+            const int64_t slot = ((int64_t(split) * ta.pairs + blockIdx.x) * a.kv.kv_heads + head) * 256 + t * 128 + row;
+            if (part && live) ta.part_ml[slot] = make_float2(m, l);
+            CT* dst = static_cast<CT*>(a.o) + int64_t(at.s.first + token) * a.o_row + int64_t(hq) * HD;
+            if (any || !part) {
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    float o[32];
+                    if (any) {
+                        tmem_ld_32x32b_x32(tO + uint32_t(c * 32), o);
+                        tmem_ld_wait();
+                    }
+                    if (!live) continue;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        float y[8];
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) y[d] = any && l != 0.f ? o[e + d] * inv : 0.f;
+                        if (part) store8(ta.part_o + slot * HD + c * 32 + e, y);
+                        else store8(dst + c * 32 + e, y);
+                    }
+                }
+            }
+        }
+    } else if (warp == 8) {
+        // ------------------------------------------------------------------------------------ products
+        if (lane == 0) {
+            constexpr uint32_t kFmt = std::is_same<MT16, __nv_bfloat16>::value ? 1u : 0u;
+            constexpr uint32_t idS = idesc_f16(kFmt, 128, 128);
+            constexpr uint32_t idO = idesc_f16(kFmt, 128, HD) | (1u << 16);  // B (V) MN-major
+            bool ok = mbar_wait(&q_full[0], 0u, abort_flag, a.b.status, kErrTimeoutMma) &&
+                      mbar_wait(&q_full[1], 0u, abort_flag, a.b.status, kErrTimeoutMma);
+            for (int j = jb; ok && j <= je && je > jb; ++j) {
+                const int i = j - jb, s = i % kPtStages, sv = (i - 1) % kPtStages;
+                for (int t = 0; ok && t < 2; ++t) {
+                    const uint32_t dS = tmem + uint32_t(t * 128), dO = tmem + 256u + uint32_t(t * 128);
+                    if (j > jb && j - 1 >= lo[t] && j - 1 < hi[t]) {
+                        if (!(ok = mbar_wait(&v_full[sv], uint32_t((i - 1) / kPtStages) & 1u, abort_flag, a.b.status,
+                                             kErrTimeoutMma) &&
+                                   mbar_wait(&p_full[t], uint32_t(j - 1 - lo[t]) & 1u, abort_flag, a.b.status,
+                                             kErrTimeoutMma)))
+                            break;
+                        tc_fence_after();
+                        const uint64_t vd = HD == 64 ? smem_desc_sw128(smem + Sh::kV + sv * Sh::kTile)
+                                                     : smem_desc_sw128_mn(smem + Sh::kV + sv * Sh::kTile, Sh::kPanel);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)  // 16 keys = 8 columns of P = 16 rows of V (2 KB)
+                            mma_f16_ts(dO, dS + uint32_t(8 * k), vd + uint64_t(128 * k), idO,
+                                       (j - 1 > lo[t] || k > 0) ? 1u : 0u);
+                        if (j == hi[t]) mma_commit(&o_full[t]);
+                    }
+                    if (j >= lo[t] && j < hi[t]) {
+                        if (!(ok = mbar_wait(&k_full[s], uint32_t(i / kPtStages) & 1u, abort_flag, a.b.status,
+                                             kErrTimeoutMma)))
+                            break;
+                        tc_fence_after();
+                        const uint64_t qd = smem_desc_sw128(smem + t * Sh::kTile);
+                        const uint64_t kd = smem_desc_sw128(smem + Sh::kK + s * Sh::kTile);
+#pragma unroll
+                        for (int k = 0; k < HD / 16; ++k) {
+                            const uint64_t off = uint64_t((k >> 2) * (Sh::kPanel >> 4) + 2 * (k & 3));
+                            mma_f16_ss(dS, qd + off, kd + off, idS, k > 0 ? 1u : 0u);
+                        }
+                        mma_commit(&s_full[t]);
+                    }
+                }
+                if (!ok) break;
+                if (j < je) mma_commit(&k_empty[s]);
+                if (j > jb) mma_commit(&v_empty[sv]);
+            }
+        }
+    } else if constexpr (kWide) {
+        // ------------------------------------------------------------------------------------ pages by TMA
+        const int per_page = 1 << a.kv.page_shift, boxes = 128 >> a.kv.page_shift;  // pages of a block
+        bool ok = true;
+        for (int j = jb; ok && j < je; ++j) {
+            const int i = j - jb, s = i % kPtStages;
+            const uint32_t ph = uint32_t(i / kPtStages) & 1u;
+            // lane b < boxes: its page; outside the context or the pool one that TMA fills with zeros
+            int page = int(a.kv.pages);
+            const int pos = (j << 7) + lane * per_page;
+            if (lane < boxes && pos < at.s.context) {
+                page = __ldg(table + (pos >> a.kv.page_shift));
+                if (page < 0 || page >= a.kv.pages) {
+                    batch_error(a.b);
+                    page = int(a.kv.pages);
+                }
+            }
+            if (!(ok = warp_wait(&k_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
+            if (lane == 0) mbar_arrive_expect_tx(&k_full[s], Sh::kTile);
+            __syncwarp();
+            if (lane < boxes)
+#pragma unroll
+                for (int d = 0; d < HD / 64; ++d)
+                    tma_load_4d(smem + Sh::kK + s * Sh::kTile + d * Sh::kPanel + lane * per_page * 128, &tmK, &k_full[s],
+                                d * 64, 0, head, page);
+            if (!(ok = warp_wait(&v_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
+            // the block that holds the context's end: rows behind it are zeroed before they are announced (they may hold
+            // anything, and P = 0 times NaN is NaN)
+            const int used = at.s.context - (j << 7);
+            const bool tail = used < 128 && (used & (per_page - 1)) != 0;
+            uint64_t* bar = tail ? v_tail : &v_full[s];
+            if (lane == 0) mbar_arrive_expect_tx(bar, Sh::kTile);
+            __syncwarp();
+            if (lane < boxes)
+#pragma unroll
+                for (int d = 0; d < HD / 64; ++d)
+                    tma_load_4d(smem + Sh::kV + s * Sh::kTile + d * Sh::kPanel + lane * per_page * 128, &tmV, bar, d * 64, 0,
+                                head, page);
+            if (tail) {  // the last block of the range: v_tail is used once
+                if (!(ok = warp_wait(v_tail, 0u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
+                const int end = (used + per_page - 1) & ~(per_page - 1);
+                for (int b = used * 8 + lane; b < end * 8; b += 32)
+#pragma unroll
+                    for (int d = 0; d < HD / 64; ++d)
+                        *reinterpret_cast<uint4*>(smem + Sh::kV + s * Sh::kTile + d * Sh::kPanel + b * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[s]);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------------------------ codes to fp16
+        constexpr int kPieces = HD / 16;             // 16-byte pieces of a row of codes
+        constexpr int kEach = 128 * kPieces / 128;   // of a tile, per thread
+        constexpr int kRowStep = 128 / kPieces;      // 16 (head_dim 128) or 32 rows between a thread's pieces
+        const int ct = threadIdx.x - 288, piece = ct % kPieces, row0 = ct / kPieces;
+        auto page_at = [&](int pos) -> int {
+            if (pos >= at.s.context) return -1;
+            const int page = __ldg(table + (pos >> a.kv.page_shift));
+            if (page >= 0 && page < a.kv.pages) return page;
+            batch_error(a.b);
+            return -1;
+        };
+        auto load = [&](const uint8_t* pool, int j, uint4 (&w)[kEach]) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int pos = (j << 7) + row0 + e * kRowStep;
+                const int page = page_at(pos);
+                w[e] = page < 0 ? make_uint4(0u, 0u, 0u, 0u)
+                                : __ldg(reinterpret_cast<const uint4*>(pool + slot_offset(a.kv, page, head, pos)) + piece);
+            }
+        };
+        auto store = [&](uint8_t* tile, const uint4 (&w)[kEach]) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int row = row0 + e * kRowStep;
+                uint4 h[2];
+                codes_to_f16<POOL>(w[e].x, h[0].x, h[0].y);
+                codes_to_f16<POOL>(w[e].y, h[0].z, h[0].w);
+                codes_to_f16<POOL>(w[e].z, h[1].x, h[1].y);
+                codes_to_f16<POOL>(w[e].w, h[1].z, h[1].w);
+                uint8_t* dst = tile + (piece >> 2) * Sh::kPanel + row * 128;
+                const int c = 2 * (piece & 3);
+                // the two panels' lanes store their halves in opposite order: no two on one bank
+                const int first = piece >> 2;
+                *reinterpret_cast<uint4*>(dst + (((c + first) ^ (row & 7)) << 4)) = first ? h[1] : h[0];
+                *reinterpret_cast<uint4*>(dst + (((c + 1 - first) ^ (row & 7)) << 4)) = first ? h[0] : h[1];
+            }
+        };
+        bool ok = true;
+        uint4 wk[kEach], wv[kEach];
+        if (jb < je) load(a.kv.k, jb, wk);
+        for (int j = jb; ok && j < je; ++j) {
+            const int i = j - jb, s = i % kPtStages, slot = i % kPtScaleSlots;
+            const uint32_t ph = uint32_t(i / kPtStages) & 1u;
+            load(a.kv.v, j, wv);
+            // thread = key: its scales (a key behind the context: any finite ones, its probability is 0)
+            const int pos = (j << 7) + ct;
+            const int page = page_at(pos);
+            float ks = 0.f, vs = 1.f;
+            if (page >= 0) {
+                const int64_t at_scale = scale_index(a.kv, page, head, pos);
+                ks = __ldg(a.kv.ks + at_scale);
+                vs = __ldg(a.kv.vs + at_scale);
+            }
+            if (vs < 3.944304526105059e-31f) vs = 3.944304526105059e-31f;  // 2^-101: a zero scale (zero codes), in log2's range
+            if (!(ok = warp_wait(&k_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
+            // K of two blocks ago is consumed, so the softmax of four blocks ago is done with this slot's scales
+            float* sc = reinterpret_cast<float*>(smem + Sh::kScale) + slot * 384;
+            sc[ct] = ks * a.scale_log2;
+            sc[128 + ct] = vs;
+            sc[256 + ct] = __log2f(vs);
+            store(smem + Sh::kK + s * Sh::kTile, wk);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&scale_full[slot]);
+                mbar_arrive(&k_full[s]);
+            }
+            if (j + 1 < je) load(a.kv.k, j + 1, wk);
+            if (!(ok = warp_wait(&v_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
+            store(smem + Sh::kV + s * Sh::kTile, wv);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[s]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the splits of the tensor-tile kernel: one warp per packed row.
+template <typename CT, int HD>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedTcArgs ta) {
+    const PagedArgs& a = ta.a;
+    PairPlace at;
+    if (!find_pair(a, int(blockIdx.x), at, false)) return;
+    const int head = int(blockIdx.y), lane = threadIdx.x & 31;
+    const int i = int(blockIdx.z) * 8 + (threadIdx.x >> 5), r = at.row0 + i;
+    if (r >= at.s.n * a.group) return;
+    const int64_t slot0 = (int64_t(blockIdx.x) * a.kv.kv_heads + head) * 256 + i;
+    const int64_t step = int64_t(ta.pairs) * a.kv.kv_heads * 256;
+    float m = -INFINITY, l = 0.f, x[HD / 32];
+    for (int s = 0; s < ta.splits; ++s) m = fmaxf(m, ta.part_ml[slot0 + s * step].x);
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) x[e] = 0.f;
+    for (int s = 0; s < ta.splits; ++s) {
+        const float2 ml = ta.part_ml[slot0 + s * step];
+        if (ml.y == 0.f) continue;  // a split without a visible key left no sums
+        const float f = ml.x == m ? 1.f : ex2_approx(ml.x - m);
+        l += ml.y * f;
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) x[e] += ta.part_o[(slot0 + s * step) * HD + e * 32 + lane] * f;
+    }
+    CT* out = static_cast<CT*>(a.o) + int64_t(at.s.first + r / a.group) * a.o_row +
+              int64_t(head * a.group + r % a.group) * HD;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) out[e * 32 + lane] = from_f32<CT>(l == 0.f ? 0.f : x[e] / l);
+}
+
+}  // namespace b2d

@@ -8,6 +8,7 @@
 #include "host.cuh"
 #include "kv_cache.cuh"
 #include "paged_attention.cuh"
+#include "paged_attention_tc.cuh"
 #include "sample.cuh"
 
 namespace b2d {
@@ -183,34 +184,110 @@ namespace {
 // Rows of the stream kernel's tiles: 8 when no sequence packs more than 8 rows, else 16.
 int stream_rows(const BatchView& b, int group) { return int64_t(b.max_new) * group <= 8 ? 8 : 16; }
 
+// Packed rows (tokens x heads per kv head) up to which a sequence goes through the stream kernel.  Its cost grows with
+// every tile of 16 rows that reads the keys again, the tensor-tile kernel's with every pair of 128; head_dim 32 has no
+// tensor-tile kernel.
+int stream_most_rows(int head_dim) { return head_dim == 32 ? 0x7fffffff : 16; }
+
+int64_t batch_packed_rows(const BatchView& b, int group) { return int64_t(std::min(b.max_new, b.rows)) * group; }
+
+// What the host knows of the tensor-tile kernel's grid: tile pairs of 256 packed rows, over all sequences, and into how
+// many parts the keys of one are cut so that few pairs still fill the SMs (at least four 128-key blocks a part).
+struct TcPlan {
+    int pairs, splits;
+};
+TcPlan tc_plan(const BatchView& b, const KvView& kv, int group, int num_sms) {
+    const int most = stream_most_rows(kv.head_dim);
+    if (batch_packed_rows(b, group) <= most) return {0, 0};
+    const int64_t packed = int64_t(b.rows) * group;
+    const int64_t pairs = packed / 256 + std::min<int64_t>(b.seqs, packed / (most + 1) + 1);
+    if (pairs > 0x7fffffff || kv.kv_heads > 65535) fail(B2D_EINVAL, "paged attention batch is too large");
+    const int64_t blocks = (int64_t(b.max_context) + 127) / 128;
+    const int64_t splits = std::min<int64_t>({num_sms / (pairs * kv.kv_heads), blocks / 4, 16});
+    return {int(pairs), int(std::max<int64_t>(1, splits))};
+}
+
 constexpr int kMaxRunsPerSm = 4;
 
+// One box = one page's slots of one head, 64 dims wide, 128-byte swizzle; pages outside the pool read as zeros.
+CUtensorMap page_tmap(const void* base, bool bf16, const b2d_kv_cache& c) {
+    CUtensorMap m;
+    const cuuint64_t dims[4] = {cuuint64_t(c.head_dim), cuuint64_t(c.page_size), cuuint64_t(c.kv_heads), cuuint64_t(c.pages)};
+    const cuuint64_t strides[3] = {cuuint64_t(c.token_stride) * 2, cuuint64_t(c.head_stride) * 2,
+                                   cuuint64_t(c.page_stride) * 2};
+    const cuuint32_t box[4] = {64, cuuint32_t(c.page_size), 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = encode_fn()(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fail(B2D_ECUDA, "cuTensorMapEncodeTiled (paged cache) failed (%d)", int(r));
+    return m;
+}
+
+struct AttentionLaunch {
+    PagedArgs a;
+    const b2d_kv_cache* cache;
+    TcPlan tc;
+    void* tc_workspace;
+    int rows, row_tiles;  // of the stream kernel; row_tiles 0: no sequence can be its
+    int num_sms;
+    cudaStream_t st;
+};
+
 template <typename CT, int POOL, int HD, int NT>
-void launch_stream(const PagedArgs& a, int num_sms, int row_tiles, cudaStream_t st) {
+void launch_stream(const AttentionLaunch& x) {
     using Sh = PagedShape<CT, POOL, HD, NT>;
     static_assert(Sh::kMinBlocks <= kMaxRunsPerSm, "the workspace holds two slots a run");
     auto kernel = paged_stream_kernel<CT, POOL, HD, NT>;
     set_smem_limit(kernel, int(Sh::kSmem));
-    const int runs = num_sms * Sh::kMinBlocks;
-    launch_k(kernel, dim3(unsigned(runs)), dim3(kPaWarps * 32), Sh::kSmem, st, 1, a);
-    const int64_t units = int64_t(a.b.seqs) * row_tiles * a.kv.kv_heads;
+    const int runs = x.num_sms * Sh::kMinBlocks;
+    launch_k(kernel, dim3(unsigned(runs)), dim3(kPaWarps * 32), Sh::kSmem, x.st, 1, x.a);
+    const int64_t units = int64_t(x.a.b.seqs) * x.row_tiles * x.a.kv.kv_heads;
     if (units > 0x7fffffff) fail(B2D_EINVAL, "paged attention batch is too large");
-    launch_k(paged_merge_kernel<CT, HD, Sh::kRows>, dim3(unsigned(units), unsigned(Sh::kRows)), dim3(256), 0, st, 1, a,
-             runs, row_tiles);
+    launch_k(paged_merge_kernel<CT, HD, Sh::kRows>, dim3(unsigned(units), unsigned(Sh::kRows)), dim3(256), 0, x.st, 1, x.a,
+             runs, x.row_tiles);
 }
 
 template <typename CT, int POOL, int HD>
-void launch_stream_rows(int rows, const PagedArgs& a, int num_sms, int row_tiles, cudaStream_t st) {
-    if (rows == 8) launch_stream<CT, POOL, HD, 1>(a, num_sms, row_tiles, st);
-    else launch_stream<CT, POOL, HD, 2>(a, num_sms, row_tiles, st);
+void launch_tc(const AttentionLaunch& x) {
+    using Sh = PagedTcShape<POOL, HD>;
+    auto kernel = paged_tc_kernel<CT, POOL, HD>;
+    set_smem_limit(kernel, int(Sh::kSmem));
+    CUtensorMap tk{}, tv{};
+    if (Sh::kWide) {
+        tk = page_tmap(x.cache->k, POOL == kPoolBf16, *x.cache);
+        tv = page_tmap(x.cache->v, POOL == kPoolBf16, *x.cache);
+    }
+    PagedTcArgs ta{x.a, x.tc.splits, x.tc.pairs, nullptr, nullptr};
+    const unsigned kvh = unsigned(x.a.kv.kv_heads);
+    if (x.tc.splits > 1) {
+        const size_t slots = size_t(x.tc.splits) * x.tc.pairs * kvh * 256;
+        ta.part_o = static_cast<float*>(x.tc_workspace);
+        ta.part_ml = reinterpret_cast<float2*>(ta.part_o + slots * HD);
+    }
+    launch_k(kernel, dim3(unsigned(x.tc.pairs), kvh, unsigned(x.tc.splits)), dim3(Sh::kThreads), Sh::kSmem, x.st, 1, tk, tv,
+             ta);
+    if (x.tc.splits > 1)
+        launch_k(paged_join_kernel<CT, HD>, dim3(unsigned(x.tc.pairs), kvh, 32u), dim3(256), 0, x.st, 1, ta);
+}
+
+template <typename CT, int POOL, int HD>
+void launch_attention_dim(const AttentionLaunch& x) {
+    if (x.row_tiles > 0) {
+        if (x.rows == 8) launch_stream<CT, POOL, HD, 1>(x);
+        else launch_stream<CT, POOL, HD, 2>(x);
+    }
+    if constexpr (HD != 32)
+        if (x.tc.pairs > 0) launch_tc<CT, POOL, HD>(x);
 }
 
 template <typename CT, int POOL>
-void launch_stream_dim(int rows, const PagedArgs& a, int num_sms, int row_tiles, cudaStream_t st) {
-    switch (a.kv.head_dim) {
-        case 32: return launch_stream_rows<CT, POOL, 32>(rows, a, num_sms, row_tiles, st);
-        case 64: return launch_stream_rows<CT, POOL, 64>(rows, a, num_sms, row_tiles, st);
-        default: return launch_stream_rows<CT, POOL, 128>(rows, a, num_sms, row_tiles, st);
+void launch_attention(const AttentionLaunch& x) {
+    switch (x.a.kv.head_dim) {
+        case 32: return launch_attention_dim<CT, POOL, 32>(x);
+        case 64: return launch_attention_dim<CT, POOL, 64>(x);
+        default: return launch_attention_dim<CT, POOL, 128>(x);
     }
 }
 
@@ -218,17 +295,28 @@ size_t stream_slots(int num_sms) { return size_t(2) * num_sms * kMaxRunsPerSm; }
 
 }  // namespace
 
+static size_t stream_bytes(const BatchView& b, const KvView& kv, int group, int num_sms) {
+    const size_t rows = stream_slots(num_sms) * stream_rows(b, group);
+    return (rows * (size_t(kv.head_dim) + 2) * 4 + 255) / 256 * 256;
+}
+
+static size_t attention_bytes(const BatchView& b, const KvView& kv, int group, int num_sms) {
+    const TcPlan tc = tc_plan(b, kv, group, num_sms);
+    const size_t tc_rows = tc.splits > 1 ? size_t(tc.splits) * tc.pairs * kv.kv_heads * 256 : 0;
+    return stream_bytes(b, kv, group, num_sms) + tc_rows * (size_t(kv.head_dim) + 2) * 4;
+}
+
 size_t paged_attention_workspace(const ServeDevice& dev, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int heads) {
     const KvView kv = cache_view(cache);
     const BatchView b = batch_view(batch, cache, dev.status);
-    const int group = check_heads(kv, heads);
-    return stream_slots(dev.num_sms) * stream_rows(b, group) * (size_t(kv.head_dim) + 2) * 4;
+    return attention_bytes(b, kv, check_heads(kv, heads), dev.num_sms);
 }
 
 void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2d_kv_batch* batch, bool bf16,
                      const void* q, int64_t q_row, void* o, int64_t o_row, int heads, float scale, int window,
                      void* workspace, size_t workspace_bytes, cudaStream_t st) {
-    PagedArgs a{};
+    AttentionLaunch x{};
+    PagedArgs& a = x.a;
     a.kv = cache_view(cache);
     a.b = batch_view(batch, cache, dev.status);
     a.group = check_heads(a.kv, heads);
@@ -240,7 +328,7 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
         fail(B2D_EINVAL, "paged attention rows must be 16-byte aligned device memory");
     if (q_row < int64_t(heads) * a.kv.head_dim || o_row < int64_t(heads) * a.kv.head_dim)
         fail(B2D_EINVAL, "paged attention row strides are below heads x head_dim");
-    const size_t need = paged_attention_workspace(dev, cache, batch, heads);
+    const size_t need = attention_bytes(a.b, a.kv, a.group, dev.num_sms);
     if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
         fail(B2D_EINVAL, "paged attention needs a 16-byte aligned workspace of %zu bytes", need);
     a.q = q;
@@ -250,21 +338,27 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
     a.heads = heads;
     a.window = window;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.min_rows = 0x7fffffff;
-    const int rows = stream_rows(a.b, a.group);
-    const size_t slots = stream_slots(dev.num_sms);
+    a.min_rows = stream_most_rows(a.kv.head_dim);
+    x.cache = cache;
+    x.tc = tc_plan(a.b, a.kv, a.group, dev.num_sms);
+    x.tc_workspace = static_cast<uint8_t*>(workspace) + stream_bytes(a.b, a.kv, a.group, dev.num_sms);
+    x.rows = stream_rows(a.b, a.group);
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * rows * a.kv.head_dim);
-    const int64_t packed = int64_t(std::min<int64_t>(a.b.max_new, a.b.rows)) * a.group;
-    const int row_tiles = int((packed + rows - 1) / rows);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + stream_slots(dev.num_sms) * x.rows * a.kv.head_dim);
+    // one sequence that may be long belongs to the tensor-tile kernel whatever its rows turn out to be
+    if (a.b.seqs == 1 && x.tc.pairs > 0) a.min_rows = 0;
+    const int64_t packed = std::min<int64_t>(batch_packed_rows(a.b, a.group), a.min_rows);
+    x.row_tiles = int((packed + x.rows - 1) / x.rows);
+    x.num_sms = dev.num_sms;
+    x.st = st;
     if (bf16) {
-        if (kind == kPoolBf16) launch_stream_dim<__nv_bfloat16, kPoolBf16>(rows, a, dev.num_sms, row_tiles, st);
-        else if (kind == kPoolI8) launch_stream_dim<__nv_bfloat16, kPoolI8>(rows, a, dev.num_sms, row_tiles, st);
-        else launch_stream_dim<__nv_bfloat16, kPoolE4m3>(rows, a, dev.num_sms, row_tiles, st);
+        if (kind == kPoolBf16) launch_attention<__nv_bfloat16, kPoolBf16>(x);
+        else if (kind == kPoolI8) launch_attention<__nv_bfloat16, kPoolI8>(x);
+        else launch_attention<__nv_bfloat16, kPoolE4m3>(x);
     } else {
-        if (kind == kPoolF16) launch_stream_dim<__half, kPoolF16>(rows, a, dev.num_sms, row_tiles, st);
-        else if (kind == kPoolI8) launch_stream_dim<__half, kPoolI8>(rows, a, dev.num_sms, row_tiles, st);
-        else launch_stream_dim<__half, kPoolE4m3>(rows, a, dev.num_sms, row_tiles, st);
+        if (kind == kPoolF16) launch_attention<__half, kPoolF16>(x);
+        else if (kind == kPoolI8) launch_attention<__half, kPoolI8>(x);
+        else launch_attention<__half, kPoolE4m3>(x);
     }
 }
 

@@ -5,8 +5,11 @@ Tolerances.  u is half a step of the 16-bit type (bf16 2^-9 relative to a value 
 a probability rounded to 16 bits is off by u of itself, so an output by u A with A = sum p |v| / sum p; a value of an
 8-bit cache rounded to 16 bits adds another u A; a score is an fp32 sum of head_dim products, off by at most
 (head_dim + 8) 2^-24 sum |q k| scale, which moves every probability by that much relative and the quotient by twice as
-much; exp2 and the scale's rounding add less than 2^-19 (scores here stay below 2^5); fp16 probabilities and values
-below 2^-14 are off by 2^-25 absolute instead, at most n keys of them; the output's own rounding adds u |o|."""
+much; exp2 and the scale's rounding add less than 2^-19 (scores here stay below 2^5); the output's own rounding adds
+u |o|.  Probabilities are rounded to fp16 for fp16 queries and for every 8-bit cache (t = p x value scale there, times
+integer codes).  An fp16 number below 2^-14 is off by 2^-25 absolute instead of u of itself.  The key that set the
+running maximum has t = 1, so with n keys the sum of t code is off by at most n 2^-25 max|code|, and the sum of p is at
+least 1 / (that key's value scale): the output is off by at most n 2^-25 max|code| x scale <= n 2^-25 max|v|."""
 import numpy as np
 import pytest
 
@@ -83,8 +86,10 @@ def attention_bound(o, a, ds, dtype, head_dim, eight_bit, keys, vmax):
     u = torch.finfo(dtype).eps / 2
     rel = u * (2 if eight_bit else 1) + 2.0 ** -18
     bound = a * rel + 2 * a * ((head_dim + 8) * 2.0 ** -24 * ds)[..., None] + u * o.abs()
+    if dtype == torch.float16 or eight_bit:
+        bound = bound + 2.0 ** -25 * keys * vmax
     if dtype == torch.float16:
-        bound = bound + 2.0 ** -24 + 2.0 ** -25 * keys * vmax
+        bound = bound + 2.0 ** -24  # outputs below 2^-14
     return bound + 1e-30
 
 
