@@ -5,14 +5,18 @@
 // in that order, packed without gaps, so the heads that share a kv head share its K / V stream.  Keys come in 128-key
 // blocks.  Bound by the exponentials and the tensor pipe alike (128 x 128 scores of 128-dim heads: 1024 clocks of each
 // on an SM); two tiles alternate so that one tile's softmax runs under the other's products:
-//   warps 0-3, 4-7  softmax of tile 0 / 1, one thread = one query row = one TMEM lane.  S (fp32, TMEM) -> p = 2^(s - m)
-//                   -> P (16 bits, TMEM, over the first half of S), row sum.  m is raised only when a block's sum of p
-//                   exceeds 2^8 (no p can be above it otherwise), then the row's sum and O are scaled down.
-//   warp 8          issues, per block and tile, O += P V of the block before and S = Q K^T (P from TMEM; K K-major, V
-//                   MN-major in shared memory).  The tensor pipe runs them in order, so S may overwrite P.
-//   16-bit caches:  warp 9 loads K / V pages with TMA, one box per page and 64-dim panel (128-byte swizzle)
-//   8-bit caches:   warps 9-12 read the codes and write them as fp16 (exact) in the same layout; key scales multiply
-//                   the scores and value scales the probabilities, as in paged_stream_kernel
+//   softmax, two warpgroups (warps 0-3 tile 0, 4-7 tile 1), one thread = one query row = one TMEM lane.  The row of S
+//     (fp32, TMEM) is read twice, 32 scores at a time, rather than held: with 128 scores in registers the compiler
+//     spilled, and spills go to L2 here (shared memory leaves next to no L1; 8.2 us a block of 8-bit keys).  m is
+//     raised only when a score exceeds it by more than 8 (log2 units: p stays below 256), and then the row's sum and O
+//     are scaled down; p = 2^(s - m) is written as 16 bits over the first half of S in two parts, each announced by
+//     itself, so that P V of the first 64 keys runs under the exponentials of the rest.
+//   one warp issues, per block and tile, O += P V of the block before and S = Q K^T (P from TMEM; K K-major, V MN-major
+//     in shared memory).  The tensor pipe runs them in order, so S may overwrite P.
+//   16-bit caches: one warp loads K / V pages with TMA, one box per page and 64-dim panel (128-byte swizzle).
+//   8-bit caches: a warpgroup reads the codes and writes them as fp16 (exact) in the same layout.  Scales, as in
+//     paged_stream_kernel: y = s + log2 vs is the logarithm of t = p vs, m follows y, t = 2^(y - m) is what is rounded
+//     and multiplied with the codes, and the row's sum adds t / vs.
 // K and V have a ring of two blocks each.  TMEM (512 columns): S_t (and P_t) at 128 t, O_t at 256 + 128 t.
 // Few units are spread over more CTAs by cutting the key range into `splits`; paged_join_kernel joins the parts.
 #pragma once
@@ -35,12 +39,14 @@ struct PagedTcArgs {
 template <int POOL, int HD>
 struct PagedTcShape {
     static constexpr bool kWide = POOL == kPoolF16 || POOL == kPoolBf16;
+    // 16-bit: softmax 0-7, products 8, TMA 9.  8-bit: softmax 0-7, codes 8-11, products 12.
     static constexpr int kThreads = kWide ? 320 : 416;
+    static constexpr int kMmaWarp = kWide ? 8 : 12;
     static constexpr uint32_t kPanel = 128 * 64 * 2;             // 128 rows of 64 dims
     static constexpr uint32_t kTile = kPanel * (HD / 64);
     static constexpr uint32_t kK = 2 * kTile;                    // after the two Q tiles
     static constexpr uint32_t kV = kK + kPtStages * kTile;
-    static constexpr uint32_t kScale = kV + kPtStages * kTile;   // [slot][key scale | value scale | its log2][128]
+    static constexpr uint32_t kScale = kV + kPtStages * kTile;   // [slot][key scale | 1 / value scale | log2 of it][128]
     static constexpr uint32_t kBar = kScale + (kWide ? 0u : kPtScaleSlots * 3u * 128u * 4u);
     // at least half of an SM's: two CTAs must not share an SM, each takes all of its TMEM
     static constexpr uint32_t kNeed = kBar + 256 + 1024;
@@ -110,8 +116,8 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
     uint64_t* v_full = k_empty + kPtStages;
     uint64_t* v_empty = v_full + kPtStages;
     uint64_t* s_full = v_empty + kPtStages;        // [tile]
-    uint64_t* p_full = s_full + 2;                 // [tile]
-    uint64_t* o_full = p_full + 2;                 // [tile]
+    uint64_t* p_full = s_full + 2;                 // [tile][half]
+    uint64_t* o_full = p_full + 4;                 // [tile]
     uint64_t* v_tail = o_full + 2;
     uint64_t* scale_full = v_tail + 1;             // [slot]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scale_full + kPtScaleSlots);
@@ -159,7 +165,8 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_full[t], 4);
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[t], 4);
+            mbar_init(&p_full[2 * t], 4);
+            mbar_init(&p_full[2 * t + 1], 4);
             mbar_init(&o_full[t], 1);
         }
         for (int s = 0; s < kPtStages; ++s) {
@@ -173,7 +180,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == Sh::kMmaWarp) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -192,30 +199,41 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         float rf = kWide ? a.scale_log2 : 1.f;  // what a raw score is multiplied by
         {
             // this row of Q into its tile (128-byte swizzle); for 8-bit caches as fp16, scaled by a power of two
-            uint4 w[HD / 8];
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const CT*>(a.q) +
                                                               int64_t(at.s.first + token) * a.q_row + int64_t(hq) * HD);
-#pragma unroll
-            for (int c = 0; c < HD / 8; ++c) w[c] = live ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
-            if constexpr (!kWide && std::is_same<CT, __nv_bfloat16>::value) {
-                uint32_t* u = reinterpret_cast<uint32_t*>(w);
+            constexpr bool kScaleQ = !kWide && std::is_same<CT, __nv_bfloat16>::value;
+            float f = 1.f;
+            if constexpr (kScaleQ) {
                 float big = 0.f;
+                if (live) {
+#pragma unroll 4
+                    for (int c = 0; c < HD / 8; ++c) {
+                        const uint4 w = __ldg(src + c);
+                        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int i = 0; i < HD / 2; ++i) {
-                    big = fmaxf(big, fabsf(__uint_as_float(u[i] << 16)));
-                    big = fmaxf(big, fabsf(__uint_as_float(u[i] & 0xffff0000u)));
+                        for (int e = 0; e < 4; ++e) {
+                            big = fmaxf(big, fabsf(__uint_as_float(u[e] << 16)));
+                            big = fmaxf(big, fabsf(__uint_as_float(u[e] & 0xffff0000u)));
+                        }
+                    }
                 }
                 const int ex = min(max(int(__float_as_uint(big) >> 23) - 127, -125), 125);
-                const float f = big > 0.f ? __uint_as_float(uint32_t(127 - ex) << 23) : 1.f;
+                f = big > 0.f ? __uint_as_float(uint32_t(127 - ex) << 23) : 1.f;
                 rf = big > 0.f ? __uint_as_float(uint32_t(127 + ex) << 23) : 1.f;
-#pragma unroll
-                for (int i = 0; i < HD / 2; ++i)
-                    u[i] = pack_16<__half>(__uint_as_float(u[i] << 16) * f, __uint_as_float(u[i] & 0xffff0000u) * f);
             }
             uint8_t* dst = smem + t * Sh::kTile + row * 128;
+#pragma unroll 4
+            for (int c = 0; c < HD / 8; ++c) {
+                uint4 w = live ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+                if constexpr (kScaleQ) {
+                    uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c)
-                *reinterpret_cast<uint4*>(dst + (c >> 3) * Sh::kPanel + (((c & 7) ^ (row & 7)) << 4)) = w[c];
+                    for (int e = 0; e < 4; ++e)
+                        u[e] = pack_16<__half>(__uint_as_float(u[e] << 16) * f, __uint_as_float(u[e] & 0xffff0000u) * f);
+                    w = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+                *reinterpret_cast<uint4*>(dst + (c >> 3) * Sh::kPanel + (((c & 7) ^ (row & 7)) << 4)) = w;
+            }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -229,8 +247,9 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         const int all_hi = __reduce_min_sync(0xffffffffu, key_hi), all_lo = __reduce_max_sync(0xffffffffu, key_lo);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int j = lo[t]; j < hi[t]; ++j) {
-            const int i = j - lo[t], key0 = j << 7;
+        const int lo_t = t ? lo[1] : lo[0], hi_t = t ? hi[1] : hi[0];
+        for (int j = lo_t; j < hi_t; ++j) {
+            const int i = j - lo_t, key0 = j << 7;  // i: blocks of this tile so far
             const bool whole = key0 >= all_lo && key0 + 127 <= all_hi;
             const int slot = (j - jb) % kPtScaleSlots;
             const float* ks = reinterpret_cast<const float*>(smem + Sh::kScale) + slot * 384;
@@ -241,84 +260,58 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             }
             if (!(ok = warp_wait(&s_full[t], uint32_t(i) & 1u, abort_flag, a.b.status, kErrTimeoutEpilogue))) break;
             tc_fence_after();
-            // 32 of the row's scores (times rf they are in log2 units), -inf where the row does not see the key
-            auto load_chunk = [&](int c, float (&x)[32]) {
-                tmem_ld_32x32b_x32(tS + uint32_t(c * 32), x);
+            // ---- first reading of the row of S, 32 scores at a time (the next ones on their way): its maximum.  What
+            // the second reading should find instead (scaled, or -inf where the row does not see the key) goes back.
+            float x[2][32];
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld_32x32b_x32(tS, x[0]);
+#pragma unroll 1
+            for (int cc = 0; cc < 4; cc += 2) {
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const int c = cc + o;
+                float(&y)[32] = x[o];
                 tmem_ld_wait();
+                if (c < 3) tmem_ld_32x32b_x32(tS + uint32_t(c * 32 + 32), x[o ^ 1]);
                 if constexpr (!kWide) {
+                    const float2 rf2 = make_float2(rf, rf);
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         const float4 k4 = *reinterpret_cast<const float4*>(ks + c * 32 + e);
-                        x[e] *= k4.x, x[e + 1] *= k4.y, x[e + 2] *= k4.z, x[e + 3] *= k4.w;
+                        const float4 v4 = *reinterpret_cast<const float4*>(ks + 256 + c * 32 + e);
+                        const float2 a0 = fma_x2(mul_x2(make_float2(y[e], y[e + 1]), make_float2(k4.x, k4.y)), rf2,
+                                                 make_float2(v4.x, v4.y));
+                        const float2 a1 = fma_x2(mul_x2(make_float2(y[e + 2], y[e + 3]), make_float2(k4.z, k4.w)), rf2,
+                                                 make_float2(v4.z, v4.w));
+                        y[e] = a0.x, y[e + 1] = a0.y, y[e + 2] = a1.x, y[e + 3] = a1.y;
                     }
                 }
                 if (!whole) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const int key = key0 + c * 32 + e;
-                        if (key < key_lo || key > key_hi) x[e] = -INFINITY;
+                        if (key < key_lo || key > key_hi) y[e] = -INFINITY;
                     }
                 }
-            };
-            auto row_max = [&]() -> float {
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float x[32];
-                    load_chunk(c, x);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const float y = x[e] * rf;
-                        mx[e & 3] = fmaxf(mx[e & 3], kWide ? y : y + ks[256 + c * 32 + e]);
-                    }
-                }
-                return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            };
-            uint32_t p[64];
-            // P of the row (packed) and its sums: of p, and of what is rounded to 16 bits (t = p x value scale)
-            auto exp_pass = [&](float& sum_t) -> float {
-                const float base = m == -INFINITY ? 0.f : -m;
-                float sp[4] = {0.f, 0.f, 0.f, 0.f}, st[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float x[32];
-                    load_chunk(c, x);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        x[e] = ex2_approx(fmaf(x[e], rf, base));
-                        sp[e & 3] += x[e];
-                    }
-                    if constexpr (!kWide) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 v4 = *reinterpret_cast<const float4*>(ks + 128 + c * 32 + e);
-                            x[e] *= v4.x, x[e + 1] *= v4.y, x[e + 2] *= v4.z, x[e + 3] *= v4.w;
-                            st[0] += x[e], st[1] += x[e + 1], st[2] += x[e + 2], st[3] += x[e + 3];
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) p[c * 16 + e] = pack_16<MT16>(x[2 * e], x[2 * e + 1]);
-                }
-                const float sum = (sp[0] + sp[1]) + (sp[2] + sp[3]);
-                sum_t = kWide ? sum : (st[0] + st[1]) + (st[2] + st[3]);
-                return sum;
-            };
-            float sum = 0.f, sum_t = 0.f;
-            bool raise = m == -INFINITY;
-            if (!__any_sync(0xffffffffu, raise)) {
-                sum = exp_pass(sum_t);
-                raise = sum_t > 256.f;
+                for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], y[e]);
+                if (!kWide || !whole) tmem_st_32x32b_x32(tS + uint32_t(c * 32), y);
             }
+            }
+            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if constexpr (kWide) top *= rf;  // rf > 0
+            if (!kWide || !whole) tmem_st_wait();
+            tmem_ld_32x32b_x32(tS, x[0]);
+            const bool raise = top > m + 8.f;  // also the first visible key: m is -inf
             if (__any_sync(0xffffffffu, raise)) {
-                const float top = fmaxf(row_max(), m);
-                const float f = !raise || m == top ? 1.f : ex2_approx(m - top);
+                const float f = raise ? ex2_approx(m - top) : 1.f;
                 if (raise) m = top;
                 l *= f;
-                if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+                if (i > 0) {
                     // S of this block is complete, and with it P V of the block before: O may be changed
 #pragma unroll
                     for (int c = 0; c < HD / 32; ++c) {
-                        float o[32];
+                        float(&o)[32] = x[1];
                         tmem_ld_32x32b_x32(tO + uint32_t(c * 32), o);
                         tmem_ld_wait();
 #pragma unroll
@@ -326,17 +319,52 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                         tmem_st_32x32b_x32(tO + uint32_t(c * 32), o);
                     }
                 }
-                sum = exp_pass(sum_t);
             }
-            l += sum;
-            tmem_st_32x32b_x32(tS, reinterpret_cast<const float(&)[32]>(p[0]));
-            tmem_st_32x32b_x32(tS + 32u, reinterpret_cast<const float(&)[32]>(p[32]));
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
+            // ---- second reading: P and the row's sum
+            const float base = m == -INFINITY ? 0.f : -m;
+            const float2 base2 = make_float2(base, base), rf2 = make_float2(rf, rf);
+            float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll 1
+            for (int cc = 0; cc < 4; cc += 2) {
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const int c = cc + o;
+                float(&y)[32] = x[o];
+                tmem_ld_wait();
+                if (c < 3) tmem_ld_32x32b_x32(tS + uint32_t(c * 32 + 32), x[o ^ 1]);
+                float p[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    float2 y0 = make_float2(y[e], y[e + 1]), y1 = make_float2(y[e + 2], y[e + 3]);
+                    y0 = kWide ? fma_x2(y0, rf2, base2) : add_x2(y0, base2);
+                    y1 = kWide ? fma_x2(y1, rf2, base2) : add_x2(y1, base2);
+                    y0.x = ex2_approx(y0.x), y0.y = ex2_approx(y0.y);
+                    y1.x = ex2_approx(y1.x), y1.y = ex2_approx(y1.y);
+                    if constexpr (kWide) {
+                        sum[0] = add_x2(sum[0], y0);
+                        sum[1] = add_x2(sum[1], y1);
+                    } else {
+                        const float4 i4 = *reinterpret_cast<const float4*>(ks + 128 + c * 32 + e);
+                        sum[0] = fma_x2(y0, make_float2(i4.x, i4.y), sum[0]);
+                        sum[1] = fma_x2(y1, make_float2(i4.z, i4.w), sum[1]);
+                    }
+                    p[e / 2] = __uint_as_float(pack_16<MT16>(y0.x, y0.y));
+                    p[e / 2 + 1] = __uint_as_float(pack_16<MT16>(y1.x, y1.y));
+                }
+                // columns 16 c .. of S are among the scores read already
+                tmem_st_32x32b_x16(tS + uint32_t(c * 16), p);
+                if (o == 1) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
+                }
+            }
+            }
+            sum[0] = add_x2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
         }
-        const bool any = hi[t] > lo[t];
+        const bool any = hi_t > lo_t;
         if (any && ok) ok = warp_wait(&o_full[t], 0u, abort_flag, a.b.status, kErrTimeoutEpilogue);
         if (ok) {
             tc_fence_after();
@@ -365,7 +393,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 }
             }
         }
-    } else if (warp == 8) {
+    } else if (warp == Sh::kMmaWarp) {
         // ------------------------------------------------------------------------------------ products
         if (lane == 0) {
             constexpr uint32_t kFmt = std::is_same<MT16, __nv_bfloat16>::value ? 1u : 0u;
@@ -375,21 +403,28 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                       mbar_wait(&q_full[1], 0u, abort_flag, a.b.status, kErrTimeoutMma);
             for (int j = jb; ok && j <= je && je > jb; ++j) {
                 const int i = j - jb, s = i % kPtStages, sv = (i - 1) % kPtStages;
-                for (int t = 0; ok && t < 2; ++t) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (!ok) break;
                     const uint32_t dS = tmem + uint32_t(t * 128), dO = tmem + 256u + uint32_t(t * 128);
                     if (j > jb && j - 1 >= lo[t] && j - 1 < hi[t]) {
                         if (!(ok = mbar_wait(&v_full[sv], uint32_t((i - 1) / kPtStages) & 1u, abort_flag, a.b.status,
-                                             kErrTimeoutMma) &&
-                                   mbar_wait(&p_full[t], uint32_t(j - 1 - lo[t]) & 1u, abort_flag, a.b.status,
                                              kErrTimeoutMma)))
                             break;
-                        tc_fence_after();
                         const uint64_t vd = HD == 64 ? smem_desc_sw128(smem + Sh::kV + sv * Sh::kTile)
                                                      : smem_desc_sw128_mn(smem + Sh::kV + sv * Sh::kTile, Sh::kPanel);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)  // 16 keys = 8 columns of P = 16 rows of V (2 KB)
-                            mma_f16_ts(dO, dS + uint32_t(8 * k), vd + uint64_t(128 * k), idO,
-                                       (j - 1 > lo[t] || k > 0) ? 1u : 0u);
+                        for (int h = 0; h < 2; ++h) {
+                            if (!(ok = mbar_wait(&p_full[2 * t + h], uint32_t(j - 1 - lo[t]) & 1u, abort_flag, a.b.status,
+                                                 kErrTimeoutMma)))
+                                break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int k = 4 * h; k < 4 * h + 4; ++k)  // 16 keys = 8 columns of P = 16 rows of V (2 KB)
+                                mma_f16_ts(dO, dS + uint32_t(8 * k), vd + uint64_t(128 * k), idO,
+                                           (j - 1 > lo[t] || k > 0) ? 1u : 0u);
+                        }
+                        if (!ok) break;
                         if (j == hi[t]) mma_commit(&o_full[t]);
                     }
                     if (j >= lo[t] && j < hi[t]) {
@@ -463,37 +498,50 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 if (lane == 0) mbar_arrive(&v_full[s]);
             }
         }
-    } else {
+    } else if (warp < 12) {
         // ------------------------------------------------------------------------------------ codes to fp16
-        constexpr int kPieces = HD / 16;             // 16-byte pieces of a row of codes
-        constexpr int kEach = 128 * kPieces / 128;   // of a tile, per thread
-        constexpr int kRowStep = 128 / kPieces;      // 16 (head_dim 128) or 32 rows between a thread's pieces
-        const int ct = threadIdx.x - 288, piece = ct % kPieces, row0 = ct / kPieces;
-        auto page_at = [&](int pos) -> int {
-            if (pos >= at.s.context) return -1;
-            const int page = __ldg(table + (pos >> a.kv.page_shift));
-            if (page >= 0 && page < a.kv.pages) return page;
-            batch_error(a.b);
-            return -1;
-        };
-        auto load = [&](const uint8_t* pool, int j, uint4 (&w)[kEach]) {
+        constexpr int kPieces = HD / 16;          // 16-byte pieces of a row of codes; also the pieces a thread handles
+        constexpr int kRowStep = 128 / kPieces;   // rows between a thread's pieces
+        const int ct = threadIdx.x - 256, piece = ct % kPieces, row0 = ct / kPieces;
+        // Pages of the rows a thread copies (and of the key whose scales it carries, last) in block j; -1 behind the
+        // context.  Asked for a block ahead, so that copies do not wait for the table.
+        auto load_pages = [&](int j, int (&pg)[kPieces + 1]) {
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int pos = (j << 7) + row0 + e * kRowStep;
-                const int page = page_at(pos);
-                w[e] = page < 0 ? make_uint4(0u, 0u, 0u, 0u)
-                                : __ldg(reinterpret_cast<const uint4*>(pool + slot_offset(a.kv, page, head, pos)) + piece);
+            for (int e = 0; e <= kPieces; ++e) {
+                const int pos = (j << 7) + (e < kPieces ? row0 + e * kRowStep : ct);
+                pg[e] = j < je && pos < at.s.context ? __ldg(table + (pos >> a.kv.page_shift)) : -1;
             }
         };
-        auto store = [&](uint8_t* tile, const uint4 (&w)[kEach]) {
+        // Out-of-range pages become -1; reported when they lie inside the context.
+        auto check_pages = [&](int j, int (&pg)[kPieces + 1]) {
+            bool bad = false;
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
+            for (int e = 0; e <= kPieces; ++e) {
+                const int pos = (j << 7) + (e < kPieces ? row0 + e * kRowStep : ct);
+                const bool out = pg[e] < 0 || pg[e] >= a.kv.pages;
+                bad = bad || (out && j < je && pos < at.s.context);
+                if (out) pg[e] = -1;
+            }
+            if (bad) batch_error(a.b);
+        };
+        // Codes of a block's rows (rows without a page: any that can be read, zeroed when stored).
+        auto load = [&](const uint8_t* pool, int j, const int (&pg)[kPieces + 1], uint4 (&w)[kPieces]) {
+#pragma unroll
+            for (int e = 0; e < kPieces; ++e)
+                w[e] = __ldg(reinterpret_cast<const uint4*>(
+                                 pool + slot_offset(a.kv, max(pg[e], 0), head, (j << 7) + row0 + e * kRowStep)) +
+                             piece);
+        };
+        auto store = [&](uint8_t* tile, const int (&pg)[kPieces + 1], const uint4 (&w)[kPieces]) {
+#pragma unroll
+            for (int e = 0; e < kPieces; ++e) {
                 const int row = row0 + e * kRowStep;
+                const uint4 c4 = pg[e] < 0 ? make_uint4(0u, 0u, 0u, 0u) : w[e];
                 uint4 h[2];
-                codes_to_f16<POOL>(w[e].x, h[0].x, h[0].y);
-                codes_to_f16<POOL>(w[e].y, h[0].z, h[0].w);
-                codes_to_f16<POOL>(w[e].z, h[1].x, h[1].y);
-                codes_to_f16<POOL>(w[e].w, h[1].z, h[1].w);
+                codes_to_f16<POOL>(c4.x, h[0].x, h[0].y);
+                codes_to_f16<POOL>(c4.y, h[0].z, h[0].w);
+                codes_to_f16<POOL>(c4.z, h[1].x, h[1].y);
+                codes_to_f16<POOL>(c4.w, h[1].z, h[1].w);
                 uint8_t* dst = tile + (piece >> 2) * Sh::kPanel + row * 128;
                 const int c = 2 * (piece & 3);
                 // the two panels' lanes store their halves in opposite order: no two on one bank
@@ -502,47 +550,55 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 *reinterpret_cast<uint4*>(dst + (((c + 1 - first) ^ (row & 7)) << 4)) = first ? h[0] : h[1];
             }
         };
+        // Thread = key: its scales (a key without a page: finite ones, its probability is 0 or its block reported).
+        auto load_scales = [&](int j, const int (&pg)[kPieces + 1], float& ks, float& vs) {
+            const int64_t i = scale_index(a.kv, max(pg[kPieces], 0), head, (j << 7) + ct);
+            ks = __ldg(a.kv.ks + i);
+            vs = __ldg(a.kv.vs + i);
+        };
         bool ok = true;
-        uint4 wk[kEach], wv[kEach];
-        if (jb < je) load(a.kv.k, jb, wk);
+        uint4 w[kPieces];  // K of a block, then V of it: asked for as soon as the tile before is stored
+        int pg[kPieces + 1], next[kPieces + 1];
+        float ks, vs;
+        load_pages(jb, pg);
+        check_pages(jb, pg);
+        load(a.kv.k, jb, pg, w);
+        load_scales(jb, pg, ks, vs);
         for (int j = jb; ok && j < je; ++j) {
             const int i = j - jb, s = i % kPtStages, slot = i % kPtScaleSlots;
             const uint32_t ph = uint32_t(i / kPtStages) & 1u;
-            load(a.kv.v, j, wv);
-            // thread = key: its scales (a key behind the context: any finite ones, its probability is 0)
-            const int pos = (j << 7) + ct;
-            const int page = page_at(pos);
-            float ks = 0.f, vs = 1.f;
-            if (page >= 0) {
-                const int64_t at_scale = scale_index(a.kv, page, head, pos);
-                ks = __ldg(a.kv.ks + at_scale);
-                vs = __ldg(a.kv.vs + at_scale);
-            }
-            if (vs < 3.944304526105059e-31f) vs = 3.944304526105059e-31f;  // 2^-101: a zero scale (zero codes), in log2's range
+            load_pages(j + 1, next);
+            if (pg[kPieces] < 0) ks = 0.f, vs = 1.f;
+            if (vs < 3.944304526105059e-31f) vs = 3.944304526105059e-31f;  // 2^-101 for a zero scale (of zero codes)
             if (!(ok = warp_wait(&k_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
             // K of two blocks ago is consumed, so the softmax of four blocks ago is done with this slot's scales
             float* sc = reinterpret_cast<float*>(smem + Sh::kScale) + slot * 384;
             sc[ct] = ks * a.scale_log2;
-            sc[128 + ct] = vs;
+            sc[128 + ct] = 1.f / vs;
             sc[256 + ct] = __log2f(vs);
-            store(smem + Sh::kK + s * Sh::kTile, wk);
+            store(smem + Sh::kK + s * Sh::kTile, pg, w);
+            load(a.kv.v, j, pg, w);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&scale_full[slot]);
                 mbar_arrive(&k_full[s]);
             }
-            if (j + 1 < je) load(a.kv.k, j + 1, wk);
+            check_pages(j + 1, next);
+            if (j + 1 < je) load_scales(j + 1, next, ks, vs);
             if (!(ok = warp_wait(&v_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
-            store(smem + Sh::kV + s * Sh::kTile, wv);
+            store(smem + Sh::kV + s * Sh::kTile, pg, w);
+            if (j + 1 < je) load(a.kv.k, j + 1, next, w);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[s]);
+#pragma unroll
+            for (int e = 0; e <= kPieces; ++e) pg[e] = next[e];
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == Sh::kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }

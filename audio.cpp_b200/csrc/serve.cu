@@ -4,6 +4,7 @@
 #include "serve.h"
 
 #include <algorithm>
+#include <cmath>
 
 #include "host.cuh"
 #include "kv_cache.cuh"
@@ -331,6 +332,7 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
     const size_t need = attention_bytes(a.b, a.kv, a.group, dev.num_sms);
     if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
         fail(B2D_EINVAL, "paged attention needs a 16-byte aligned workspace of %zu bytes", need);
+    if (!(scale > 0.f) || !std::isfinite(scale)) fail(B2D_EINVAL, "paged attention scale must be positive and finite");
     a.q = q;
     a.o = o;
     a.q_row = q_row;

@@ -482,7 +482,8 @@ B2D_API size_t b2d_paged_attention_workspace(b2d_ctx* ctx, const b2d_kv_cache* c
 
 /* Causal attention of the batch's rows over the cache (their own keys and values already appended): head h of the row
  * at position p reads kv head h / (heads / kv_heads) and
- *   o = sum_j softmax_j(scale q . k_j) v_j  over the positions j <= p, with window > 0 only those above p - window.
+ *   o = sum_j softmax_j(scale q . k_j) v_j  over the positions j <= p, with window > 0 only those above p - window;
+ * scale is positive and finite.
  * q, o: [rows, heads, head_dim] fp16 (bf16 = 0) or bf16 (bf16 = 1), row strides q_row / o_row in elements, 16-byte
  * aligned; a 16-bit cache has the queries' type.  heads is 1 to 128 times kv_heads.  A row that sees no key gives
  * zeros.  Keys and values at the positions of a context that a new row may see must be finite (what lies behind a
