@@ -2,22 +2,23 @@
 // 64 or 128.  Same contract as paged_stream_kernel (paged_attention.cuh), which keeps the sequences of few rows.
 //
 // A CTA takes two 128-row query tiles of one (sequence, kv head): the rows are (token, query head of the group) pairs
-// in that order, packed without gaps, so the heads that share a kv head share its K / V stream.  Keys come in 128-key
-// blocks.  Bound by the exponentials and the tensor pipe alike (128 x 128 scores of 128-dim heads: 1024 clocks of each
-// on an SM); two tiles alternate so that one tile's softmax runs under the other's products:
-//   softmax, two warpgroups (warps 0-3 tile 0, 4-7 tile 1), one thread = one query row = one TMEM lane.  The row of S
-//     (fp32, TMEM) is read twice, 32 scores at a time, rather than held: with 128 scores in registers the compiler
-//     spilled, and spills go to L2 here (shared memory leaves next to no L1; 8.2 us a block of 8-bit keys).  m is
-//     raised only when a score exceeds it by more than 8 (log2 units: p stays below 256), and then the row's sum and O
-//     are scaled down; p = 2^(s - m) is written as 16 bits over the first half of S in two parts, each announced by
-//     itself, so that P V of the first 64 keys runs under the exponentials of the rest.
-//   one warp issues, per block and tile, O += P V of the block before and S = Q K^T (P from TMEM; K K-major, V MN-major
-//     in shared memory).  The tensor pipe runs them in order, so S may overwrite P.
+// in that order, packed without gaps, so the heads that share a kv head share its K / V stream.  Keys are loaded in
+// blocks of 128 and worked on in halves of 64.  Bound by the exponentials and the tensor pipe alike (128 x 128 scores of
+// 128-dim heads: 1024 clocks of each on an SM), so every role runs ahead of the others as far as its buffers go:
+//   softmax, two warpgroups (warps 0-3 tile 0, 4-7 tile 1), one thread = one query row = one TMEM lane.  64 scores of
+//     the row (fp32, TMEM) come to registers; m is raised only when a score exceeds it by more than 8 (log2 units: p
+//     stays below 256), and then the row's sum and O are scaled down; p = 2^(s - m) is written as 16 bits over the
+//     scores it came from.
+//   one warp issues, per half and tile, O += P V of two halves before and S = Q K^T (P from TMEM; K K-major, V MN-major
+//     in shared memory).  The tensor pipe runs them in order, so S may overwrite that P; the half in between is the
+//     softmax's meanwhile.  (With one 128-key S a tile the softmax waited for its own products: 2.6 us a block in
+//     place of SUBBLOCK_US, although N = 64 reads Q from shared memory twice as often.)
 //   16-bit caches: one warp loads K / V pages with TMA, one box per page and 64-dim panel (128-byte swizzle).
 //   8-bit caches: a warpgroup reads the codes and writes them as fp16 (exact) in the same layout.  Scales, as in
 //     paged_stream_kernel: y = s + log2 vs is the logarithm of t = p vs, m follows y, t = 2^(y - m) is what is rounded
 //     and multiplied with the codes, and the row's sum adds t / vs.
-// K and V have a ring of two blocks each.  TMEM (512 columns): S_t (and P_t) at 128 t, O_t at 256 + 128 t.
+// K and V have a ring of two blocks each.  TMEM (512 columns): S (and P) of tile t, half h at 128 t + 64 h, O_t at
+// 256 + 128 t.
 // Few units are spread over more CTAs by cutting the key range into `splits`; paged_join_kernel joins the parts.
 #pragma once
 
@@ -115,10 +116,10 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
     uint64_t* k_empty = k_full + kPtStages;
     uint64_t* v_full = k_empty + kPtStages;
     uint64_t* v_empty = v_full + kPtStages;
-    uint64_t* s_full = v_empty + kPtStages;        // [tile]
-    uint64_t* p_full = s_full + 2;                 // [tile][half]
-    uint64_t* o_full = p_full + 4;                 // [tile]
-    uint64_t* v_tail = o_full + 2;
+    uint64_t* s_full = v_empty + kPtStages;        // [tile][half]
+    uint64_t* p_full = s_full + 4;                 // [tile][half]
+    uint64_t* o_done = p_full + 4;                 // [tile][half]: its P V has been added
+    uint64_t* v_tail = o_done + 4;
     uint64_t* scale_full = v_tail + 1;             // [slot]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scale_full + kPtScaleSlots);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
     const int seq_rows = at.s.n * a.group;
     const int p_base = at.s.context - at.s.n;  // position of the sequence's first new token
 
-    // key blocks each tile sees, cut to this split's share of the pair's range
+    // halves (64 keys) that each tile sees, cut to this split's share of the pair's blocks jb .. je - 1
     int lo[2], hi[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -140,15 +141,16 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         if (r0 <= r1) {
             const int p0 = p_base + r0 / a.group, p1 = p_base + r1 / a.group;
             if (p1 >= 0) {
-                lo[t] = a.window > 0 ? max(0, p0 - a.window + 1) >> 7 : 0;
-                hi[t] = (p1 >> 7) + 1;
+                lo[t] = a.window > 0 ? max(0, p0 - a.window + 1) >> 6 : 0;
+                hi[t] = (p1 >> 6) + 1;
             }
         }
     }
-    int jb = lo[0], je = hi[0];
+    int jb = 0, je = 0;
+    if (hi[0] > lo[0]) jb = lo[0] >> 1, je = (hi[0] + 1) >> 1;
     if (hi[1] > lo[1]) {
-        if (je > jb) jb = min(jb, lo[1]), je = max(je, hi[1]);
-        else jb = lo[1], je = hi[1];
+        jb = je > jb ? min(jb, lo[1] >> 1) : lo[1] >> 1;
+        je = max(je, (hi[1] + 1) >> 1);
     }
     if (ta.splits > 1) {
         const int n = je - jb, b0 = jb;
@@ -157,17 +159,18 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        lo[t] = max(lo[t], jb);
-        hi[t] = min(hi[t], je);
+        lo[t] = max(lo[t], 2 * jb);
+        hi[t] = min(hi[t], 2 * je);
     }
 
     if (threadIdx.x == 0) {
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_full[t], 4);
-            mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[2 * t], 4);
-            mbar_init(&p_full[2 * t + 1], 4);
-            mbar_init(&o_full[t], 1);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(&s_full[2 * t + h], 1);
+                mbar_init(&p_full[2 * t + h], 4);
+                mbar_init(&o_done[2 * t + h], 1);
+            }
         }
         for (int s = 0; s < kPtStages; ++s) {
             mbar_init(&k_full[s], kWide ? 1 : 4);
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         if (lane == 0) mbar_arrive(&q_full[t]);
 
         const uint32_t lane_off = uint32_t(wq * 32) << 16;
-        const uint32_t tS = tmem + lane_off + uint32_t(t * 128), tO = tmem + lane_off + 256u + uint32_t(t * 128);
+        const uint32_t tS0 = tmem + lane_off + uint32_t(t * 128), tO = tmem + lane_off + 256u + uint32_t(t * 128);
         const int p_row = live ? p_base + token : 0x3fffffff;  // a lane without a row sees every key (of a zero query)
         const int key_hi = p_row, key_lo = live && a.window > 0 ? p_row - a.window + 1 : 0;
         // keys that every row of the warp sees
@@ -248,94 +251,83 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         const int lo_t = t ? lo[1] : lo[0], hi_t = t ? hi[1] : hi[0];
-        for (int j = lo_t; j < hi_t; ++j) {
-            const int i = j - lo_t, key0 = j << 7;  // i: blocks of this tile so far
-            const bool whole = key0 >= all_lo && key0 + 127 <= all_hi;
-            const int slot = (j - jb) % kPtScaleSlots;
-            const float* ks = reinterpret_cast<const float*>(smem + Sh::kScale) + slot * 384;
+        for (int u = lo_t; u < hi_t; ++u) {
+            const int i = u - lo_t, h = u & 1, key0 = u << 6, blk = (u >> 1) - jb;  // i: halves of this tile so far
+            const bool whole = key0 >= all_lo && key0 + 63 <= all_hi;
+            const uint32_t tS = tS0 + uint32_t(h * 64);
+            const float* ks = reinterpret_cast<const float*>(smem + Sh::kScale) + (blk % kPtScaleSlots) * 384 + h * 64;
             if constexpr (!kWide) {
-                if (!(ok = warp_wait(&scale_full[slot], uint32_t((j - jb) / kPtScaleSlots) & 1u, abort_flag, a.b.status,
-                                     kErrTimeoutEpilogue)))
+                if (!(ok = warp_wait(&scale_full[blk % kPtScaleSlots], uint32_t(blk / kPtScaleSlots) & 1u, abort_flag,
+                                     a.b.status, kErrTimeoutEpilogue)))
                     break;
             }
-            if (!(ok = warp_wait(&s_full[t], uint32_t(i) & 1u, abort_flag, a.b.status, kErrTimeoutEpilogue))) break;
+            if (!(ok = warp_wait(&s_full[2 * t + h], uint32_t(i >> 1) & 1u, abort_flag, a.b.status, kErrTimeoutEpilogue)))
+                break;
             tc_fence_after();
-            // ---- first reading of the row of S, 32 scores at a time (the next ones on their way): its maximum.  What
-            // the second reading should find instead (scaled, or -inf where the row does not see the key) goes back.
             float x[2][32];
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             tmem_ld_32x32b_x32(tS, x[0]);
-#pragma unroll 1
-            for (int cc = 0; cc < 4; cc += 2) {
+            tmem_ld_32x32b_x32(tS + 32u, x[1]);
+            tmem_ld_wait();
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int o = 0; o < 2; ++o) {
-                const int c = cc + o;
-                float(&y)[32] = x[o];
-                tmem_ld_wait();
-                if (c < 3) tmem_ld_32x32b_x32(tS + uint32_t(c * 32 + 32), x[o ^ 1]);
+            for (int c = 0; c < 2; ++c) {
                 if constexpr (!kWide) {
                     const float2 rf2 = make_float2(rf, rf);
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         const float4 k4 = *reinterpret_cast<const float4*>(ks + c * 32 + e);
                         const float4 v4 = *reinterpret_cast<const float4*>(ks + 256 + c * 32 + e);
-                        const float2 a0 = fma_x2(mul_x2(make_float2(y[e], y[e + 1]), make_float2(k4.x, k4.y)), rf2,
+                        const float2 a0 = fma_x2(mul_x2(make_float2(x[c][e], x[c][e + 1]), make_float2(k4.x, k4.y)), rf2,
                                                  make_float2(v4.x, v4.y));
-                        const float2 a1 = fma_x2(mul_x2(make_float2(y[e + 2], y[e + 3]), make_float2(k4.z, k4.w)), rf2,
-                                                 make_float2(v4.z, v4.w));
-                        y[e] = a0.x, y[e + 1] = a0.y, y[e + 2] = a1.x, y[e + 3] = a1.y;
+                        const float2 a1 = fma_x2(mul_x2(make_float2(x[c][e + 2], x[c][e + 3]), make_float2(k4.z, k4.w)),
+                                                 rf2, make_float2(v4.z, v4.w));
+                        x[c][e] = a0.x, x[c][e + 1] = a0.y, x[c][e + 2] = a1.x, x[c][e + 3] = a1.y;
                     }
                 }
                 if (!whole) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const int key = key0 + c * 32 + e;
-                        if (key < key_lo || key > key_hi) y[e] = -INFINITY;
+                        if (key < key_lo || key > key_hi) x[c][e] = -INFINITY;
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], y[e]);
-                if (!kWide || !whole) tmem_st_32x32b_x32(tS + uint32_t(c * 32), y);
-            }
+                for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[c][e]);
             }
             float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             if constexpr (kWide) top *= rf;  // rf > 0
-            if (!kWide || !whole) tmem_st_wait();
-            tmem_ld_32x32b_x32(tS, x[0]);
             const bool raise = top > m + 8.f;  // also the first visible key: m is -inf
             if (__any_sync(0xffffffffu, raise)) {
                 const float f = raise ? ex2_approx(m - top) : 1.f;
                 if (raise) m = top;
                 l *= f;
                 if (i > 0) {
-                    // S of this block is complete, and with it P V of the block before: O may be changed
+                    // O holds the halves up to the one before once its P V is done.  (One barrier a half: this S being
+                    // full says that the P V of two halves before is, so the phase waited for is the running one.)
+                    if (!(ok = warp_wait(&o_done[2 * t + (h ^ 1)], uint32_t((i - 1) >> 1) & 1u, abort_flag, a.b.status,
+                                         kErrTimeoutEpilogue)))
+                        break;
+                    tc_fence_after();
 #pragma unroll
-                    for (int c = 0; c < HD / 32; ++c) {
-                        float(&o)[32] = x[1];
-                        tmem_ld_32x32b_x32(tO + uint32_t(c * 32), o);
+                    for (int c = 0; c < HD / 16; ++c) {
+                        float o[16];
+                        tmem_ld_32x32b_x16(tO + uint32_t(c * 16), o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= f;
-                        tmem_st_32x32b_x32(tO + uint32_t(c * 32), o);
+                        for (int e = 0; e < 16; ++e) o[e] *= f;
+                        tmem_st_32x32b_x16(tO + uint32_t(c * 16), o);
                     }
                 }
             }
-            // ---- second reading: P and the row's sum
             const float base = m == -INFINITY ? 0.f : -m;
             const float2 base2 = make_float2(base, base), rf2 = make_float2(rf, rf);
             float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll 1
-            for (int cc = 0; cc < 4; cc += 2) {
 #pragma unroll
-            for (int o = 0; o < 2; ++o) {
-                const int c = cc + o;
-                float(&y)[32] = x[o];
-                tmem_ld_wait();
-                if (c < 3) tmem_ld_32x32b_x32(tS + uint32_t(c * 32 + 32), x[o ^ 1]);
+            for (int c = 0; c < 2; ++c) {
                 float p[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
-                    float2 y0 = make_float2(y[e], y[e + 1]), y1 = make_float2(y[e + 2], y[e + 3]);
+                    float2 y0 = make_float2(x[c][e], x[c][e + 1]), y1 = make_float2(x[c][e + 2], x[c][e + 3]);
                     y0 = kWide ? fma_x2(y0, rf2, base2) : add_x2(y0, base2);
                     y1 = kWide ? fma_x2(y1, rf2, base2) : add_x2(y1, base2);
                     y0.x = ex2_approx(y0.x), y0.y = ex2_approx(y0.y);
@@ -351,21 +343,19 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                     p[e / 2] = __uint_as_float(pack_16<MT16>(y0.x, y0.y));
                     p[e / 2 + 1] = __uint_as_float(pack_16<MT16>(y1.x, y1.y));
                 }
-                // columns 16 c .. of S are among the scores read already
                 tmem_st_32x32b_x16(tS + uint32_t(c * 16), p);
-                if (o == 1) {
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
-                }
             }
-            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
             sum[0] = add_x2(sum[0], sum[1]);
             l += sum[0].x + sum[0].y;
         }
         const bool any = hi_t > lo_t;
-        if (any && ok) ok = warp_wait(&o_full[t], 0u, abort_flag, a.b.status, kErrTimeoutEpilogue);
+        if (ok && any)
+            ok = warp_wait(&o_done[2 * t + ((hi_t - 1) & 1)], uint32_t((hi_t - lo_t - 1) >> 1) & 1u, abort_flag, a.b.status,
+                           kErrTimeoutEpilogue);
         if (ok) {
             tc_fence_after();
             const bool part = ta.splits > 1;
@@ -395,56 +385,61 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         }
     } else if (warp == Sh::kMmaWarp) {
         // ------------------------------------------------------------------------------------ products
-        if (lane == 0) {
-            constexpr uint32_t kFmt = std::is_same<MT16, __nv_bfloat16>::value ? 1u : 0u;
-            constexpr uint32_t idS = idesc_f16(kFmt, 128, 128);
-            constexpr uint32_t idO = idesc_f16(kFmt, 128, HD) | (1u << 16);  // B (V) MN-major
-            bool ok = mbar_wait(&q_full[0], 0u, abort_flag, a.b.status, kErrTimeoutMma) &&
-                      mbar_wait(&q_full[1], 0u, abort_flag, a.b.status, kErrTimeoutMma);
-            for (int j = jb; ok && j <= je && je > jb; ++j) {
-                const int i = j - jb, s = i % kPtStages, sv = (i - 1) % kPtStages;
+        // The whole warp keeps the books and waits, one elected lane issues.
+        constexpr uint32_t kFmt = std::is_same<MT16, __nv_bfloat16>::value ? 1u : 0u;
+        constexpr uint32_t idS = idesc_f16(kFmt, 128, 64);
+        constexpr uint32_t idO = idesc_f16(kFmt, 128, HD) | (1u << 16);  // B (V) MN-major
+        const uint64_t q_desc = smem_desc_sw128(smem), k_desc = smem_desc_sw128(smem + Sh::kK);
+        const uint64_t v_desc = HD == 64 ? smem_desc_sw128(smem + Sh::kV) : smem_desc_sw128_mn(smem + Sh::kV, Sh::kPanel);
+        constexpr uint64_t kTileStep = Sh::kTile >> 4, kHalfStep = 8192 >> 4;  // 64 rows of 128 bytes
+        bool ok = warp_wait(&q_full[0], 0u, abort_flag, a.b.status, kErrTimeoutMma) &&
+                  warp_wait(&q_full[1], 0u, abort_flag, a.b.status, kErrTimeoutMma);
+        for (int u = 2 * jb; ok && je > jb && u < 2 * je + 2; ++u) {
+            const int w = u - 2;  // the half whose P V is due
+            const int h = u & 1, blk = (u >> 1) - jb, s = blk % kPtStages, sw = (blk - 1) & (kPtStages - 1);
+            if (h == 0) {  // both blocks of this round have to be there
+                if (blk > 0)
+                    ok = warp_wait(&v_full[sw], uint32_t((blk - 1) / kPtStages) & 1u, abort_flag, a.b.status, kErrTimeoutMma);
+                if (ok && u < 2 * je)
+                    ok = warp_wait(&k_full[s], uint32_t(blk / kPtStages) & 1u, abort_flag, a.b.status, kErrTimeoutMma);
+                if (!ok) break;
+                tc_fence_after();
+            }
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (!ok) break;
-                    const uint32_t dS = tmem + uint32_t(t * 128), dO = tmem + 256u + uint32_t(t * 128);
-                    if (j > jb && j - 1 >= lo[t] && j - 1 < hi[t]) {
-                        if (!(ok = mbar_wait(&v_full[sv], uint32_t((i - 1) / kPtStages) & 1u, abort_flag, a.b.status,
-                                             kErrTimeoutMma)))
-                            break;
-                        const uint64_t vd = HD == 64 ? smem_desc_sw128(smem + Sh::kV + sv * Sh::kTile)
-                                                     : smem_desc_sw128_mn(smem + Sh::kV + sv * Sh::kTile, Sh::kPanel);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (!(ok = mbar_wait(&p_full[2 * t + h], uint32_t(j - 1 - lo[t]) & 1u, abort_flag, a.b.status,
-                                                 kErrTimeoutMma)))
-                                break;
-                            tc_fence_after();
-#pragma unroll
-                            for (int k = 4 * h; k < 4 * h + 4; ++k)  // 16 keys = 8 columns of P = 16 rows of V (2 KB)
-                                mma_f16_ts(dO, dS + uint32_t(8 * k), vd + uint64_t(128 * k), idO,
-                                           (j - 1 > lo[t] || k > 0) ? 1u : 0u);
-                        }
-                        if (!ok) break;
-                        if (j == hi[t]) mma_commit(&o_full[t]);
-                    }
-                    if (j >= lo[t] && j < hi[t]) {
-                        if (!(ok = mbar_wait(&k_full[s], uint32_t(i / kPtStages) & 1u, abort_flag, a.b.status,
-                                             kErrTimeoutMma)))
-                            break;
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t dS = tmem + uint32_t(t * 128) + uint32_t(h * 64), dO = tmem + 256u + uint32_t(t * 128);
+                if (ok && w >= lo[t] && w < hi[t]) {
+                    const int i = w - lo[t];
+                    ok = warp_wait(&p_full[2 * t + h], uint32_t(i >> 1) & 1u, abort_flag, a.b.status, kErrTimeoutMma);
+                    if (ok) {
                         tc_fence_after();
-                        const uint64_t qd = smem_desc_sw128(smem + t * Sh::kTile);
-                        const uint64_t kd = smem_desc_sw128(smem + Sh::kK + s * Sh::kTile);
+                        const uint64_t vd = v_desc + uint64_t(sw) * kTileStep + uint64_t(h) * kHalfStep;
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)  // 16 keys = 8 columns of P = 16 rows of V (2 KB)
+                                mma_f16_ts(dO, dS + uint32_t(8 * k), vd + uint64_t(128 * k), idO, (i > 0 || k > 0) ? 1u : 0u);
+                            mma_commit(&o_done[2 * t + h]);
+                        }
+                    }
+                }
+                if (ok && u < 2 * je && u >= lo[t] && u < hi[t]) {
+                    const uint64_t qd = q_desc + uint64_t(t) * kTileStep;
+                    const uint64_t kd = k_desc + uint64_t(s) * kTileStep + uint64_t(h) * kHalfStep;
+                    if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < HD / 16; ++k) {
                             const uint64_t off = uint64_t((k >> 2) * (Sh::kPanel >> 4) + 2 * (k & 3));
                             mma_f16_ss(dS, qd + off, kd + off, idS, k > 0 ? 1u : 0u);
                         }
-                        mma_commit(&s_full[t]);
+                        mma_commit(&s_full[2 * t + h]);
                     }
                 }
-                if (!ok) break;
-                if (j < je) mma_commit(&k_empty[s]);
-                if (j > jb) mma_commit(&v_empty[sv]);
+            }
+            if (!ok) break;
+            // a block is free once both tiles have used its second half
+            if (h == 1 && elect_one()) {
+                if (u < 2 * je) mma_commit(&k_empty[s]);
+                if (blk > 0) mma_commit(&v_empty[sw]);
             }
         }
     } else if constexpr (kWide) {

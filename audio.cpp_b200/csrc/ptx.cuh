@@ -446,6 +446,18 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint16_t cta_mask
         : "memory");
 }
 
+// One lane of a converged warp (always the same one).  Code under it keeps warp-uniform operands in uniform registers;
+// under `lane == 0` every tcgen05.mma first moved its descriptors there, some 70 clocks an instruction.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 __device__ __forceinline__ uint32_t elect_one_lane() {
     return (threadIdx.x & 31u) == 0u;
 }
