@@ -9,7 +9,7 @@
 //     the row (fp32, TMEM) come to registers; m is raised only when a score exceeds it by more than 8 (log2 units: p
 //     stays below 256), and then the row's sum and O are scaled down; p = 2^(s - m) is written as 16 bits over the
 //     scores it came from.
-//   one warp issues, per half and tile, O += P V of two halves before and S = Q K^T (P from TMEM; K K-major, V MN-major
+//   one warp a tile issues, per half, O += P V of two halves before and S = Q K^T (P from TMEM; K K-major, V MN-major
 //     in shared memory).  The tensor pipe runs them in order, so S may overwrite that P; the half in between is the
 //     softmax's meanwhile.  (With one 128-key S a tile the softmax waited for its own products: 2.6 us a block in
 //     place of SUBBLOCK_US, although N = 64 reads Q from shared memory twice as often.)
@@ -40,9 +40,10 @@ struct PagedTcArgs {
 template <int POOL, int HD>
 struct PagedTcShape {
     static constexpr bool kWide = POOL == kPoolF16 || POOL == kPoolBf16;
-    // 16-bit: softmax 0-7, products 8, TMA 9.  8-bit: softmax 0-7, codes 8-11, products 12.
-    static constexpr int kThreads = kWide ? 320 : 416;
-    static constexpr int kMmaWarp = kWide ? 8 : 12;
+    // Warps: softmax 0-7, products 8 and 9 (one a tile), then one for TMA (16-bit) or three pairs for the codes (8-bit).
+    static constexpr int kCodePairs = 3;
+    static constexpr int kThreads = kWide ? 352 : 320 + 64 * kCodePairs;
+    static constexpr int kMmaWarp = 8;
     static constexpr uint32_t kPanel = 128 * 64 * 2;             // 128 rows of 64 dims
     static constexpr uint32_t kTile = kPanel * (HD / 64);
     static constexpr uint32_t kK = 2 * kTile;                    // after the two Q tiles
@@ -173,10 +174,10 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             }
         }
         for (int s = 0; s < kPtStages; ++s) {
-            mbar_init(&k_full[s], kWide ? 1 : 4);
-            mbar_init(&k_empty[s], 1);
+            mbar_init(&k_full[s], kWide ? 1 : 4);  // 8-bit: two warps for each half
+            mbar_init(&k_empty[s], 2);
             mbar_init(&v_full[s], kWide ? 1 : 4);
-            mbar_init(&v_empty[s], 1);
+            mbar_init(&v_empty[s], 2);
         }
         mbar_init(v_tail, 1);
         for (int s = 0; s < kPtScaleSlots; ++s) mbar_init(&scale_full[s], 4);
@@ -383,60 +384,60 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 }
             }
         }
-    } else if (warp == Sh::kMmaWarp) {
+    } else if (warp < Sh::kMmaWarp + 2) {
         // ------------------------------------------------------------------------------------ products
-        // The whole warp keeps the books and waits, one elected lane issues.
+        // A warp a tile keeps the books and waits, one elected lane issues.  (One warp for both tiles spent 1400 clocks a
+        // half on issuing and waiting.)
+        const int t = warp - Sh::kMmaWarp;
         constexpr uint32_t kFmt = std::is_same<MT16, __nv_bfloat16>::value ? 1u : 0u;
         constexpr uint32_t idS = idesc_f16(kFmt, 128, 64);
         constexpr uint32_t idO = idesc_f16(kFmt, 128, HD) | (1u << 16);  // B (V) MN-major
-        const uint64_t q_desc = smem_desc_sw128(smem), k_desc = smem_desc_sw128(smem + Sh::kK);
-        const uint64_t v_desc = HD == 64 ? smem_desc_sw128(smem + Sh::kV) : smem_desc_sw128_mn(smem + Sh::kV, Sh::kPanel);
         constexpr uint64_t kTileStep = Sh::kTile >> 4, kHalfStep = 8192 >> 4;  // 64 rows of 128 bytes
-        bool ok = warp_wait(&q_full[0], 0u, abort_flag, a.b.status, kErrTimeoutMma) &&
-                  warp_wait(&q_full[1], 0u, abort_flag, a.b.status, kErrTimeoutMma);
+        const uint64_t q_desc = smem_desc_sw128(smem + t * Sh::kTile), k_desc = smem_desc_sw128(smem + Sh::kK);
+        const uint64_t v_desc = HD == 64 ? smem_desc_sw128(smem + Sh::kV) : smem_desc_sw128_mn(smem + Sh::kV, Sh::kPanel);
+        const uint32_t dO = tmem + 256u + uint32_t(t * 128);
+        const int lo_t = t ? lo[1] : lo[0], hi_t = t ? hi[1] : hi[0];
+        bool ok = warp_wait(&q_full[t], 0u, abort_flag, a.b.status, kErrTimeoutMma);
         for (int u = 2 * jb; ok && je > jb && u < 2 * je + 2; ++u) {
             const int w = u - 2;  // the half whose P V is due
-            const int h = u & 1, blk = (u >> 1) - jb, s = blk % kPtStages, sw = (blk - 1) & (kPtStages - 1);
-            if (h == 0) {  // both blocks of this round have to be there
+            const int h = u & 1, blk = (u >> 1) - jb, s = blk & (kPtStages - 1), sw = (blk - 1) & (kPtStages - 1);
+            const uint32_t dS = tmem + uint32_t(t * 128) + uint32_t(h * 64);
+            // both blocks of this round have to be there -- also for a tile without a use for them, whose warp
+            // must not give a block back twice before the other tile's has once
+            if (h == 0) {
                 if (blk > 0)
-                    ok = warp_wait(&v_full[sw], uint32_t((blk - 1) / kPtStages) & 1u, abort_flag, a.b.status, kErrTimeoutMma);
+                    ok = warp_wait(&v_full[sw], uint32_t((blk - 1) / kPtStages) & 1u, abort_flag, a.b.status,
+                                   kErrTimeoutMma);
                 if (ok && u < 2 * je)
                     ok = warp_wait(&k_full[s], uint32_t(blk / kPtStages) & 1u, abort_flag, a.b.status, kErrTimeoutMma);
                 if (!ok) break;
                 tc_fence_after();
             }
+            if (w >= lo_t && w < hi_t) {
+                const int i = w - lo_t;
+                if (!(ok = warp_wait(&p_full[2 * t + h], uint32_t(i >> 1) & 1u, abort_flag, a.b.status, kErrTimeoutMma)))
+                    break;
+                tc_fence_after();
+                const uint64_t vd = v_desc + uint64_t(sw) * kTileStep + uint64_t(h) * kHalfStep;
+                if (elect_one()) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint32_t dS = tmem + uint32_t(t * 128) + uint32_t(h * 64), dO = tmem + 256u + uint32_t(t * 128);
-                if (ok && w >= lo[t] && w < hi[t]) {
-                    const int i = w - lo[t];
-                    ok = warp_wait(&p_full[2 * t + h], uint32_t(i >> 1) & 1u, abort_flag, a.b.status, kErrTimeoutMma);
-                    if (ok) {
-                        tc_fence_after();
-                        const uint64_t vd = v_desc + uint64_t(sw) * kTileStep + uint64_t(h) * kHalfStep;
-                        if (elect_one()) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)  // 16 keys = 8 columns of P = 16 rows of V (2 KB)
-                                mma_f16_ts(dO, dS + uint32_t(8 * k), vd + uint64_t(128 * k), idO, (i > 0 || k > 0) ? 1u : 0u);
-                            mma_commit(&o_done[2 * t + h]);
-                        }
-                    }
-                }
-                if (ok && u < 2 * je && u >= lo[t] && u < hi[t]) {
-                    const uint64_t qd = q_desc + uint64_t(t) * kTileStep;
-                    const uint64_t kd = k_desc + uint64_t(s) * kTileStep + uint64_t(h) * kHalfStep;
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < HD / 16; ++k) {
-                            const uint64_t off = uint64_t((k >> 2) * (Sh::kPanel >> 4) + 2 * (k & 3));
-                            mma_f16_ss(dS, qd + off, kd + off, idS, k > 0 ? 1u : 0u);
-                        }
-                        mma_commit(&s_full[2 * t + h]);
-                    }
+                    for (int k = 0; k < 4; ++k)  // 16 keys = 8 columns of P = 16 rows of V (2 KB)
+                        mma_f16_ts(dO, dS + uint32_t(8 * k), vd + uint64_t(128 * k), idO, (i > 0 || k > 0) ? 1u : 0u);
+                    mma_commit(&o_done[2 * t + h]);
                 }
             }
-            if (!ok) break;
-            // a block is free once both tiles have used its second half
+            if (u < 2 * je && u >= lo_t && u < hi_t) {
+                const uint64_t kd = k_desc + uint64_t(s) * kTileStep + uint64_t(h) * kHalfStep;
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const uint64_t off = uint64_t((k >> 2) * (Sh::kPanel >> 4) + 2 * (k & 3));
+                        mma_f16_ss(dS, q_desc + off, kd + off, idS, k > 0 ? 1u : 0u);
+                    }
+                    mma_commit(&s_full[2 * t + h]);
+                }
+            }
+            // a block is free once both tiles' warps are past its second half
             if (h == 1 && elect_one()) {
                 if (u < 2 * je) mma_commit(&k_empty[s]);
                 if (blk > 0) mma_commit(&v_empty[sw]);
@@ -493,102 +494,97 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 if (lane == 0) mbar_arrive(&v_full[s]);
             }
         }
-    } else if (warp < 12) {
+    } else {
         // ------------------------------------------------------------------------------------ codes to fp16
-        constexpr int kPieces = HD / 16;          // 16-byte pieces of a row of codes; also the pieces a thread handles
-        constexpr int kRowStep = 128 / kPieces;   // rows between a thread's pieces
-        const int ct = threadIdx.x - 256, piece = ct % kPieces, row0 = ct / kPieces;
-        // Pages of the rows a thread copies (and of the key whose scales it carries, last) in block j; -1 behind the
-        // context.  Asked for a block ahead, so that copies do not wait for the table.
-        auto load_pages = [&](int j, int (&pg)[kPieces + 1]) {
-#pragma unroll
-            for (int e = 0; e <= kPieces; ++e) {
-                const int pos = (j << 7) + (e < kPieces ? row0 + e * kRowStep : ct);
-                pg[e] = j < je && pos < at.s.context ? __ldg(table + (pos >> a.kv.page_shift)) : -1;
-            }
+        // The half tiles K a, K b, V a, V b of block 0, of block 1, .. go around the pairs of warps: a pair asks for its
+        // next half as soon as it has stored one, so a load has the time of three to arrive.
+        constexpr int kRowPieces = HD / 16;              // 16-byte pieces of a row of codes
+        constexpr int kPieces = 64 * kRowPieces / 64;    // pieces of a half tile that a thread copies
+        constexpr int kRowStep = 64 / kRowPieces;        // rows between them
+        const int pair = (warp - 10) >> 1, ct = (threadIdx.x - 320) & 63, piece = ct % kRowPieces, row0 = ct / kRowPieces;
+        const int units = 4 * (je - jb);
+        const int page_mask = (1 << a.kv.page_shift) - 1;
+        // Lane g (mod 4) holds the page of the half's 16 rows g (pages are multiples of 16 rows), -1 behind the context.
+        auto unit_key = [&](int n) { return ((jb + (n >> 2)) << 7) + ((n & 1) << 6); };  // position of its first row
+        auto load_page = [&](int n) -> int {
+            const int pos = unit_key(n) + ((lane & 3) << 4);
+            return n < units && pos < at.s.context ? __ldg(table + (pos >> a.kv.page_shift)) : -1;
         };
-        // Out-of-range pages become -1; reported when they lie inside the context.
-        auto check_pages = [&](int j, int (&pg)[kPieces + 1]) {
-            bool bad = false;
-#pragma unroll
-            for (int e = 0; e <= kPieces; ++e) {
-                const int pos = (j << 7) + (e < kPieces ? row0 + e * kRowStep : ct);
-                const bool out = pg[e] < 0 || pg[e] >= a.kv.pages;
-                bad = bad || (out && j < je && pos < at.s.context);
-                if (out) pg[e] = -1;
-            }
-            if (bad) batch_error(a.b);
+        // An out-of-range page becomes -1; reported when it lies inside the context.
+        auto check_page = [&](int n, int pg) -> int {
+            if (pg >= 0 && pg < a.kv.pages) return pg;
+            if (n < units && unit_key(n) + ((lane & 3) << 4) < at.s.context) batch_error(a.b);
+            return -1;
         };
-        // Codes of a block's rows (rows without a page: any that can be read, zeroed when stored).
-        auto load = [&](const uint8_t* pool, int j, const int (&pg)[kPieces + 1], uint4 (&w)[kPieces]) {
-#pragma unroll
-            for (int e = 0; e < kPieces; ++e)
-                w[e] = __ldg(reinterpret_cast<const uint4*>(
-                                 pool + slot_offset(a.kv, max(pg[e], 0), head, (j << 7) + row0 + e * kRowStep)) +
-                             piece);
-        };
-        auto store = [&](uint8_t* tile, const int (&pg)[kPieces + 1], const uint4 (&w)[kPieces]) {
+        uint4 w[kPieces];
+        float ks = 0.f, vs = 1.f;  // of key ct, with a half of K
+        // Rows without a page: any that can be read, zeroed when stored.
+        auto load = [&](int n, int pg) {
+            const uint8_t* base = (n & 2 ? a.kv.v : a.kv.k) + int64_t(head) * a.kv.head_stride + piece * 16;
+            const int first = (n & 1) << 6;
 #pragma unroll
             for (int e = 0; e < kPieces; ++e) {
                 const int row = row0 + e * kRowStep;
-                const uint4 c4 = pg[e] < 0 ? make_uint4(0u, 0u, 0u, 0u) : w[e];
+                const int p = max(__shfl_sync(0xffffffffu, pg, row >> 4), 0);
+                w[e] = __ldg(reinterpret_cast<const uint4*>(base + int64_t(p) * a.kv.page_stride +
+                                                            int64_t((first + row) & page_mask) * a.kv.token_stride));
+            }
+            if (!(n & 2)) {
+                const int p = max(__shfl_sync(0xffffffffu, pg, ct >> 4), 0);
+                const int64_t i = ((int64_t(p) * a.kv.kv_heads + head) << a.kv.page_shift) + ((first + ct) & page_mask);
+                ks = __ldg(a.kv.ks + i);
+                vs = __ldg(a.kv.vs + i);
+            }
+        };
+        bool ok = true;
+        int n = pair;
+        int pg = check_page(n, load_page(n)), next = load_page(n + Sh::kCodePairs);
+        if (n < units) load(n, pg);
+        for (; ok && n < units; n += Sh::kCodePairs) {
+            const int i = n >> 2, s = i % kPtStages, slot = i % kPtScaleSlots, first = (n & 1) << 6;
+            const bool is_v = (n & 2) != 0;
+            const int used = at.s.context - unit_key(n);  // rows from here on are behind the context
+            const uint32_t ph = uint32_t(i / kPtStages) & 1u;
+            if (!(ok = warp_wait(is_v ? &v_empty[s] : &k_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer)))
+                break;
+            uint8_t* tile = smem + (is_v ? Sh::kV : Sh::kK) + s * Sh::kTile + (piece >> 2) * Sh::kPanel;
+#pragma unroll
+            for (int e = 0; e < kPieces; ++e) {
+                const int row = row0 + e * kRowStep;
+                const bool there = __shfl_sync(0xffffffffu, pg, row >> 4) >= 0 && row < used;
+                const uint4 c4 = there ? w[e] : make_uint4(0u, 0u, 0u, 0u);
                 uint4 h[2];
                 codes_to_f16<POOL>(c4.x, h[0].x, h[0].y);
                 codes_to_f16<POOL>(c4.y, h[0].z, h[0].w);
                 codes_to_f16<POOL>(c4.z, h[1].x, h[1].y);
                 codes_to_f16<POOL>(c4.w, h[1].z, h[1].w);
-                uint8_t* dst = tile + (piece >> 2) * Sh::kPanel + row * 128;
+                uint8_t* dst = tile + (first + row) * 128;
                 const int c = 2 * (piece & 3);
                 // the two panels' lanes store their halves in opposite order: no two on one bank
-                const int first = piece >> 2;
-                *reinterpret_cast<uint4*>(dst + (((c + first) ^ (row & 7)) << 4)) = first ? h[1] : h[0];
-                *reinterpret_cast<uint4*>(dst + (((c + 1 - first) ^ (row & 7)) << 4)) = first ? h[0] : h[1];
+                const int o = piece >> 2;
+                *reinterpret_cast<uint4*>(dst + (((c + o) ^ (row & 7)) << 4)) = o ? h[1] : h[0];
+                *reinterpret_cast<uint4*>(dst + (((c + 1 - o) ^ (row & 7)) << 4)) = o ? h[0] : h[1];
             }
-        };
-        // Thread = key: its scales (a key without a page: finite ones, its probability is 0 or its block reported).
-        auto load_scales = [&](int j, const int (&pg)[kPieces + 1], float& ks, float& vs) {
-            const int64_t i = scale_index(a.kv, max(pg[kPieces], 0), head, (j << 7) + ct);
-            ks = __ldg(a.kv.ks + i);
-            vs = __ldg(a.kv.vs + i);
-        };
-        bool ok = true;
-        uint4 w[kPieces];  // K of a block, then V of it: asked for as soon as the tile before is stored
-        int pg[kPieces + 1], next[kPieces + 1];
-        float ks, vs;
-        load_pages(jb, pg);
-        check_pages(jb, pg);
-        load(a.kv.k, jb, pg, w);
-        load_scales(jb, pg, ks, vs);
-        for (int j = jb; ok && j < je; ++j) {
-            const int i = j - jb, s = i % kPtStages, slot = i % kPtScaleSlots;
-            const uint32_t ph = uint32_t(i / kPtStages) & 1u;
-            load_pages(j + 1, next);
-            if (pg[kPieces] < 0) ks = 0.f, vs = 1.f;
-            if (vs < 3.944304526105059e-31f) vs = 3.944304526105059e-31f;  // 2^-101 for a zero scale (of zero codes)
-            if (!(ok = warp_wait(&k_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
-            // K of two blocks ago is consumed, so the softmax of four blocks ago is done with this slot's scales
-            float* sc = reinterpret_cast<float*>(smem + Sh::kScale) + slot * 384;
-            sc[ct] = ks * a.scale_log2;
-            sc[128 + ct] = 1.f / vs;
-            sc[256 + ct] = __log2f(vs);
-            store(smem + Sh::kK + s * Sh::kTile, pg, w);
-            load(a.kv.v, j, pg, w);
+            if (!is_v) {
+                // K of two blocks ago is consumed, so the softmax of four blocks ago is done with this slot's scales
+                float* sc = reinterpret_cast<float*>(smem + Sh::kScale) + slot * 384 + first + ct;
+                // a key without a page: finite scales, its probability is 0 or its block reported
+                const bool there = __shfl_sync(0xffffffffu, pg, ct >> 4) >= 0 && ct < used;
+                float v = there ? vs : 1.f;
+                if (v < 3.944304526105059e-31f) v = 3.944304526105059e-31f;  // 2^-101 for a zero scale (of zero codes)
+                sc[0] = there ? ks * a.scale_log2 : 0.f;
+                sc[128] = 1.f / v;
+                sc[256] = __log2f(v);
+            }
+            pg = check_page(n + Sh::kCodePairs, next);
+            if (n + Sh::kCodePairs < units) load(n + Sh::kCodePairs, pg);
+            next = load_page(n + 2 * Sh::kCodePairs);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(&scale_full[slot]);
-                mbar_arrive(&k_full[s]);
+                if (!is_v) mbar_arrive(&scale_full[slot]);
+                mbar_arrive(is_v ? &v_full[s] : &k_full[s]);
             }
-            check_pages(j + 1, next);
-            if (j + 1 < je) load_scales(j + 1, next, ks, vs);
-            if (!(ok = warp_wait(&v_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
-            store(smem + Sh::kV + s * Sh::kTile, pg, w);
-            if (j + 1 < je) load(a.kv.k, j + 1, next, w);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&v_full[s]);
-#pragma unroll
-            for (int e = 0; e <= kPieces; ++e) pg[e] = next[e];
         }
     }
     tc_fence_before();

@@ -195,6 +195,17 @@ __device__ __forceinline__ float2 mul_x2(float2 a, float2 b) {
     return d;
 }
 
+// A warpgroup's registers per thread from here on (all its warps take the same one).  The block's warpgroups share what
+// it was launched with.
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 __device__ __forceinline__ void tma_prefetch_desc(const void* tmap) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
 }
