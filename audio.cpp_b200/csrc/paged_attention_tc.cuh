@@ -14,9 +14,12 @@
 //     softmax's meanwhile.  (With one 128-key S a tile the softmax waited for its own products: 2.6 us a block in
 //     place of SUBBLOCK_US, although N = 64 reads Q from shared memory twice as often.)
 //   16-bit caches: one warp loads K / V pages with TMA, one box per page and 64-dim panel (128-byte swizzle).
-//   8-bit caches: a warpgroup reads the codes and writes them as fp16 (exact) in the same layout.  Scales, as in
-//     paged_stream_kernel: y = s + log2 vs is the logarithm of t = p vs, m follows y, t = 2^(y - m) is what is rounded
-//     and multiplied with the codes, and the row's sum adds t / vs.
+//   8-bit caches: three pairs of warps read the codes and write them as fp16 in the same layout.  fp16 queries: the codes
+//     stay exact and scales are applied as in paged_stream_kernel: y = s + log2 vs is the logarithm of t = p vs, m
+//     follows y, t = 2^(y - m) is what is rounded and multiplied with the codes, and the row's sum adds t / vs.  bf16
+//     queries: the warps write round(code x scale / 2^e), 2^e the power of two of the largest of 32 scales, so that the
+//     softmax has one factor of its scores and one exponent to add for 32 keys in place of 48 shared loads a half.
+//     Those roundings are of 2^-11 at most, the queries' and the output's own of 2^-8.
 // K and V have a ring of two blocks each.  TMEM (512 columns): S (and P) of tile t, half h at 128 t + 64 h, O_t at
 // 256 + 128 t.
 // Few units are spread over more CTAs by cutting the key range into `splits`; paged_join_kernel joins the parts.
@@ -28,6 +31,9 @@ namespace b2d {
 
 constexpr int kPtStages = 2;
 constexpr int kPtScaleSlots = 4;
+// Per block: bf16 queries 4 factors of K and 4 exponents of V, fp16 queries the key scales, 1 / value scales and log2 of
+// the value scales of 128 keys.
+constexpr int kPtScaleFloats = 3 * 128;
 
 struct PagedTcArgs {
     PagedArgs a;
@@ -48,8 +54,8 @@ struct PagedTcShape {
     static constexpr uint32_t kTile = kPanel * (HD / 64);
     static constexpr uint32_t kK = 2 * kTile;                    // after the two Q tiles
     static constexpr uint32_t kV = kK + kPtStages * kTile;
-    static constexpr uint32_t kScale = kV + kPtStages * kTile;   // [slot][key scale | 1 / value scale | log2 of it][128]
-    static constexpr uint32_t kBar = kScale + (kWide ? 0u : kPtScaleSlots * 3u * 128u * 4u);
+    static constexpr uint32_t kScale = kV + kPtStages * kTile;   // [slot]: see kPtScaleFloats
+    static constexpr uint32_t kBar = kScale + (kWide ? 0u : kPtScaleSlots * kPtScaleFloats * 4u);
     // at least half of an SM's: two CTAs must not share an SM, each takes all of its TMEM
     static constexpr uint32_t kNeed = kBar + 256 + 1024;
     static constexpr uint32_t kSmem = kNeed > 120u * 1024u ? kNeed : 120u * 1024u;
@@ -107,7 +113,9 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                     const PagedTcArgs ta) {
     using Sh = PagedTcShape<POOL, HD>;
     constexpr bool kWide = Sh::kWide;
-    using MT16 = typename std::conditional<kWide, CT, __half>::type;  // the products' 16-bit type
+    constexpr bool kFold = !kWide && std::is_same<CT, __nv_bfloat16>::value;  // 8-bit scales are in the fp16 values
+    constexpr bool kApart = !kWide && !kFold;                                 // .. or applied key by key in the softmax
+    using MT16 = typename std::conditional<kWide, CT, __half>::type;          // the products' 16-bit type
     const PagedArgs& a = ta.a;
     extern __shared__ uint8_t pt_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~uintptr_t(1023));
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             const int i = u - lo_t, h = u & 1, key0 = u << 6, blk = (u >> 1) - jb;  // i: halves of this tile so far
             const bool whole = key0 >= all_lo && key0 + 63 <= all_hi;
             const uint32_t tS = tS0 + uint32_t(h * 64);
-            const float* ks = reinterpret_cast<const float*>(smem + Sh::kScale) + (blk % kPtScaleSlots) * 384 + h * 64;
+            const float* sc = reinterpret_cast<const float*>(smem + Sh::kScale) + (blk % kPtScaleSlots) * kPtScaleFloats;
             if constexpr (!kWide) {
                 if (!(ok = warp_wait(&scale_full[blk % kPtScaleSlots], uint32_t(blk / kPtScaleSlots) & 1u, abort_flag,
                                      a.b.status, kErrTimeoutEpilogue)))
@@ -269,19 +277,28 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             tmem_ld_32x32b_x32(tS, x[0]);
             tmem_ld_32x32b_x32(tS + 32u, x[1]);
             tmem_ld_wait();
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            // factor of the raw scores, and exponent of V that joins theirs: one each for 32 keys
+            float fk[2] = {rf, rf}, ev[2] = {0.f, 0.f};
+            if constexpr (kFold) {
+                const float2 f2 = *reinterpret_cast<const float2*>(sc + 2 * h);
+                const float2 e2 = *reinterpret_cast<const float2*>(sc + 4 + 2 * h);
+                // not zero: a masked score has to stay -inf when it is multiplied
+                fk[0] = fmaxf(rf * f2.x, 1.17549435e-38f), fk[1] = fmaxf(rf * f2.y, 1.17549435e-38f);
+                ev[0] = e2.x, ev[1] = e2.y;
+            }
+            float top = -INFINITY;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                if constexpr (!kWide) {
-                    const float2 rf2 = make_float2(rf, rf);
+                if constexpr (kApart) {
+                    const float* kf = sc + h * 64 + c * 32;
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
-                        const float4 k4 = *reinterpret_cast<const float4*>(ks + c * 32 + e);
-                        const float4 v4 = *reinterpret_cast<const float4*>(ks + 256 + c * 32 + e);
-                        const float2 a0 = fma_x2(mul_x2(make_float2(x[c][e], x[c][e + 1]), make_float2(k4.x, k4.y)), rf2,
+                        const float4 k4 = *reinterpret_cast<const float4*>(kf + e);
+                        const float4 v4 = *reinterpret_cast<const float4*>(kf + 256 + e);
+                        const float2 a0 = fma_x2(make_float2(x[c][e], x[c][e + 1]), make_float2(k4.x, k4.y),
                                                  make_float2(v4.x, v4.y));
-                        const float2 a1 = fma_x2(mul_x2(make_float2(x[c][e + 2], x[c][e + 3]), make_float2(k4.z, k4.w)),
-                                                 rf2, make_float2(v4.z, v4.w));
+                        const float2 a1 = fma_x2(make_float2(x[c][e + 2], x[c][e + 3]), make_float2(k4.z, k4.w),
+                                                 make_float2(v4.z, v4.w));
                         x[c][e] = a0.x, x[c][e + 1] = a0.y, x[c][e + 2] = a1.x, x[c][e + 3] = a1.y;
                     }
                 }
@@ -292,11 +309,12 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                         if (key < key_lo || key > key_hi) x[c][e] = -INFINITY;
                     }
                 }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[c][e]);
+                const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                top = fmaxf(top, kApart ? most : fmaf(most, fk[c], ev[c]));  // factors are positive
             }
-            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            if constexpr (kWide) top *= rf;  // rf > 0
             const bool raise = top > m + 8.f;  // also the first visible key: m is -inf
             if (__any_sync(0xffffffffu, raise)) {
                 const float f = raise ? ex2_approx(m - top) : 1.f;
@@ -321,37 +339,40 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 }
             }
             const float base = m == -INFINITY ? 0.f : -m;
-            const float2 base2 = make_float2(base, base), rf2 = make_float2(rf, rf);
-            float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+            float sum_h = 0.f;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+                const float2 f2 = make_float2(fk[c], fk[c]), base2 = make_float2(base + ev[c], base + ev[c]);
+                float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
                 float p[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
                     float2 y0 = make_float2(x[c][e], x[c][e + 1]), y1 = make_float2(x[c][e + 2], x[c][e + 3]);
-                    y0 = kWide ? fma_x2(y0, rf2, base2) : add_x2(y0, base2);
-                    y1 = kWide ? fma_x2(y1, rf2, base2) : add_x2(y1, base2);
+                    y0 = kApart ? add_x2(y0, base2) : fma_x2(y0, f2, base2);
+                    y1 = kApart ? add_x2(y1, base2) : fma_x2(y1, f2, base2);
                     y0.x = ex2_approx(y0.x), y0.y = ex2_approx(y0.y);
                     y1.x = ex2_approx(y1.x), y1.y = ex2_approx(y1.y);
-                    if constexpr (kWide) {
-                        sum[0] = add_x2(sum[0], y0);
-                        sum[1] = add_x2(sum[1], y1);
-                    } else {
-                        const float4 i4 = *reinterpret_cast<const float4*>(ks + 128 + c * 32 + e);
+                    if constexpr (kApart) {
+                        const float4 i4 = *reinterpret_cast<const float4*>(sc + 128 + h * 64 + c * 32 + e);
                         sum[0] = fma_x2(y0, make_float2(i4.x, i4.y), sum[0]);
                         sum[1] = fma_x2(y1, make_float2(i4.z, i4.w), sum[1]);
+                    } else {
+                        sum[0] = add_x2(sum[0], y0);
+                        sum[1] = add_x2(sum[1], y1);
                     }
                     p[e / 2] = __uint_as_float(pack_16<MT16>(y0.x, y0.y));
                     p[e / 2 + 1] = __uint_as_float(pack_16<MT16>(y1.x, y1.y));
                 }
                 tmem_st_32x32b_x16(tS + uint32_t(c * 16), p);
+                sum[0] = add_x2(sum[0], sum[1]);
+                const float part = sum[0].x + sum[0].y;
+                sum_h += kFold ? part * ex2_approx(-ev[c]) : part;
             }
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
-            sum[0] = add_x2(sum[0], sum[1]);
-            l += sum[0].x + sum[0].y;
+            l += sum_h;
         }
         const bool any = hi_t > lo_t;
         if (ok && any)
@@ -498,30 +519,31 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         // ------------------------------------------------------------------------------------ codes to fp16
         // The half tiles K a, K b, V a, V b of block 0, of block 1, .. go around the pairs of warps: a pair asks for its
         // next half as soon as it has stored one, so a load has the time of three to arrive.
-        constexpr int kRowPieces = HD / 16;              // 16-byte pieces of a row of codes
-        constexpr int kPieces = 64 * kRowPieces / 64;    // pieces of a half tile that a thread copies
-        constexpr int kRowStep = 64 / kRowPieces;        // rows between them
-        const int pair = (warp - 10) >> 1, ct = (threadIdx.x - 320) & 63, piece = ct % kRowPieces, row0 = ct / kRowPieces;
+        constexpr int kRowPieces = HD / 16;          // 16-byte pieces of a row of codes
+        constexpr int kRowStep = 32 / kRowPieces;    // rows between the pieces that a lane copies
+        constexpr int kPieces = kRowPieces;          // of the warp's 32 rows
+        const int pair = (warp - 10) >> 1, sub = (warp - 10) & 1, piece = lane % kRowPieces, row0 = lane / kRowPieces;
         const int units = 4 * (je - jb);
         const int page_mask = (1 << a.kv.page_shift) - 1;
-        // Lane g (mod 4) holds the page of the half's 16 rows g (pages are multiples of 16 rows), -1 behind the context.
-        auto unit_key = [&](int n) { return ((jb + (n >> 2)) << 7) + ((n & 1) << 6); };  // position of its first row
+        // Row r of the warp: key unit_key + r.  Lane g (mod 2) holds the page of the 16 rows g (pages are multiples of
+        // 16 rows), -1 behind the context.
+        auto unit_key = [&](int n) { return ((jb + (n >> 2)) << 7) + ((n & 1) << 6) + (sub << 5); };
         auto load_page = [&](int n) -> int {
-            const int pos = unit_key(n) + ((lane & 3) << 4);
+            const int pos = unit_key(n) + ((lane & 1) << 4);
             return n < units && pos < at.s.context ? __ldg(table + (pos >> a.kv.page_shift)) : -1;
         };
         // An out-of-range page becomes -1; reported when it lies inside the context.
         auto check_page = [&](int n, int pg) -> int {
             if (pg >= 0 && pg < a.kv.pages) return pg;
-            if (n < units && unit_key(n) + ((lane & 3) << 4) < at.s.context) batch_error(a.b);
+            if (n < units && unit_key(n) + ((lane & 1) << 4) < at.s.context) batch_error(a.b);
             return -1;
         };
         uint4 w[kPieces];
-        float ks = 0.f, vs = 1.f;  // of key ct, with a half of K
+        float ks = 0.f, vs = 0.f;  // scales of row `lane`; ks for K only
         // Rows without a page: any that can be read, zeroed when stored.
         auto load = [&](int n, int pg) {
+            const int first = unit_key(n) & page_mask;
             const uint8_t* base = (n & 2 ? a.kv.v : a.kv.k) + int64_t(head) * a.kv.head_stride + piece * 16;
-            const int first = (n & 1) << 6;
 #pragma unroll
             for (int e = 0; e < kPieces; ++e) {
                 const int row = row0 + e * kRowStep;
@@ -529,52 +551,85 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 w[e] = __ldg(reinterpret_cast<const uint4*>(base + int64_t(p) * a.kv.page_stride +
                                                             int64_t((first + row) & page_mask) * a.kv.token_stride));
             }
-            if (!(n & 2)) {
-                const int p = max(__shfl_sync(0xffffffffu, pg, ct >> 4), 0);
-                const int64_t i = ((int64_t(p) * a.kv.kv_heads + head) << a.kv.page_shift) + ((first + ct) & page_mask);
-                ks = __ldg(a.kv.ks + i);
-                vs = __ldg(a.kv.vs + i);
-            }
+            const int p = max(__shfl_sync(0xffffffffu, pg, lane >> 4), 0);
+            const int64_t i = ((int64_t(p) * a.kv.kv_heads + head) << a.kv.page_shift) + ((first + lane) & page_mask);
+            if (!(n & 2)) ks = __ldg(a.kv.ks + i);
+            vs = __ldg(a.kv.vs + i);
         };
+        // Power of two of the largest of the warp's 32 scales (NaN and infinities, which are to come through, aside).
+        auto exponent = [&](float scale) -> int {
+            const uint32_t u = __float_as_uint(scale);
+            const uint32_t most = __reduce_max_sync(0xffffffffu, u < 0x7f800000u ? u : 0u);
+            return min(max(int(most >> 23) - 127, -101), 126);  // held scales are 0 or at least 2^-100
+        };
+        auto power = [](int e) { return __uint_as_float(uint32_t(e + 127) << 23); };
         bool ok = true;
         int n = pair;
         int pg = check_page(n, load_page(n)), next = load_page(n + Sh::kCodePairs);
         if (n < units) load(n, pg);
         for (; ok && n < units; n += Sh::kCodePairs) {
-            const int i = n >> 2, s = i % kPtStages, slot = i % kPtScaleSlots, first = (n & 1) << 6;
+            const int i = n >> 2, s = i % kPtStages, slot = i % kPtScaleSlots, group = 2 * (n & 1) + sub;
             const bool is_v = (n & 2) != 0;
             const int used = at.s.context - unit_key(n);  // rows from here on are behind the context
             const uint32_t ph = uint32_t(i / kPtStages) & 1u;
+            // a row without a page: zero codes; its probability is 0 or its block reported
+            const bool there = __shfl_sync(0xffffffffu, pg, lane >> 4) >= 0 && lane < used;
+            int e_k = 0, e_v = 0;
+            uint32_t parts = 0;
+            if constexpr (kFold) {
+                e_k = exponent(there && !is_v ? ks : 0.f);
+                e_v = exponent(there ? vs : 0.f);
+                const float unit = there ? (is_v ? vs * power(-e_v) : ks * power(-e_k)) : 0.f;
+                // the scale in two fp16 parts: code x high + code x low is rounded once (but for 2^-10 of a step)
+                const __half high = __float2half_rn(unit);
+                const __half2 both = __halves2half2(high, __float2half_rn(unit - __half2float(high)));
+                parts = *reinterpret_cast<const uint32_t*>(&both);
+            }
             if (!(ok = warp_wait(is_v ? &v_empty[s] : &k_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer)))
                 break;
-            uint8_t* tile = smem + (is_v ? Sh::kV : Sh::kK) + s * Sh::kTile + (piece >> 2) * Sh::kPanel;
+            uint8_t* tile = smem + (is_v ? Sh::kV : Sh::kK) + s * Sh::kTile + (piece >> 2) * Sh::kPanel + group * 32 * 128;
 #pragma unroll
             for (int e = 0; e < kPieces; ++e) {
                 const int row = row0 + e * kRowStep;
-                const bool there = __shfl_sync(0xffffffffu, pg, row >> 4) >= 0 && row < used;
-                const uint4 c4 = there ? w[e] : make_uint4(0u, 0u, 0u, 0u);
-                uint4 h[2];
-                codes_to_f16<POOL>(c4.x, h[0].x, h[0].y);
-                codes_to_f16<POOL>(c4.y, h[0].z, h[0].w);
-                codes_to_f16<POOL>(c4.z, h[1].x, h[1].y);
-                codes_to_f16<POOL>(c4.w, h[1].z, h[1].w);
-                uint8_t* dst = tile + (first + row) * 128;
+                const bool zero = __shfl_sync(0xffffffffu, pg, row >> 4) < 0 || row >= used;
+                const uint4 c4 = zero ? make_uint4(0u, 0u, 0u, 0u) : w[e];
+                uint32_t h[8];
+                codes_to_f16<POOL>(c4.x, h[0], h[1]);
+                codes_to_f16<POOL>(c4.y, h[2], h[3]);
+                codes_to_f16<POOL>(c4.z, h[4], h[5]);
+                codes_to_f16<POOL>(c4.w, h[6], h[7]);
+                if constexpr (kFold) {
+                    const uint32_t hl = __shfl_sync(0xffffffffu, parts, row);
+                    const __half2 both = *reinterpret_cast<const __half2*>(&hl);
+                    const __half2 hi2 = __low2half2(both), lo2 = __high2half2(both);
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) {
+                        const __half2 c2 = *reinterpret_cast<const __half2*>(&h[d]);
+                        const __half2 y = __hfma2(c2, hi2, __hmul2(c2, lo2));
+                        h[d] = *reinterpret_cast<const uint32_t*>(&y);
+                    }
+                }
+                uint8_t* dst = tile + row * 128;
                 const int c = 2 * (piece & 3);
                 // the two panels' lanes store their halves in opposite order: no two on one bank
                 const int o = piece >> 2;
-                *reinterpret_cast<uint4*>(dst + (((c + o) ^ (row & 7)) << 4)) = o ? h[1] : h[0];
-                *reinterpret_cast<uint4*>(dst + (((c + 1 - o) ^ (row & 7)) << 4)) = o ? h[0] : h[1];
+                const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
+                *reinterpret_cast<uint4*>(dst + (((c + o) ^ (row & 7)) << 4)) = o ? h1 : h0;
+                *reinterpret_cast<uint4*>(dst + (((c + 1 - o) ^ (row & 7)) << 4)) = o ? h0 : h1;
             }
             if (!is_v) {
                 // K of two blocks ago is consumed, so the softmax of four blocks ago is done with this slot's scales
-                float* sc = reinterpret_cast<float*>(smem + Sh::kScale) + slot * 384 + first + ct;
-                // a key without a page: finite scales, its probability is 0 or its block reported
-                const bool there = __shfl_sync(0xffffffffu, pg, ct >> 4) >= 0 && ct < used;
-                float v = there ? vs : 1.f;
-                if (v < 3.944304526105059e-31f) v = 3.944304526105059e-31f;  // 2^-101 for a zero scale (of zero codes)
-                sc[0] = there ? ks * a.scale_log2 : 0.f;
-                sc[128] = 1.f / v;
-                sc[256] = __log2f(v);
+                float* sc = reinterpret_cast<float*>(smem + Sh::kScale) + slot * kPtScaleFloats;
+                if constexpr (kApart) {
+                    float v = there ? vs : 1.f;
+                    if (v < 3.944304526105059e-31f) v = 3.944304526105059e-31f;  // 2^-101 for a zero scale (of zero codes)
+                    sc[group * 32 + lane] = there ? ks * a.scale_log2 : 0.f;
+                    sc[128 + group * 32 + lane] = 1.f / v;
+                    sc[256 + group * 32 + lane] = __log2f(v);
+                } else if (lane == 0) {
+                    sc[group] = power(e_k) * a.scale_log2;
+                    sc[4 + group] = float(e_v);
+                }
             }
             pg = check_page(n + Sh::kCodePairs, next);
             if (n + Sh::kCodePairs < units) load(n + Sh::kCodePairs, pg);

@@ -9,7 +9,9 @@ much; exp2 and the scale's rounding add less than 2^-19 (scores here stay below 
 u |o|.  Probabilities are rounded to fp16 for fp16 queries and for every 8-bit cache (t = p x value scale there, times
 integer codes).  An fp16 number below 2^-14 is off by 2^-25 absolute instead of u of itself.  The key that set the
 running maximum has t = 1, so with n keys the sum of t code is off by at most n 2^-25 max|code|, and the sum of p is at
-least 1 / (that key's value scale): the output is off by at most n 2^-25 max|code| x scale <= n 2^-25 max|v|."""
+least 1 / (that key's value scale): the output is off by at most n 2^-25 max|code| x scale <= n 2^-25 max|v|.  bf16
+queries on an 8-bit cache: chunks multiply keys rounded to fp16, each off by 2^-11 of itself (or 2^-25 of the largest of
+its neighbours), which moves a score by at most 2^-11 sum |q k| scale."""
 import numpy as np
 import pytest
 
@@ -85,7 +87,8 @@ def attention(q, k, v, start, context, scale, window):
 def attention_bound(o, a, ds, dtype, head_dim, eight_bit, keys, vmax):
     u = torch.finfo(dtype).eps / 2
     rel = u * (2 if eight_bit else 1) + 2.0 ** -18
-    bound = a * rel + 2 * a * ((head_dim + 8) * 2.0 ** -24 * ds)[..., None] + u * o.abs()
+    score = (head_dim + 8) * 2.0 ** -24 + (2.0 ** -11 if eight_bit and dtype == torch.bfloat16 else 0.0)
+    bound = a * rel + 2 * a * (score * ds)[..., None] + u * o.abs()
     if dtype == torch.float16 or eight_bit:
         bound = bound + 2.0 ** -25 * keys * vmax
     if dtype == torch.float16:
