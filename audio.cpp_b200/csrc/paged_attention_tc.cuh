@@ -548,8 +548,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             for (int e = 0; e < kPieces; ++e) {
                 const int row = row0 + e * kRowStep;
                 const int p = max(__shfl_sync(0xffffffffu, pg, row >> 4), 0);
-                w[e] = __ldg(reinterpret_cast<const uint4*>(base + int64_t(p) * a.kv.page_stride +
-                                                            int64_t((first + row) & page_mask) * a.kv.token_stride));
+                w[e] = load_once(base + int64_t(p) * a.kv.page_stride + int64_t((first + row) & page_mask) * a.kv.token_stride);
             }
             const int p = max(__shfl_sync(0xffffffffu, pg, lane >> 4), 0);
             const int64_t i = ((int64_t(p) * a.kv.kv_heads + head) << a.kv.page_shift) + ((first + lane) & page_mask);

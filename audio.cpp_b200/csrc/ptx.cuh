@@ -166,6 +166,15 @@ __device__ __forceinline__ float ex2_approx(float x) {
     return y;
 }
 
+// 16 bytes of data that this SM reads once: not kept in L1.
+__device__ __forceinline__ uint4 load_once(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
 // Two fp32 operations in one instruction (each half rounded as the plain one would be).
 __device__ __forceinline__ float2 fma_x2(float2 a, float2 b, float2 c) {
     float2 d;
