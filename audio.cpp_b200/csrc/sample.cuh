@@ -5,9 +5,13 @@
 // those with w >= min_p; each cut is a prefix of that order.  The token is the first index (in index order) whose
 // running sum over kept entries passes u Z.
 //
-// A row is read from HBM once: a cluster of up to 8 CTAs holds it in shared memory (fp32), and every later pass reads
-// it there.  A cut is found by a histogram of 2048 bins (linear in the logit, later linear in the ordered bits of the
-// crossing bin) until the crossing bin holds few enough entries to rank them one against the other.
+// A row is read from HBM once: a cluster of up to 8 CTAs holds it in shared memory (in its own type), and every later
+// pass reads it there.  A cut is found by counting entries in 2048 bins (linear in the logit, later linear in the ordered
+// bits).  For a cut by mass, a bin's mass lies between its count times the weights at its two edges, which brackets the
+// crossing to a few bins; the masses above the bracket and of its upper half are then summed exactly, which decides
+// for a half, and that is counted again until it holds few enough entries to rank them one against the other.  The
+// undecided range of ordered bits at least halves every round, so there are at most 33.  (Summing masses into the bins
+// took three more shared atomics an entry.)
 // Which token comes out depends on sums of up to 2^18 terms and on comparisons next to a border, so the weights are
 // computed in fp64 and added as integers (units of 2^-45 of the largest weight): sums of integers do not depend on
 // the order of threads, warps or CTAs, so neither does the token.
@@ -26,8 +30,8 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 2048;
-constexpr int kSampleList = 1024;         // entries ranked one against the other
-constexpr int kSampleMaxSlice = 32768;    // entries a CTA holds; 16-bit pieces of a weight then add up in 32 bits
+constexpr int kSampleList = 512;          // entries ranked one against the other
+constexpr int kSampleMaxSlice = 32768;    // entries a CTA holds
 constexpr int kSampleMaxCluster = 8;
 constexpr double kSampleUnit = 35184372088832.0;  // 2^45
 
@@ -52,22 +56,43 @@ __device__ __forceinline__ uint32_t ordered_bits(float x) {
 
 struct SampleShared {
     uint32_t count[kSampleBins];
-    uint32_t mass[3][kSampleBins];  // 16-bit pieces of the weights, lowest first
     uint64_t list_entry[kSampleList];  // (ordered bits, ~index): larger = earlier in the order
     uint64_t list_weight[kSampleList];
+    double power[64];                  // 2^(i / 64)
+    double warp_f64[2][kSampleWarps];
     uint64_t warp_u64[kSampleWarps + 1];
     uint32_t warp_u32[kSampleWarps + 1];
-    uint64_t best;       // largest (ordered bits, ~index) of this CTA
-    uint32_t low;        // smallest ordered bits above -inf of this CTA
-    uint64_t total;      // mass of this CTA
-    uint32_t key_lo, key_hi;
+    // of this CTA, read by the others
+    uint64_t best;         // largest (ordered bits, ~index)
+    uint32_t low;          // smallest ordered bits above -inf
+    uint64_t total;        // mass
+    uint64_t upper;        // mass of the bracket's upper half
+    uint32_t inside[2];    // entries in the halves
+    uint32_t key_lo[2], key_hi[2];  // their ordered bits
     uint32_t list_fill;
     // published by rank 0
-    int bin;
-    uint32_t bin_count, before_count;
-    uint64_t before_mass;
-    uint64_t cut;        // last kept (ordered bits, ~index)
+    int bin_lo, bin_hi;    // the bracket
+    uint32_t before_count;
+    uint64_t cut;          // last kept (ordered bits, ~index)
 };
+
+// exp(t) in units of 2^-45 for -32 < t <= 0, to the nearest unit but for some 2^-46: t log2 e = n + i / 64 + r with
+// |r| <= 1 / 128, 2^r by its Taylor polynomial of degree 4 (the next term is below 2^-44.5), 2^(i / 64) from a table.
+__device__ __forceinline__ uint64_t exp_units(double t, const double* power) {
+    constexpr double kMagic = 6755399441055744.0;  // 1.5 x 2^52: adding it rounds to an integer in the low bits
+    const double y = t * 92.33248261689366;        // 64 log2 e
+    const double z = y + kMagic;
+    const int i = __double2loint(z);
+    const double r = (y - (z - kMagic)) * 0.010830424696249145;  // ln 2 / 64
+    double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
+    p = fma(r, p, 0.5);
+    p = fma(r, p, 1.0);
+    p = fma(r, p, 1.0);
+    const double w = p * power[i & 63];
+    // times 2^(n + 45) by the exponent bits, then to an integer by the same trick
+    const double u = __hiloint2double(__double2hiint(w) + (((i >> 6) + 45) << 20), __double2loint(w)) + kMagic;
+    return uint64_t(__double_as_longlong(u)) & 0x3ffffffffffffull;
+}
 
 __device__ __forceinline__ uint64_t warp_add_u64(uint64_t v) {
 #pragma unroll
@@ -84,10 +109,10 @@ __device__ __forceinline__ uint64_t warp_scan_u64(uint64_t v, int lane) {  // in
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t sample_raw[];
     SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_raw);
-    float* x = reinterpret_cast<float*>(sample_raw + ((sizeof(SampleShared) + 15) & ~size_t(15)));
+    T* xs = reinterpret_cast<T*>(sample_raw + ((sizeof(SampleShared) + 15) & ~size_t(15)));
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), ranks = int(cluster.num_blocks());
     const int row = int(blockIdx.x) / ranks;
@@ -96,14 +121,22 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     const int per_warp = a.slice / kSampleWarps;  // a multiple of 32; a warp owns consecutive entries
     const int w0 = warp * per_warp, w1 = min(w0 + per_warp, have);
 
+    // An entry: a NaN counts as -inf, zeros of both signs are one value.
+    auto entry_value = [](T raw) -> float {
+        const float v = to_f32(raw);
+        return v != v ? -INFINITY : v + 0.f;
+    };
+    auto x = [&](int i) { return entry_value(xs[i]); };
+
     // ---- the row into shared memory; its best entry and its lowest finite one
+    if (tid < 64) sh.power[tid] = exp2(double(tid) / 64.0);
     const T* src = static_cast<const T*>(a.logits) + int64_t(row) * a.row_stride + base;
     uint64_t best = 0;
     uint32_t low = 0xffffffffu;
     for (int i = tid; i < have; i += kSampleThreads) {
-        float v = to_f32(src[i]);
-        v = v != v ? -INFINITY : v + 0.f;
-        x[i] = v;
+        const T raw = src[i];
+        xs[i] = raw;
+        const float v = entry_value(raw);
         const uint32_t key = ordered_bits(v);
         const uint64_t entry = uint64_t(key) << 32 | uint32_t(~uint32_t(base + i));
         best = best > entry ? best : entry;
@@ -150,12 +183,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     auto weight = [&](float v) -> uint64_t {
         if (v == m) return uint64_t(kSampleUnit);
         const double t = (double(v) - double(m)) * inv_t;
-        if (!(t > -32.0) || v == -INFINITY) return 0;  // rounds to zero units
-        return uint64_t(__double2ll_rn(exp(t) * kSampleUnit));
+        if (!(t > -31.9) || v == -INFINITY) return 0;  // under half a unit
+        return exp_units(t, sh.power);
     };
 
     uint64_t cut = 0;  // entries at or above it (as (ordered bits, ~index)) are kept
-    auto entry_of = [&](int i) { return uint64_t(ordered_bits(x[i])) << 32 | uint32_t(~uint32_t(base + i)); };
+    auto entry_of = [&](int i) { return uint64_t(ordered_bits(x(i))) << 32 | uint32_t(~uint32_t(base + i)); };
 
     // Sum over the cluster of the kept entries' weights (at least `least` units each).  Every thread gets the total
     // and the sum of the ranks before; warp_u64 keeps the warps' running sums.
@@ -163,7 +196,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
         uint64_t sum = 0;
         for (int i = w0 + lane; i < w1; i += 32)
             if (entry_of(i) >= cut) {
-                const uint64_t w = weight(x[i]);
+                const uint64_t w = weight(x(i));
                 sum += w >= least ? w : 0;
             }
         sum = warp_add_u64(sum);
@@ -192,113 +225,191 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     auto find_cut = [&](bool by_mass, uint32_t want, uint64_t target) {
         const float span = fminf(32.f * temp, m - from_ordered(low));
         const float per_unit = span > 0.f ? float(kSampleBins) / span : 0.f;
-        uint32_t key_lo = 0, key_hi = 0xffffffffu;
-        uint32_t before_count = 0;
+        uint32_t key_lo = 0, key_hi = 0xffffffffu;  // what is still undecided
+        uint32_t before_count = 0;                  // kept for certain: everything above key_hi
         uint64_t before_mass = 0;
-        for (int round = 0;; ++round) {
+        SampleShared* lead = cluster.map_shared_rank(&sh, 0);
+        for (int round = 0; round < 40; ++round) {
             int shift = 0;
             while (((key_hi - key_lo) >> shift) >= uint32_t(kSampleBins)) ++shift;
             auto bin_of = [&](float v, uint32_t key) -> int {
                 if (round == 0) return min(kSampleBins - 1, max(0, int((m - v) * per_unit)));
                 return int((key_hi - key) >> shift);
             };
-            auto active = [&](int i, uint32_t& key) {
-                key = ordered_bits(x[i]);
+            auto active = [&](int i, float v, uint32_t& key) {
+                key = ordered_bits(v);
                 return key >= key_lo && key <= key_hi && (uint64_t(key) << 32 | uint32_t(~uint32_t(base + i))) >= cut;
             };
-            for (int i = tid; i < kSampleBins; i += kSampleThreads)
-                sh.count[i] = sh.mass[0][i] = sh.mass[1][i] = sh.mass[2][i] = 0;
-            if (tid == 0) sh.list_fill = 0;
+            for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.count[i] = 0;
+            if (tid < 2) sh.list_fill = 0, sh.key_lo[tid] = 0xffffffffu, sh.key_hi[tid] = 0, sh.inside[tid] = 0;
             __syncthreads();
             for (int i = tid; i < have; i += kSampleThreads) {
+                const float v = x(i);
                 uint32_t key;
-                if (!active(i, key)) continue;
-                const int b = bin_of(x[i], key);
-                atomicAdd(&sh.count[b], 1u);
-                if (by_mass) {
-                    const uint64_t w = weight(x[i]);
-                    if (w) atomicAdd(&sh.mass[0][b], uint32_t(w) & 0xffffu);
-                    if (w >> 16) atomicAdd(&sh.mass[1][b], uint32_t(w >> 16) & 0xffffu);
-                    if (w >> 32) atomicAdd(&sh.mass[2][b], uint32_t(w >> 32));
-                }
+                if (active(i, v, key)) atomicAdd(&sh.count[bin_of(v, key)], 1u);
             }
             cluster.sync();
             if (rank == 0) {
-                // every thread sums a few consecutive bins over the ranks, then the bins are scanned in order
-                constexpr int kEach = kSampleBins / kSampleThreads;
-                uint32_t cnt[kEach];
-                uint64_t mass[kEach];
-                uint64_t own_mass = 0, own_count = 0;
-                for (int e = 0; e < kEach; ++e) {
-                    const int b = tid * kEach + e;
-                    cnt[e] = 0;
-                    mass[e] = 0;
-                    for (int r = 0; r < ranks; ++r) {
-                        const SampleShared* p = cluster.map_shared_rank(&sh, r);
-                        cnt[e] += p->count[b];
-                        if (by_mass)
-                            mass[e] += uint64_t(p->mass[0][b]) + (uint64_t(p->mass[1][b]) << 16) +
-                                       (uint64_t(p->mass[2][b]) << 32);
-                    }
-                    own_count += cnt[e];
-                    own_mass += mass[e];
+                // every thread sums four consecutive bins over the ranks, then the bins are scanned in order
+                static_assert(kSampleBins == 4 * kSampleThreads, "four bins a thread");
+                uint32_t cnt[4] = {0, 0, 0, 0};
+                for (int r = 0; r < ranks; ++r) {
+                    const uint4 c4 = *reinterpret_cast<const uint4*>(&cluster.map_shared_rank(&sh, r)->count[tid * 4]);
+                    cnt[0] += c4.x, cnt[1] += c4.y, cnt[2] += c4.z, cnt[3] += c4.w;
                 }
-                const uint64_t scan_c = warp_scan_u64(own_count, lane), scan_m = warp_scan_u64(own_mass, lane);
-                if (lane == 31) sh.warp_u64[warp] = scan_m, sh.warp_u32[warp] = uint32_t(scan_c);
-                if (tid == 0) sh.bin = -1;
+                // least and most a bin's entries can weigh, in units
+                double least[4], most[4];
+                uint32_t own_c = 0;
+                double own_l = 0, own_m = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int b = tid * 4 + e;
+                    least[e] = most[e] = 0;
+                    if (by_mass && cnt[e] > 0) {
+                        if (round == 0) {  // edges b / per_unit below m, give or take their rounding
+                            const double step = per_unit > 0.f ? inv_t / double(per_unit) : 0.0;
+                            most[e] = cnt[e] * kSampleUnit * exp(-step * b) * 1.001;
+                            least[e] = b == kSampleBins - 1 ? 0.0 : cnt[e] * kSampleUnit * exp(-step * (b + 1)) * 0.999;
+                        } else {
+                            const uint32_t top = key_hi - (uint32_t(b) << shift);
+                            const uint32_t end = (1u << shift) - 1u, bottom = top - key_lo < end ? key_lo : top - end;
+                            most[e] = double(cnt[e]) * double(weight(from_ordered(top)));
+                            least[e] = double(cnt[e]) * double(weight(from_ordered(bottom)));
+                        }
+                    }
+                    own_c += cnt[e];
+                    own_l += least[e];
+                    own_m += most[e];
+                }
+                double scan_l = own_l, scan_m = own_m;
+                uint32_t scan_c = own_c;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double yl = __shfl_up_sync(0xffffffffu, scan_l, o), ym = __shfl_up_sync(0xffffffffu, scan_m, o);
+                    const uint32_t yc = __shfl_up_sync(0xffffffffu, scan_c, o);
+                    if (lane >= o) scan_l += yl, scan_m += ym, scan_c += yc;
+                }
+                if (lane == 31) sh.warp_f64[0][warp] = scan_l, sh.warp_f64[1][warp] = scan_m, sh.warp_u32[warp] = scan_c;
+                if (tid == 0) sh.bin_lo = kSampleBins, sh.bin_hi = -1;
                 __syncthreads();
-                uint64_t run_m = before_mass + scan_m - own_mass;
-                uint32_t run_c = before_count + uint32_t(scan_c - own_count);
-                for (int i = 0; i < warp; ++i) run_m += sh.warp_u64[i], run_c += sh.warp_u32[i];
-                // the bin that holds the prefix's last entry
-                int mine = -1;
-                uint32_t c_at = 0;
-                uint64_t m_at = 0;
-                uint32_t n_at = 0;
-                for (int e = 0; e < kEach; ++e) {
-                    if (cnt[e] > 0 && (by_mass ? run_m < target : run_c < want)) {
-                        mine = tid * kEach + e;
-                        c_at = run_c;
-                        m_at = run_m;
-                        n_at = cnt[e];
+                uint32_t run_c = before_count + scan_c - own_c;
+                double run_l = double(before_mass) + scan_l - own_l, run_m = double(before_mass) + scan_m - own_m;
+                for (int i = 0; i < warp; ++i)
+                    run_c += sh.warp_u32[i], run_l += sh.warp_f64[0][i], run_m += sh.warp_f64[1][i];
+                // The prefix ends in the last nonempty bin that begins below the target: by counts exactly that bin, by
+                // mass between the first bin that may end at or above the target and the last that may begin below it
+                // (sums of 2^11 fp64 terms: a millionth either way is far more than their rounding).
+                int lo = kSampleBins, hi = -1;
+                uint32_t at[4];
+                const double want_mass = double(target);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    at[e] = run_c;
+                    if (cnt[e] > 0) {
+                        const int b = tid * 4 + e;
+                        if (by_mass) {
+                            if (run_l * 0.999999 < want_mass) hi = b;
+                            if ((run_m + most[e]) * 1.000001 >= want_mass) lo = min(lo, b);
+                        } else if (run_c < want) {
+                            hi = b;
+                        }
                     }
                     run_c += cnt[e];
-                    run_m += mass[e];
+                    run_l += least[e];
+                    run_m += most[e];
                 }
-                if (mine >= 0) atomicMax(&sh.bin, mine);
+                if (hi >= 0) atomicMax(&sh.bin_hi, hi);
+                if (lo < kSampleBins) atomicMin(&sh.bin_lo, lo);
                 __syncthreads();
-                if (mine >= 0 && sh.bin == mine) sh.bin_count = n_at, sh.before_count = c_at, sh.before_mass = m_at;
+                if (tid == 0) sh.bin_lo = by_mass ? min(sh.bin_lo, sh.bin_hi) : sh.bin_hi;
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (tid * 4 + e == sh.bin_lo) sh.before_count = at[e];
             }
             cluster.sync();
-            SampleShared* lead = cluster.map_shared_rank(&sh, 0);
-            const int bin = lead->bin;
-            const uint32_t bin_count = lead->bin_count;
+            const int bin_lo = lead->bin_lo, bin_hi = lead->bin_hi, middle = (bin_lo + bin_hi) >> 1;
             before_count = lead->before_count;
-            before_mass = lead->before_mass;
-            if (bin_count <= uint32_t(kSampleList)) {
-                uint32_t offset = 0;
-                for (int r = 0; r < rank; ++r) offset += cluster.map_shared_rank(&sh, r)->count[bin];
+            // ---- exactly: the masses above the bracket and of its upper half, its entries by halves and their ranges
+            uint64_t above = 0, upper = 0;
+            uint32_t inside[2] = {0, 0}, lo_key[2] = {0xffffffffu, 0xffffffffu}, hi_key[2] = {0, 0};
+            for (int i = tid; i < have; i += kSampleThreads) {
+                const float v = x(i);
+                uint32_t key;
+                if (!active(i, v, key)) continue;
+                const int b = bin_of(v, key);
+                if (b > bin_hi) continue;
+                if (b >= bin_lo) {
+                    const bool second = b > middle;
+                    inside[0] += second ? 0u : 1u;
+                    inside[1] += second ? 1u : 0u;
+                    if (second) lo_key[1] = min(lo_key[1], key), hi_key[1] = max(hi_key[1], key);
+                    else lo_key[0] = min(lo_key[0], key), hi_key[0] = max(hi_key[0], key);
+                    if (by_mass && !second && bin_hi > bin_lo) upper += weight(v);
+                } else if (by_mass) {
+                    above += weight(v);
+                }
+            }
+            if (by_mass) above = warp_add_u64(above), upper = warp_add_u64(upper);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                inside[h] = __reduce_add_sync(0xffffffffu, inside[h]);
+                lo_key[h] = __reduce_min_sync(0xffffffffu, lo_key[h]);
+                hi_key[h] = __reduce_max_sync(0xffffffffu, hi_key[h]);
+                if (lane == 0) {
+                    atomicAdd(&sh.inside[h], inside[h]);
+                    atomicMin(&sh.key_lo[h], lo_key[h]);
+                    atomicMax(&sh.key_hi[h], hi_key[h]);
+                }
+            }
+            if (lane == 0) sh.warp_u64[warp] = above, sh.list_weight[warp] = upper;
+            __syncthreads();
+            if (tid == 0) {
+                for (int i = 1; i < kSampleWarps; ++i) above += sh.warp_u64[i], upper += sh.list_weight[i];
+                sh.total = above;
+                sh.upper = upper;
+            }
+            cluster.sync();
+            uint64_t upper_all = 0;
+            for (int r = 0; r < ranks; ++r) {
+                const SampleShared* p = cluster.map_shared_rank(&sh, r);
+                before_mass += p->total;
+                upper_all += p->upper;
+            }
+            // the last kept entry is in the lower half if something behind the upper one is kept
+            const int half = by_mass && bin_hi > bin_lo && before_mass + upper_all < target ? 1 : 0;
+            uint32_t offset = 0, inside_all = 0, low_key = 0xffffffffu, high_key = 0;
+            for (int r = 0; r < ranks; ++r) {
+                const SampleShared* p = cluster.map_shared_rank(&sh, r);
+                if (r < rank) offset += p->inside[half];
+                inside_all += p->inside[half];
+                low_key = min(low_key, p->key_lo[half]);
+                high_key = max(high_key, p->key_hi[half]);
+                if (half) before_count += p->inside[0];
+            }
+            if (half) before_mass += upper_all;
+            if (inside_all <= uint32_t(kSampleList)) {
                 for (int i = tid; i < have; i += kSampleThreads) {
+                    const float v = x(i);
                     uint32_t key;
-                    if (!active(i, key) || bin_of(x[i], key) != bin) continue;
+                    if (!active(i, v, key) || key < low_key || key > high_key) continue;
                     const uint32_t at = offset + atomicAdd(&sh.list_fill, 1u);
-                    lead->list_entry[at] = entry_of(i);
-                    lead->list_weight[at] = by_mass ? weight(x[i]) : 0;
+                    lead->list_entry[at] = uint64_t(key) << 32 | uint32_t(~uint32_t(base + i));
+                    lead->list_weight[at] = by_mass ? weight(v) : 0;
                 }
                 cluster.sync();
                 if (rank == 0) {
                     // the list's last kept entry: the lowest one whose rank / mass before it still qualifies
-                    if (tid == 0) sh.cut = ~uint64_t(0);
-                    __syncthreads();
                     uint64_t kept = ~uint64_t(0);
-                    for (uint32_t i = tid; i < bin_count; i += kSampleThreads) {
-                        const uint64_t e = sh.list_entry[i];
+                    if (uint32_t(tid) < inside_all) {
+                        const uint64_t e = sh.list_entry[tid];
                         uint32_t c = before_count;
                         uint64_t ms = before_mass;
-                        for (uint32_t j = 0; j < bin_count; ++j)
+                        for (uint32_t j = 0; j < inside_all; ++j)
                             if (sh.list_entry[j] > e) ++c, ms += sh.list_weight[j];
-                        if (by_mass ? ms < target : c < want) kept = e < kept ? e : kept;
+                        if (by_mass ? ms < target : c < want) kept = e;
                     }
+                    static_assert(kSampleList <= kSampleThreads, "one entry a thread");
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) {
                         const uint64_t y = __shfl_xor_sync(0xffffffffu, kept, o);
@@ -308,54 +419,35 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
                     __syncthreads();
                     if (tid == 0) {
                         for (int i = 1; i < kSampleWarps; ++i) kept = sh.warp_u64[i] < kept ? sh.warp_u64[i] : kept;
-                        sh.cut = kept;
+                        // none in the bracket: everything above it
+                        sh.cut = kept != ~uint64_t(0) ? kept : (uint64_t(high_key) + 1) << 32;
                     }
                 }
                 cluster.sync();
                 cut = lead->cut;
                 return;
             }
-            // too many for the list: the range of the bin's ordered bits
-            uint32_t lo_key = 0xffffffffu, hi_key = 0;
-            for (int i = tid; i < have; i += kSampleThreads) {
-                uint32_t key;
-                if (!active(i, key) || bin_of(x[i], key) != bin) continue;
-                lo_key = min(lo_key, key);
-                hi_key = max(hi_key, key);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                lo_key = min(lo_key, __shfl_xor_sync(0xffffffffu, lo_key, o));
-                hi_key = max(hi_key, __shfl_xor_sync(0xffffffffu, hi_key, o));
-            }
-            if (tid == 0) sh.key_lo = 0xffffffffu, sh.key_hi = 0;
-            __syncthreads();
-            if (lane == 0) atomicMin(&sh.key_lo, lo_key), atomicMax(&sh.key_hi, hi_key);
-            cluster.sync();
-            lo_key = 0xffffffffu;
-            hi_key = 0;
-            for (int r = 0; r < ranks; ++r) {
-                const SampleShared* p = cluster.map_shared_rank(&sh, r);
-                lo_key = min(lo_key, p->key_lo);
-                hi_key = max(hi_key, p->key_hi);
-            }
             cluster.sync();  // read by every rank before it is written again
-            key_lo = lo_key;
-            key_hi = hi_key;
+            key_lo = low_key;
+            key_hi = high_key;
             if (key_lo != key_hi) continue;
-            // one value fills the bin: its first entries by index are kept
+            // one value fills the bracket: its first entries by index are kept
             uint32_t need = want - before_count;
             if (by_mass) {
                 const uint64_t w = weight(from_ordered(key_lo));
-                const uint64_t left = target - before_mass;  // > 0: the bin was chosen by before_mass < target
-                const uint64_t n = w ? (left + w - 1) / w : bin_count;
-                need = uint32_t(n < bin_count ? n : bin_count);
+                const uint64_t left = target > before_mass ? target - before_mass : 0;
+                const uint64_t n = w ? (left + w - 1) / w : (left ? inside_all : 0);
+                need = uint32_t(n < inside_all ? n : inside_all);
+            }
+            if (need == 0) {
+                cut = (uint64_t(key_hi) + 1) << 32;
+                return;
             }
             // ties in the ranks, then the warps, before this one
             uint32_t mine = 0;
             for (int i = w0 + lane; i < w1; i += 32) {
                 uint32_t key;
-                mine += active(i, key) ? 1u : 0u;
+                mine += active(i, x(i), key) ? 1u : 0u;
             }
             mine = __reduce_add_sync(0xffffffffu, mine);
             __syncthreads();
@@ -364,17 +456,17 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
             if (tid == 0) {
                 uint32_t run = 0;
                 for (int i = 0; i < kSampleWarps; ++i) run += sh.warp_u32[i];
-                sh.list_fill = run;
+                sh.inside[0] = run;
             }
             cluster.sync();
             uint32_t run = 0;
-            for (int r = 0; r < rank; ++r) run += cluster.map_shared_rank(&sh, r)->list_fill;
+            for (int r = 0; r < rank; ++r) run += cluster.map_shared_rank(&sh, r)->inside[0];
             for (int i = 0; i < warp; ++i) run += sh.warp_u32[i];
             if (run < need && need <= run + mine) {
                 for (int i0 = w0; i0 < w1; i0 += 32) {
                     const int i = i0 + lane;
                     uint32_t key = 0;
-                    const bool hit = i < w1 && active(i, key);
+                    const bool hit = i < w1 && active(i, x(i), key);
                     const uint32_t vote = __ballot_sync(0xffffffffu, hit);
                     const uint32_t nth = run + __popc(vote & ((2u << lane) - 1u));
                     if (hit && nth == need) lead->cut = entry_of(i);
@@ -414,7 +506,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
                 const int i = i0 + lane;
                 uint64_t w = 0;
                 if (i < w1 && entry_of(i) >= cut) {
-                    w = weight(x[i]);
+                    w = weight(x(i));
                     if (w < least) w = 0;
                 }
                 const uint64_t upto = run + warp_scan_u64(w, lane);

@@ -395,7 +395,8 @@ void sample_tokens(const ServeDevice&, const b2d_sample_request* rq, cudaStream_
     int ranks = 1;
     while (ranks < kSampleMaxCluster && a.vocab > 4096 * ranks) ranks *= 2;
     a.slice = ((a.vocab + ranks - 1) / ranks + kSampleThreads - 1) / kSampleThreads * kSampleThreads;
-    const size_t smem = ((sizeof(SampleShared) + 15) & ~size_t(15)) + size_t(a.slice) * 4;
+    const size_t elem = rq->logits_type == B2D_TYPE_F32 ? 4 : 2;
+    const size_t smem = ((sizeof(SampleShared) + 15) & ~size_t(15)) + size_t(a.slice) * elem;
     constexpr int kLimit = int((sizeof(SampleShared) + 15) & ~size_t(15)) + kSampleMaxSlice * 4;
     auto go = [&](auto kernel) {
         set_smem_limit(kernel, kLimit);
