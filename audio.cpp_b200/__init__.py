@@ -257,22 +257,33 @@ def _ptr(a) -> int:
     return a.ctypes.data
 
 
-# torch dtypes by name (this layer does not import torch)
+# torch dtypes by name (this layer does not import torch), and the same by dtype object, filled as they are met
 _TENSOR_TYPES = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16,
-                 "torch.int8": TYPE_I8, "torch.float8_e4m3fn": TYPE_E4M3}
+                 "torch.int8": TYPE_I8, "torch.float8_e4m3fn": TYPE_E4M3, "torch.int32": -32}
+_DTYPES: Dict[object, int] = {}
+_INT32 = -32
+_FLOATS = (TYPE_F32, TYPE_F16, TYPE_BF16)
+
+
+def _dtype(t) -> int:
+    kind = _DTYPES.get(t.dtype)
+    if kind is None:
+        kind = _DTYPES[t.dtype] = _TENSOR_TYPES.get(str(t.dtype), -1)
+    return kind
 
 
 def _tensor_type(t, allowed, what: str) -> int:
-    got = _TENSOR_TYPES.get(str(t.dtype))
+    got = _dtype(t)
     if got not in allowed:
         raise B2DError(-1, "%s of type %s" % (what, t.dtype))
     return got
 
 
-def _want(t, what: str, shape, dtype: str, device=None):
+def _want(t, what: str, shape, kind: int, device=None):
     """A contiguous tensor of this shape and type (on this device), or a refusal."""
-    if tuple(t.shape) != tuple(shape) or str(t.dtype) != dtype or not t.is_contiguous():
-        raise B2DError(-1, "%s must be a contiguous %s tensor of shape %s" % (what, dtype, tuple(shape)))
+    if t.shape != shape or _dtype(t) != kind or not t.is_contiguous():
+        name = next(n for n, k in _TENSOR_TYPES.items() if k == kind)
+        raise B2DError(-1, "%s must be a contiguous %s tensor of shape %s" % (what, name, tuple(shape)))
     if device is not None and t.device != device:
         raise B2DError(-1, "%s is on %s, not on %s" % (what, t.device, device))
     return t
@@ -294,16 +305,18 @@ class PagedCache:
         if kind in (TYPE_I8, TYPE_E4M3):
             if k_scale is None or v_scale is None:
                 raise B2DError(-1, "an 8-bit paged cache needs its scales")
-            _want(k_scale, "k_scale", k.shape[:3], "torch.float32", k.device)
-            _want(v_scale, "v_scale", k.shape[:3], "torch.float32", k.device)
+            _want(k_scale, "k_scale", k.shape[:3], TYPE_F32, k.device)
+            _want(v_scale, "v_scale", k.shape[:3], TYPE_F32, k.device)
         else:
             k_scale = v_scale = None
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.type, self.device = kind, k.device
+        self.type, self.device = kind, k.get_device()
         pages, kv_heads, page_size, head_dim = k.shape
+        self.page_size, self.kv_heads, self.head_dim = page_size, kv_heads, head_dim
         self.desc = KvCacheDesc(kind, page_size, pages, kv_heads, head_dim, k.stride(0), k.stride(1), k.stride(2),
                                 k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
                                 v_scale.data_ptr() if v_scale is not None else None)
+        self.ref = C.byref(self.desc)
 
 
 class PagedBatch:
@@ -312,26 +325,31 @@ class PagedBatch:
 
     def __init__(self, row_start, context, page_table, rows: int, max_new: int, max_context: int):
         seqs = context.shape[0]
-        _want(context, "context", (seqs,), "torch.int32")
-        _want(row_start, "row_start", (seqs + 1,), "torch.int32", context.device)
-        if page_table.dim() != 2 or page_table.shape[0] != seqs or str(page_table.dtype) != "torch.int32" or \
+        _want(context, "context", (seqs,), _INT32)
+        _want(row_start, "row_start", (seqs + 1,), _INT32, context.device)
+        if page_table.dim() != 2 or page_table.shape[0] != seqs or _dtype(page_table) != _INT32 or \
                 (page_table.numel() and page_table.stride(1) != 1) or page_table.device != context.device:
             raise B2DError(-1, "page_table must be an int32 tensor [seqs, pages] with contiguous rows")
         self.row_start, self.context, self.page_table = row_start, context, page_table
-        self.rows, self.device = rows, context.device
+        self.rows, self.device = rows, context.get_device()
         stride = page_table.stride(0) if seqs > 1 else page_table.shape[1]
         if stride < page_table.shape[1]:
             raise B2DError(-1, "page_table rows overlap")
-        self.table_pages = page_table.shape[1]
+        self.table_pages, self.max_context = page_table.shape[1] if seqs else 1 << 40, max_context
         self.desc = KvBatchDesc(seqs, max_new, max_context, rows, row_start.data_ptr(), context.data_ptr(),
                                 page_table.data_ptr(), stride)
+        self.ref = C.byref(self.desc)
+
+    def fits(self, cache: PagedCache) -> None:
+        """Refuses a table whose rows do not hold max_context (the library sees their stride, not their width)."""
+        if self.table_pages * cache.page_size < self.max_context:
+            raise B2DError(-1, "page_table rows of %d pages do not hold max_context %d"
+                           % (self.table_pages, self.max_context))
 
 
 def check_paged(cache: PagedCache, batch: PagedBatch, heads: int = 0) -> None:
     """The checks that the calls make of a cache, a batch and (unless 0) the query heads; needs no GPU."""
-    if batch.desc.seqs and -(-batch.desc.max_context // cache.desc.page_size) > batch.table_pages:
-        raise B2DError(-1, "page_table rows of %d pages do not hold max_context %d"
-                       % (batch.table_pages, batch.desc.max_context))
+    batch.fits(cache)
     err = C.create_string_buffer(256)
     st = lib().b2d_kv_check(C.byref(cache.desc), C.byref(batch.desc), heads, err, 256)
     if st != 0:
@@ -411,61 +429,70 @@ class Context:
                                          C.c_void_p(stream)))
 
     # ------------------------------------------------------- serving operators
-    def _on_device(self, *tensors) -> None:
-        for t in tensors:
-            if t is not None and (t.device.type != "cuda" or t.device.index != self.device):
-                raise B2DError(-1, "tensor on %s; this context's device is cuda:%d" % (t.device, self.device))
+    # The library checks descriptions, sizes, strides and alignment; what it cannot see is checked here: that tensors
+    # have the shapes, types and device the call takes them to have.
+    def _elsewhere(self, what: str):
+        return B2DError(-1, "%s is not on this context's device cuda:%d" % (what, self.device))
 
     def _cache_rows(self, cache: PagedCache, batch: PagedBatch, k, v):
         """(element type, row stride) of k / v rows [rows, kv_heads, head_dim] whose last two dimensions are packed."""
-        check_paged(cache, batch)
-        kind = _tensor_type(k, (TYPE_F32, TYPE_F16, TYPE_BF16), "cache rows")
-        shape = (batch.rows, cache.desc.kv_heads, cache.desc.head_dim)
-        for t in (k, v):
-            if tuple(t.shape) != shape or t.dtype != k.dtype or t.stride(2) != 1 or t.stride(1) != shape[2] or \
-                    t.stride(0) != k.stride(0):
-                raise B2DError(-1, "cache rows must be alike, [rows, kv_heads, head_dim] = %s, heads packed" % (shape,))
-        self._on_device(cache.k, batch.context, k, v)
-        return kind, k.stride(0) if batch.rows > 1 else shape[1] * shape[2]
+        batch.fits(cache)
+        kind = _tensor_type(k, _FLOATS, "cache rows")
+        shape = (batch.rows, cache.kv_heads, cache.head_dim)
+        stride = k.stride()
+        if k.shape != shape or v.shape != shape or v.dtype != k.dtype or stride[2] != 1 or stride[1] != shape[2] or \
+                v.stride() != stride:
+            raise B2DError(-1, "cache rows must be alike, [rows, kv_heads, head_dim] = %s, heads packed" % (shape,))
+        dev = self.device
+        if k.get_device() != dev or v.get_device() != dev or cache.device != dev or batch.device != dev:
+            raise self._elsewhere("a cache, batch or rows tensor")
+        return kind, stride[0] if shape[0] > 1 else shape[1] * shape[2]
 
     def kv_append(self, cache: PagedCache, batch: PagedBatch, k, v, stream: int = 0) -> None:
         """Writes the batch's rows into the cache, quantising them to its type (b2d_kv_append)."""
         kind, stride = self._cache_rows(cache, batch, k, v)
-        self.check(lib().b2d_kv_append(self._h, C.byref(cache.desc), C.byref(batch.desc), kind, _ptr(k), _ptr(v), stride,
-                                       C.c_void_p(stream)))
+        st = lib().b2d_kv_append(self._h, cache.ref, batch.ref, kind, k.data_ptr(), v.data_ptr(), stride, stream)
+        if st:
+            self.check(st)
 
     def kv_gather(self, cache: PagedCache, batch: PagedBatch, k_out, v_out, stream: int = 0) -> None:
         """Reads the batch's rows back as the values they stand for (b2d_kv_gather)."""
         kind, stride = self._cache_rows(cache, batch, k_out, v_out)
-        self.check(lib().b2d_kv_gather(self._h, C.byref(cache.desc), C.byref(batch.desc), kind, _ptr(k_out), _ptr(v_out),
-                                       stride, C.c_void_p(stream)))
+        st = lib().b2d_kv_gather(self._h, cache.ref, batch.ref, kind, k_out.data_ptr(), v_out.data_ptr(), stride, stream)
+        if st:
+            self.check(st)
 
     def paged_attention_workspace(self, cache: PagedCache, batch: PagedBatch, heads: int) -> int:
         """Bytes of workspace paged_attention needs for batches of these bounds."""
         check_paged(cache, batch, heads)
-        return lib().b2d_paged_attention_workspace(self._h, C.byref(cache.desc), C.byref(batch.desc), heads)
+        return lib().b2d_paged_attention_workspace(self._h, cache.ref, batch.ref, heads)
 
     def paged_attention(self, q, cache: PagedCache, batch: PagedBatch, out, scale: Optional[float] = None,
                         window: int = 0, workspace=None, stream: int = 0) -> None:
         """Causal attention of the batch's rows over the cache (b2d_paged_attention): q, out [rows, heads, head_dim]
         float16 or bfloat16 with packed heads; scale defaults to head_dim ** -0.5; workspace: a uint8 tensor of
         paged_attention_workspace bytes (calls that may overlap need one each)."""
-        hd = cache.desc.head_dim
-        if q.dim() != 3 or q.shape[0] != batch.rows or q.shape[2] != hd:
+        hd = cache.head_dim
+        shape, qs, os_ = q.shape, q.stride(), out.stride()
+        if len(shape) != 3 or shape[0] != batch.rows or shape[2] != hd:
             raise B2DError(-1, "paged attention queries must be [rows, heads, head_dim]")
-        heads = q.shape[1]
-        check_paged(cache, batch, heads)
+        batch.fits(cache)
         kind = _tensor_type(q, (TYPE_F16, TYPE_BF16), "paged attention queries")
-        for t in (q, out):
-            if t.shape != q.shape or t.dtype != q.dtype or t.stride(2) != 1 or t.stride(1) != hd:
-                raise B2DError(-1, "paged attention q and out must be alike with packed heads")
-        self._on_device(cache.k, batch.context, q, out, workspace)
-        rows = [t.stride(0) if batch.rows > 1 else heads * hd for t in (q, out)]
-        self.check(lib().b2d_paged_attention(
-            self._h, C.byref(cache.desc), C.byref(batch.desc), int(kind == TYPE_BF16), _ptr(q), rows[0], _ptr(out),
-            rows[1], heads, float(hd ** -0.5 if scale is None else scale), window,
-            _ptr(workspace) if workspace is not None else None, workspace.numel() if workspace is not None else 0,
-            C.c_void_p(stream)))
+        if out.shape != shape or out.dtype != q.dtype or qs[2] != 1 or qs[1] != hd or os_[2] != 1 or os_[1] != hd:
+            raise B2DError(-1, "paged attention q and out must be alike with packed heads")
+        dev = self.device
+        if q.get_device() != dev or out.get_device() != dev or cache.device != dev or batch.device != dev or \
+                (workspace is not None and workspace.get_device() != dev):
+            raise self._elsewhere("a cache, batch, query, output or workspace tensor")
+        heads = shape[1]
+        many = shape[0] > 1
+        st = lib().b2d_paged_attention(
+            self._h, cache.ref, batch.ref, 1 if kind == TYPE_BF16 else 0, q.data_ptr(), qs[0] if many else heads * hd,
+            out.data_ptr(), os_[0] if many else heads * hd, heads, hd ** -0.5 if scale is None else scale, window,
+            workspace.data_ptr() if workspace is not None else None, workspace.nbytes if workspace is not None else 0,
+            stream)
+        if st:
+            self.check(st)
 
     def sample_tokens(self, logits, temperature, top_k, top_p, min_p, uniform, tokens, probs=None,
                       stream: int = 0) -> None:
@@ -473,20 +500,26 @@ class Context:
         None.  temperature, top_p, min_p, uniform, probs: float32 [rows]; top_k, tokens: int32 [rows]."""
         if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1):
             raise B2DError(-1, "logits must be [rows, vocab] with contiguous rows")
-        kind = _tensor_type(logits, (TYPE_F32, TYPE_F16, TYPE_BF16), "logits")
+        kind = _tensor_type(logits, _FLOATS, "logits")
         rows, vocab = logits.shape
-        for name, t, dtype in (("temperature", temperature, "torch.float32"), ("top_k", top_k, "torch.int32"),
-                               ("top_p", top_p, "torch.float32"), ("min_p", min_p, "torch.float32"),
-                               ("uniform", uniform, "torch.float32"), ("tokens", tokens, "torch.int32"),
-                               ("probs", probs, "torch.float32")):
-            if t is not None:
-                _want(t, name, (rows,), dtype)
-        self._on_device(logits, temperature, top_k, top_p, min_p, uniform, tokens, probs)
-        rq = SampleRequest(kind, rows, vocab, logits.stride(0) if rows > 1 else vocab, _ptr(logits), _ptr(temperature),
-                           _ptr(top_k) if top_k is not None else None, _ptr(top_p) if top_p is not None else None,
-                           _ptr(min_p) if min_p is not None else None, _ptr(uniform), _ptr(tokens),
-                           _ptr(probs) if probs is not None else None)
-        self.check(lib().b2d_sample_tokens(self._h, C.byref(rq), C.c_void_p(stream)))
+        dev = self.device
+        if logits.get_device() != dev:
+            raise self._elsewhere("logits")
+        at = [logits.data_ptr()]
+        for name, t, want in (("temperature", temperature, TYPE_F32), ("top_k", top_k, _INT32), ("top_p", top_p, TYPE_F32),
+                              ("min_p", min_p, TYPE_F32), ("uniform", uniform, TYPE_F32), ("tokens", tokens, _INT32),
+                              ("probs", probs, TYPE_F32)):
+            if t is None:
+                at.append(None)
+                continue
+            _want(t, name, (rows,), want)
+            if t.get_device() != dev:
+                raise self._elsewhere(name)
+            at.append(t.data_ptr())
+        st = lib().b2d_sample_tokens(self._h, C.byref(SampleRequest(kind, rows, vocab,
+                                                                    logits.stride(0) if rows > 1 else vocab, *at)), stream)
+        if st:
+            self.check(st)
 
 
 WeightSpec = Tuple[str, int, Tuple[int, ...], np.ndarray]  # (name, ggml type, dims, raw payload)

@@ -82,16 +82,25 @@ __device__ __forceinline__ float pool_scale(float amax, bool finite) {
     return s < 7.888609052210118e-31f ? 0.f : s;  // 2^-100
 }
 
+// The code of x / scale, rounded from the exact quotient, with inv = 1 / scale to fp32.  The product x inv is off by less
+// than 2^-22 of itself, so it rounds like the quotient unless it lies that close to a half-way point; int8 sees that
+// from the exact remainder x - n scale, e4m3 by rounding a little above and a little below.
 template <int POOL>
-__device__ __forceinline__ uint8_t pool_code(float x, float scale) {
-    if (!(scale > 0.f)) return 0;  // zero vector, or one that reads back as NaN whatever its codes
-    const float y = div_to_odd(x, scale);
+__device__ __forceinline__ uint8_t pool_code(float x, float scale, float inv) {
+    const float t = x * inv;
     if constexpr (POOL == kPoolI8) {
-        return uint8_t(int8_t(fminf(fmaxf(rintf(y), -127.f), 127.f)));
+        float n = rintf(t);
+        const float r = __fmaf_rn(-n, scale, x), half = 0.5f * scale;
+        if (fabsf(r) >= half) {  // n is a neighbour's, or a tie
+            if (fabsf(r) > half || (int(n) & 1)) n += r > 0.f ? 1.f : -1.f;
+        }
+        return uint8_t(int8_t(fminf(fmaxf(n, -127.f), 127.f)));
     } else {
-        uint16_t r;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(y));
-        return uint8_t(r & 0xff);
+        uint16_t two;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(t * 1.0000005f), "f"(t * 0.9999995f));
+        if ((two >> 8) != (two & 0xff))
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(div_to_odd(x, scale)));
+        return uint8_t(two & 0xff);
     }
 }
 
@@ -228,10 +237,12 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, BatchView b, 
             }
             if (page < 0) continue;
             const float scale = pool_scale<POOL>(amax, fin != 0);
+            const bool live_scale = scale > 0.f;  // else zeros, or a vector that reads back as NaN whatever its codes
+            const float inv = __frcp_rn(scale);
             uint2 codes;
             uint8_t* c = reinterpret_cast<uint8_t*>(&codes);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = pool_code<POOL>(x[e], scale);
+            for (int e = 0; e < 8; ++e) c[e] = live_scale ? pool_code<POOL>(x[e], scale, inv) : uint8_t(0);
             *reinterpret_cast<uint2*>((is_v ? kv.v : kv.k) + slot_offset(kv, page, head, at.pos) + lane * 8) = codes;
             if (lane == 0) (is_v ? kv.vs : kv.ks)[scale_index(kv, page, head, at.pos)] = scale;
         }

@@ -65,28 +65,66 @@ __device__ __forceinline__ UnitSpan unit_span(const PagedArgs& a, int seq, bool 
 __device__ __forceinline__ int64_t seq_tiles(const PagedArgs& a, const UnitSpan& u) {
     return int64_t(u.tiles) * u.row_tiles * a.kv.kv_heads;
 }
-__device__ __forceinline__ int64_t run_begin(int64_t total, int run, int runs) { return total * run / runs; }
-// The run that tile t falls into.
-__device__ __forceinline__ int run_of(int64_t total, int64_t t, int runs) {
-    int r = int(t * runs / total);
-    while (run_begin(total, r + 1, runs) <= t) ++r;
-    while (run_begin(total, r, runs) > t) --r;
-    return r;
+// The list cut into as many equal runs as there are CTAs for it, none of them empty: the first `extra` have one tile more.
+struct Runs {
+    int64_t each;
+    int extra, count;
+    __device__ __forceinline__ Runs(int64_t total, int most) {
+        count = int(total < most ? total : most);
+        each = count > 0 ? total / count : 0;
+        extra = count > 0 ? int(total - each * count) : 0;
+    }
+    __device__ __forceinline__ int64_t begin(int r) const { return each * r + (r < extra ? r : extra); }
+    __device__ __forceinline__ int of(int64_t tile) const {  // the run that a tile falls into
+        const int64_t longer = (each + 1) * extra;
+        return int(tile < longer ? tile / (each + 1) : extra + (tile - longer) / each);
+    }
+};
+
+// Block-wide sums of tiles: over all sequences, and over those before `upto`.  sm: two per warp.
+template <int ROWS>
+__device__ __forceinline__ void count_tiles(const PagedArgs& a, int upto, int64_t* sm, bool report, int64_t& total,
+                                            int64_t& before) {
+    int64_t all = 0, some = 0;
+    for (int s = threadIdx.x; s < a.b.seqs; s += blockDim.x) {
+        const int64_t t = seq_tiles(a, unit_span<ROWS>(a, s, report));
+        all += t;
+        some += s < upto ? t : 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+        some += __shfl_xor_sync(0xffffffffu, some, o);
+    }
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = all, sm[(blockDim.x >> 5) + (threadIdx.x >> 5)] = some;
+    __syncthreads();
+    total = before = 0;
+    for (int w = 0; w < int(blockDim.x >> 5); ++w) total += sm[w], before += sm[(blockDim.x >> 5) + w];
 }
 
-// Block-wide: tiles of all sequences before `upto` (all threads get the sum; upto = seqs gives the total).
+// Warp-wide: the sequence that holds tile `at` of the list, and the tile's place in it.
 template <int ROWS>
-__device__ __forceinline__ int64_t tiles_before(const PagedArgs& a, int upto, int64_t* sm, bool report) {
-    int64_t sum = 0;
-    for (int s = threadIdx.x; s < upto; s += blockDim.x) sum += seq_tiles(a, unit_span<ROWS>(a, s, report));
+__device__ __forceinline__ int find_tile(const PagedArgs& a, int64_t at, int64_t& off) {
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < a.b.seqs; s0 += 32) {
+        const int s = s0 + lane;
+        const int64_t t = s < a.b.seqs ? seq_tiles(a, unit_span<ROWS>(a, s, false)) : 0;
+        int64_t upto = t;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    int64_t all = 0;
-    for (int w = 0; w < int(blockDim.x >> 5); ++w) all += sm[w];
-    return all;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, upto > at);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            off = at - __shfl_sync(0xffffffffu, upto - t, l);
+            return s0 + l;
+        }
+        at -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    off = 0;
+    return 0;
 }
 
 // ---- fragments ---------------------------------------------------------------------------------------------
@@ -179,27 +217,21 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
     constexpr int ROWS = Sh::kRows, KW = Sh::kKw, VW = Sh::kVw, MT = HD / 16;
     using MT16 = typename std::conditional<kWide, CT, __half>::type;  // the products' 16-bit type
     extern __shared__ float pa_sm[];  // [warp][row][HD] O, then [warp][row] (m, l)
-    __shared__ int64_t red[kPaWarps];
+    __shared__ int64_t red[2 * kPaWarps];
+    pdl_trigger();  // the joining kernel may get ready
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     float* sm_o = pa_sm;
     float2* sm_ml = reinterpret_cast<float2*>(pa_sm + kPaWarps * ROWS * HD);
 
-    const int64_t total = tiles_before<ROWS>(a, a.b.seqs, red, blockIdx.x == 0);
-    if (total == 0) return;
-    const int runs = int(gridDim.x);
-    int64_t at = run_begin(total, blockIdx.x, runs);
-    const int64_t end = run_begin(total, blockIdx.x + 1, runs);
-    if (at >= end) return;
-    // the sequence that holds the run's first tile
-    int seq = 0;
-    int64_t off = at;
-    UnitSpan u;
-    for (;; ++seq) {
-        u = unit_span<ROWS>(a, seq, false);
-        const int64_t t = seq_tiles(a, u);
-        if (off < t) break;
-        off -= t;
-    }
+    int64_t total, none;
+    count_tiles<ROWS>(a, 0, red, blockIdx.x == 0, total, none);
+    const Runs runs(total, int(gridDim.x));
+    if (int(blockIdx.x) >= runs.count) return;
+    int64_t at = runs.begin(blockIdx.x);
+    const int64_t end = runs.begin(blockIdx.x + 1);
+    int64_t off;
+    int seq = find_tile<ROWS>(a, at, off);
+    UnitSpan u = unit_span<ROWS>(a, seq, false);
     bool first_segment = true;
     while (at < end) {
         if (off >= seq_tiles(a, u)) {
@@ -525,8 +557,8 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
 // Joins the parts of the units that several runs share (and writes the zeros of rows in empty contexts).  Grid:
 // (sequence x row tile x kv head, row of the tile); `runs` is the stream kernel's grid.
 template <typename CT, int HD, int ROWS>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a, int runs, int row_tiles) {
-    __shared__ int64_t red[8];
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a, int most_runs, int row_tiles) {
+    __shared__ int64_t red[16];
     __shared__ float sm_x[8][HD];
     __shared__ float2 sm_ml[8];
     const int seq = blockIdx.x / (row_tiles * a.kv.kv_heads), unit = blockIdx.x % (row_tiles * a.kv.kv_heads);
@@ -536,26 +568,27 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a, int
     if (rt >= u.row_tiles || row >= u.s.n * a.group) return;
     CT* out = static_cast<CT*>(a.o) + int64_t(u.s.first + row / a.group) * a.o_row +
               int64_t(head * a.group + row % a.group) * HD;
+    int64_t total, first;
+    count_tiles<ROWS>(a, seq, red, false, total, first);
+    pdl_wait();  // the parts are written
     if (u.tiles == 0) {
         for (int d = threadIdx.x; d < HD; d += blockDim.x) out[d] = from_f32<CT>(0.f);
         return;
     }
-    const int64_t total = tiles_before<ROWS>(a, a.b.seqs, red, false);
-    const int64_t first = tiles_before<ROWS>(a, seq, red, false) + int64_t(unit) * u.tiles;
-    const int r0 = run_of(total, first, runs), r1 = run_of(total, first + u.tiles - 1, runs);
+    first += int64_t(unit) * u.tiles;
+    const Runs runs(total, most_runs);
+    const int r0 = runs.of(first), r1 = runs.of(first + u.tiles - 1);
     if (r0 == r1) return;  // one run held the whole unit and wrote it
     // run r0 began before the unit or exactly at it; in both cases this unit is its last segment
+    const bool r0_before = runs.begin(r0) < first;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto slot_of = [&](int run) -> int64_t {
-        return 2 * int64_t(run) + (run == r0 && run_begin(total, run, runs) < first ? 1 : 0);
-    };
     float m = -INFINITY, l = 0.f;
     float x[(HD + 31) / 32];
 #pragma unroll
     for (int e = 0; e < HD / 32; ++e) x[e] = 0.f;
+#pragma unroll 4
     for (int run = r0 + warp; run <= r1; run += 8) {
-        if (run_begin(total, run, runs) >= run_begin(total, run + 1, runs)) continue;
-        const int64_t slot = slot_of(run) * ROWS + r;
+        const int64_t slot = (2 * int64_t(run) + (run == r0 && r0_before ? 1 : 0)) * ROWS + r;
         const float2 ml = a.part_ml[slot];
         const float mn = fmaxf(m, ml.x);
         const float f0 = m == mn ? 1.f : ex2_approx(m - mn), f1 = ml.x == mn ? 1.f : ex2_approx(ml.x - mn);

@@ -246,6 +246,7 @@ void launch_stream(const AttentionLaunch& x) {
     launch_k(kernel, dim3(unsigned(runs)), dim3(kPaWarps * 32), Sh::kSmem, x.st, 1, x.a);
     const int64_t units = int64_t(x.a.b.seqs) * x.row_tiles * x.a.kv.kv_heads;
     if (units > 0x7fffffff) fail(B2D_EINVAL, "paged attention batch is too large");
+    const PdlScope early;  // it gets ready while the runs work, and waits for them before it reads
     launch_k(paged_merge_kernel<CT, HD, Sh::kRows>, dim3(unsigned(units), unsigned(Sh::kRows)), dim3(256), 0, x.st, 1, x.a,
              runs, x.row_tiles);
 }
