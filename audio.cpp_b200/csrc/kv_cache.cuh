@@ -197,7 +197,7 @@ __device__ __forceinline__ int64_t scale_index(const KvView& kv, int page, int h
 // 16-bit sources (two of fp32), 8-byte stores of 8-bit pools, the largest magnitude found by shuffles, nothing
 // staged in shared memory but the batch description.
 template <typename Src, int POOL>
-__global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, BatchView b, const Src* __restrict__ k,
+__global__ void __launch_bounds__(256, 8) kv_append_kernel(KvView kv, BatchView b, const Src* __restrict__ k,
                                                         const Src* __restrict__ v, int64_t row_stride) {
     extern __shared__ int kv_batch_sm[];
     int* start = kv_batch_sm;
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, BatchView b, 
 // the destination type); a row without a place reads as zeros, rows of no sequence are left as they were.  Bound by
 // HBM like the write above, same division of the work.
 template <typename Dst, int POOL>
-__global__ void __launch_bounds__(256) kv_gather_kernel(KvView kv, BatchView b, Dst* __restrict__ k,
+__global__ void __launch_bounds__(256, 8) kv_gather_kernel(KvView kv, BatchView b, Dst* __restrict__ k,
                                                         Dst* __restrict__ v, int64_t row_stride) {
     extern __shared__ int kv_batch_sm[];
     int* start = kv_batch_sm;

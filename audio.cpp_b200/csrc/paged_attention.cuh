@@ -205,7 +205,7 @@ struct PagedShape {
     static constexpr int kKPiece = (kKw < 4 ? kKw : 4) * 4;  // bytes of one load
     static constexpr int kVPiece = (kVw < 4 ? kVw : 4) * 4;
     // CTAs an SM holds: what the registers allow without spilling (the O accumulators of 16 rows of 128 take 64)
-    static constexpr int kMinBlocks = (kWide ? 3 : 4) - (HD == 128 && NT == 2 ? 1 : 0);
+    static constexpr int kMinBlocks = HD == 128 ? (NT == 1 ? 3 : 2) : kWide ? 3 : 4;
     static constexpr size_t kSmem = size_t(kPaWarps) * kRows * (HD + 2) * 4;
 };
 
