@@ -26,6 +26,7 @@ struct KvView {
     int64_t page_stride, head_stride, token_stride;  // bytes
     int64_t pages;
     int page_shift;
+    int head_shift;  // log2 kv_heads, or -1
     int kv_heads;
     int head_dim;
 };
@@ -82,26 +83,53 @@ __device__ __forceinline__ float pool_scale(float amax, bool finite) {
     return s < 7.888609052210118e-31f ? 0.f : s;  // 2^-100
 }
 
-// The code of x / scale, rounded from the exact quotient, with inv = 1 / scale to fp32.  The product x inv is off by less
-// than 2^-22 of itself, so it rounds like the quotient unless it lies that close to a half-way point; int8 sees that
-// from the exact remainder x - n scale, e4m3 by rounding a little above and a little below.
+// The codes of eight x / scale, rounded from the exact quotients, with inv = 1 / scale to fp32.  A product x inv is off by
+// less than 2^-22 of itself, so it rounds like the quotient unless that lies so close to a half-way point; int8 sees it
+// from the exact remainder x - n scale, e4m3 by rounding a little above and a little below.  Such vectors are rare and
+// are done again from quotients rounded to odd.  (The write is bound by instructions as much as by HBM: conversions to
+// integers, a quarter of the rate of the rest, are avoided by adding 1.5 2^23, which leaves the integer in the low bits.)
 template <int POOL>
-__device__ __forceinline__ uint8_t pool_code(float x, float scale, float inv) {
-    const float t = x * inv;
+__device__ __forceinline__ uint2 pool_codes(const float (&x)[8], float scale, float inv) {
+    uint32_t w[2];
     if constexpr (POOL == kPoolI8) {
-        float n = rintf(t);
-        const float r = __fmaf_rn(-n, scale, x), half = 0.5f * scale;
-        if (fabsf(r) >= half) {  // n is a neighbour's, or a tie
-            if (fabsf(r) > half || (int(n) & 1)) n += r > 0.f ? 1.f : -1.f;
+        constexpr float kMagic = 12582912.f;
+        float far = 0.f;
+        uint32_t u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float z = __fadd_rn(__fmul_rn(x[e], inv), kMagic);
+            u[e] = __float_as_uint(z);
+            far = fmaxf(far, fabsf(__fmaf_rn(-__fsub_rn(z, kMagic), scale, x[e])));
         }
-        return uint8_t(int8_t(fminf(fmaxf(n, -127.f), 127.f)));
+        if (far >= 0.5f * scale) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__fadd_rn(div_to_odd(x[e], scale), kMagic));
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            w[h] = __byte_perm(__byte_perm(u[4 * h], u[4 * h + 1], 0x0040), __byte_perm(u[4 * h + 2], u[4 * h + 3], 0x0040),
+                               0x5410);
     } else {
-        uint16_t two;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(t * 1.0000005f), "f"(t * 0.9999995f));
-        if ((two >> 8) != (two & 0xff))
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(div_to_odd(x, scale)));
-        return uint8_t(two & 0xff);
+        auto pack = [](float lo, float hi) -> uint32_t {
+            uint16_t two;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(hi), "f"(lo));
+            return two;
+        };
+        const float up = inv * 1.0000005f, down = inv * 0.9999995f;
+        uint32_t a[4], differ = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            a[e] = pack(x[2 * e] * up, x[2 * e + 1] * up);
+            differ |= a[e] ^ pack(x[2 * e] * down, x[2 * e + 1] * down);
+        }
+        if (differ) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = pack(div_to_odd(x[2 * e], scale), div_to_odd(x[2 * e + 1], scale));
+        }
+        w[0] = a[0] | a[1] << 16;
+        w[1] = a[2] | a[3] << 16;
     }
+    return make_uint2(w[0], w[1]);
 }
 
 __device__ __forceinline__ float2 e4m3x2_to_f32(uint16_t two) {
@@ -213,7 +241,8 @@ __global__ void __launch_bounds__(256, 8) kv_append_kernel(KvView kv, BatchView 
         const bool live = i < 2u * half;
         const uint32_t is_v = i >= half ? 1u : 0u;
         const uint32_t r = live ? i - is_v * half : 0u;
-        const int row = int(r / uint32_t(kv.kv_heads)), head = int(r % uint32_t(kv.kv_heads));
+        const int row = kv.head_shift >= 0 ? int(r >> kv.head_shift) : int(r / uint32_t(kv.kv_heads));
+        const int head = int(r) - row * kv.kv_heads;
         float x[8];
         load8((is_v ? v : k) + int64_t(row) * row_stride + head * kv.head_dim + lane * 8, x);
         const RowPlace at = place_row(b, start, context, row);
@@ -223,26 +252,15 @@ __global__ void __launch_bounds__(256, 8) kv_append_kernel(KvView kv, BatchView 
             if (page < 0) continue;
             store8(reinterpret_cast<T*>((is_v ? kv.v : kv.k) + slot_offset(kv, page, head, at.pos)) + lane * 8, x);
         } else {
-            float amax = 0.f;
-            bool finite = true;
+            // the largest magnitude by its bits, which an infinity or a NaN exceeds
+            uint32_t most = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                amax = fmaxf(amax, fabsf(x[e]));
-                finite = finite && fabsf(x[e]) <= 3.402823466e38f;
-            }
-            int fin = finite ? 1 : 0;
-            for (int o = lanes >> 1; o > 0; o >>= 1) {
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                fin &= __shfl_xor_sync(0xffffffffu, fin, o);
-            }
+            for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+            for (int o = lanes >> 1; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
             if (page < 0) continue;
-            const float scale = pool_scale<POOL>(amax, fin != 0);
-            const bool live_scale = scale > 0.f;  // else zeros, or a vector that reads back as NaN whatever its codes
-            const float inv = __frcp_rn(scale);
-            uint2 codes;
-            uint8_t* c = reinterpret_cast<uint8_t*>(&codes);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = live_scale ? pool_code<POOL>(x[e], scale, inv) : uint8_t(0);
+            const float scale = pool_scale<POOL>(__uint_as_float(most), most < 0x7f800000u);
+            // a scale of 0 or NaN: zeros, or a vector that reads back as NaN whatever its codes
+            const uint2 codes = scale > 0.f ? pool_codes<POOL>(x, scale, __frcp_rn(scale)) : make_uint2(0u, 0u);
             *reinterpret_cast<uint2*>((is_v ? kv.v : kv.k) + slot_offset(kv, page, head, at.pos) + lane * 8) = codes;
             if (lane == 0) (is_v ? kv.vs : kv.ks)[scale_index(kv, page, head, at.pos)] = scale;
         }
@@ -266,7 +284,8 @@ __global__ void __launch_bounds__(256, 8) kv_gather_kernel(KvView kv, BatchView 
     for (uint32_t i = blockIdx.x * per_block + threadIdx.x / lanes; i < 2u * half; i += gridDim.x * per_block) {
         const uint32_t is_v = i >= half ? 1u : 0u;
         const uint32_t r = i - is_v * half;
-        const int row = int(r / uint32_t(kv.kv_heads)), head = int(r % uint32_t(kv.kv_heads));
+        const int row = kv.head_shift >= 0 ? int(r >> kv.head_shift) : int(r / uint32_t(kv.kv_heads));
+        const int head = int(r) - row * kv.kv_heads;
         const RowPlace at = place_row(b, start, context, row);
         if (at.seq < 0) continue;
         const int page = at.pos >= 0 ? page_of(b, kv, at.seq, at.pos) : -1;

@@ -9,7 +9,9 @@
 // Each warp streams its own 16-key steps straight from global memory into the MMA fragments: the order of the head
 // dimension inside a dot product, and of the keys inside P V, is free, so a lane takes whole 16-byte pieces of its
 // key rows (K: lanes of a quad side by side; V: eight quads side by side) and no shared memory or ldmatrix is needed.
-// K of the next step is requested as soon as this step's S is issued, V as soon as its P V is.
+// 16-bit pools: K of the next step is requested as soon as this step's S is issued, V as soon as its P V is (8 KB a warp on
+// their way).  8-bit pools have half the bytes a step, too few on their way from registers alone (4.1 TB/s): each lane
+// copies its own pieces three steps ahead into a ring in shared memory with cp.async and reads back what it copied.
 //
 // 8-bit pools: codes are exact in fp16, so both products run on bare codes in fp16 and nothing is rounded but P.  The
 // key's scale multiplies the finished score; bf16 queries are brought to fp16 by a power of two per row that makes
@@ -195,6 +197,42 @@ __device__ __forceinline__ void load_words(const uint8_t* p, int step, uint32_t 
     }
 }
 
+// Asynchronous copies of `BYTES` (4, 8 or 16) a lane into shared memory, in groups.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+// W words in pieces of min(W, 4) words: piece j of a lane at dst + (32 j + lane) pieces.
+template <int W>
+__device__ __forceinline__ void copy_words(uint32_t dst, const uint8_t* p, int step) {
+    constexpr int PW = W < 4 ? W : 4;
+#pragma unroll
+    for (int j = 0; j < W / PW; ++j) copy_async<PW * 4>(dst + uint32_t(j) * 32u * PW * 4u, p + j * step);
+}
+template <int W>
+__device__ __forceinline__ void read_words(const uint32_t* src, uint32_t (&w)[W]) {
+    constexpr int PW = W < 4 ? W : 4;
+#pragma unroll
+    for (int j = 0; j < W / PW; ++j)
+        if constexpr (PW == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(src + j * 32 * PW);
+            w[4 * j] = x.x, w[4 * j + 1] = x.y, w[4 * j + 2] = x.z, w[4 * j + 3] = x.w;
+        } else if constexpr (PW == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(src);
+            w[0] = x.x, w[1] = x.y;
+        } else {
+            w[0] = *src;
+        }
+}
+
 template <typename CT, int POOL, int HD, int NT>
 struct PagedShape {
     static constexpr bool kWide = POOL == kPoolF16 || POOL == kPoolBf16;
@@ -204,9 +242,13 @@ struct PagedShape {
     static constexpr int kVw = HD / 8 * kElem / 4;  // words of a value a lane holds for P V (eight quads share it)
     static constexpr int kKPiece = (kKw < 4 ? kKw : 4) * 4;  // bytes of one load
     static constexpr int kVPiece = (kVw < 4 ? kVw : 4) * 4;
+    static constexpr int kDepth = 4;  // 8-bit: steps in the ring
+    static constexpr int kRingWords = 32 * (2 * kKw + 4 * kVw + 1);  // of one step of a warp: K, V, a scale a lane
     // CTAs an SM holds: what the registers allow without spilling (the O accumulators of 16 rows of 128 take 64)
     static constexpr int kMinBlocks = HD == 128 ? (NT == 1 ? 3 : 2) : kWide ? 3 : 4;
-    static constexpr size_t kSmem = size_t(kPaWarps) * kRows * (HD + 2) * 4;
+    static constexpr size_t kJoin = size_t(kPaWarps) * kRows * (HD + 2) * 4;
+    static constexpr size_t kRing = kWide ? 0 : size_t(kPaWarps) * kDepth * kRingWords * 4;
+    static constexpr size_t kSmem = kJoin > kRing ? kJoin : kRing;  // the ring is empty when the warps join
 };
 
 template <typename CT, int POOL, int HD, int NT>
@@ -344,11 +386,6 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
             const uint8_t* base = a.kv.k + slot_offset(a.kv, p, head, (st << 4) + g) + c * Sh::kKPiece;
             load_words<KW>(base, 4 * Sh::kKPiece, kr[0]);
             load_words<KW>(base + 8 * a.kv.token_stride, 4 * Sh::kKPiece, kr[1]);
-            if constexpr (!kWide) {
-                const float* s = a.kv.ks + scale_index(a.kv, p, head, (st << 4) + g);
-                ksc[0] = __ldg(s);
-                ksc[1] = __ldg(s + 8);
-            }
         };
         auto load_v = [&](int st, int p) {
             if (p < 0) p = 0;
@@ -357,20 +394,74 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
             load_words<VW>(base + a.kv.token_stride, 8 * Sh::kVPiece, vr[1]);
             load_words<VW>(base + 8 * a.kv.token_stride, 8 * Sh::kVPiece, vr[2]);
             load_words<VW>(base + 9 * a.kv.token_stride, 8 * Sh::kVPiece, vr[3]);
-            if constexpr (!kWide) {
-                const float* s = a.kv.vs + scale_index(a.kv, p, head, (st << 4) + g);
-                vsc[0] = __ldg(s);
-                vsc[1] = __ldg(s + 8);
-            }
+        };
+        // 8-bit: one step into slot `slot` of the warp's ring; lane l < 16 takes the key scale of row l, the others the
+        // value scale of row l - 16.
+        uint32_t* ring = reinterpret_cast<uint32_t*>(pa_sm) + warp * Sh::kDepth * Sh::kRingWords;
+        constexpr int kKRow = 32 * KW, kVRow = 32 * VW, kVAt = 2 * kKRow, kScaleAt = kVAt + 4 * kVRow;
+        constexpr int KP = Sh::kKPiece / 4, VP = Sh::kVPiece / 4;  // words of a piece
+        auto copy_step = [&](int st, int p, int slot) {
+            if (p < 0) p = 0;
+            const uint32_t dst = smem_u32(ring + slot * Sh::kRingWords);
+            const uint8_t* kb = a.kv.k + slot_offset(a.kv, p, head, (st << 4) + g) + c * Sh::kKPiece;
+            copy_words<KW>(dst + lane * KP * 4, kb, 4 * Sh::kKPiece);
+            copy_words<KW>(dst + (kKRow + lane * KP) * 4, kb + 8 * a.kv.token_stride, 4 * Sh::kKPiece);
+            const uint8_t* vb = a.kv.v + slot_offset(a.kv, p, head, (st << 4) + 2 * c) + g * Sh::kVPiece;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                copy_words<VW>(dst + (kVAt + r * kVRow + lane * VP) * 4, vb + ((r & 1) + (r >> 1) * 8) * a.kv.token_stride,
+                               8 * Sh::kVPiece);
+            const float* sc = (lane < 16 ? a.kv.ks : a.kv.vs) + scale_index(a.kv, p, head, (st << 4) + (lane & 15));
+            copy_async<4>(dst + (kScaleAt + lane) * 4, sc);
         };
         int page = -1, next_page = 0;
-        if (step < step_end) {
-            page = checked(fetch_page(step));
-            load_k(step, page);
-            load_v(step, page);
-            next_page = fetch_page(step + kPaWarps);
+        uint32_t bad = 0;  // 8-bit: bit d, the step d steps from here is on a bad page
+        int ahead = step;  // 8-bit: the next step to copy
+        int slot = 0;
+        if constexpr (kWide) {
+            if (step < step_end) {
+                page = checked(fetch_page(step));
+                load_k(step, page);
+                load_v(step, page);
+                next_page = fetch_page(step + kPaWarps);
+            }
+        } else {
+            int first_pages[Sh::kDepth];
+#pragma unroll
+            for (int d = 0; d < Sh::kDepth; ++d) first_pages[d] = fetch_page(step + d * kPaWarps);
+#pragma unroll
+            for (int d = 0; d < Sh::kDepth - 1; ++d) {
+                if (ahead < step_end) {
+                    const int p = checked(first_pages[d]);
+                    bad |= (p < 0 ? 1u : 0u) << d;
+                    copy_step(ahead, p, d);
+                }
+                copy_commit();
+                ahead += kPaWarps;
+            }
+            next_page = first_pages[Sh::kDepth - 1];
         }
         for (; step < step_end; step += kPaWarps) {
+            if constexpr (!kWide) {
+                // the slot that the step before this one left, for the last of the steps ahead
+                if (ahead < step_end) {
+                    const int p = checked(next_page);
+                    bad |= (p < 0 ? 1u : 0u) << (Sh::kDepth - 1);
+                    copy_step(ahead, p, slot == 0 ? Sh::kDepth - 1 : slot - 1);
+                    next_page = fetch_page(ahead + kPaWarps);
+                }
+                copy_commit();
+                ahead += kPaWarps;
+                copy_wait<Sh::kDepth - 1>();
+                __syncwarp();  // the scales are other lanes' copies
+                const uint32_t* src = ring + slot * Sh::kRingWords;
+                read_words<KW>(src + lane * KP, kr[0]);
+                read_words<KW>(src + kKRow + lane * KP, kr[1]);
+                const float* sc = reinterpret_cast<const float*>(src + kScaleAt);
+                ksc[0] = sc[g], ksc[1] = sc[g + 8], vsc[0] = sc[16 + g], vsc[1] = sc[24 + g];
+                page = bad & 1u ? -1 : 0;
+                bad >>= 1;
+            }
             const int pos = step << 4;
             const int after = step + kPaWarps;
             const bool more = after < step_end;
@@ -395,7 +486,12 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
             }
             const float ks0 = kWide ? 1.f : ksc[0], ks1 = kWide ? 1.f : ksc[1];
             const int this_page = page;
-            if (more) {
+            if constexpr (!kWide) {
+                const uint32_t* src = ring + slot * Sh::kRingWords + kVAt + lane * VP;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) read_words<VW>(src + r * kVRow, vr[r]);
+                slot = slot + 1 == Sh::kDepth ? 0 : slot + 1;
+            } else if (more) {
                 page = checked(next_page);
                 load_k(after, page);
                 next_page = fetch_page(after + kPaWarps);
@@ -495,8 +591,11 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
                     }
                 }
             }
-            if (more) load_v(after, page);
+            if constexpr (kWide) {
+                if (more) load_v(after, page);
+            }
         }
+        if constexpr (!kWide) copy_wait<0>();
 
         // ---- join the warps through shared memory
         __syncthreads();  // the previous segment's join has been read
@@ -519,7 +618,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
             }
         __syncthreads();
         const bool complete = k0 == 0 && k1 == u.tiles;
-        const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+        const int part = 2 * blockIdx.x + (first_segment ? 0 : 1);
         for (int i = threadIdx.x; i < ROWS * (HD / 8); i += blockDim.x) {
             const int r = i / (HD / 8), d = i % (HD / 8) * 8;
             float mm = -INFINITY;
@@ -546,10 +645,11 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
                            int64_t(head * a.group + row % a.group) * HD + d,
                        x);
             } else {
-                store8(a.part_o + (int64_t(slot) * ROWS + r) * HD + d, x);
-                if (d == 0) a.part_ml[int64_t(slot) * ROWS + r] = make_float2(mm, ll);
+                store8(a.part_o + (int64_t(part) * ROWS + r) * HD + d, x);
+                if (d == 0) a.part_ml[int64_t(part) * ROWS + r] = make_float2(mm, ll);
             }
         }
+        if constexpr (!kWide) __syncthreads();  // the ring of the next segment takes the same memory
         first_segment = false;
     }
 }

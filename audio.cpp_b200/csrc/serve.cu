@@ -59,6 +59,9 @@ KvView cache_view(const b2d_kv_cache* c) {
     v.token_stride = c->token_stride * elem;
     v.pages = c->pages;
     v.page_shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+    v.head_shift = -1;
+    for (int b = 0; b < 16; ++b)
+        if (c->kv_heads == 1 << b) v.head_shift = b;
     v.kv_heads = c->kv_heads;
     v.head_dim = c->head_dim;
     return v;
