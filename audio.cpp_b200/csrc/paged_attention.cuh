@@ -466,11 +466,11 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
             const int after = step + kPaWarps;
             const bool more = after < step_end;
             // ---- S^T = K Q^T
-            float s[NT][4];
+            float s[NT][4], s2[NT][4];  // two chains of products, joined below
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+                for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks) {
                 uint32_t a0, a1, a2, a3;
@@ -482,8 +482,12 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                    mma_16816(s[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], MT16{});
+                    mma_16816(ks & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], MT16{});
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
             const float ks0 = kWide ? 1.f : ksc[0], ks1 = kWide ? 1.f : ksc[1];
             const int this_page = page;
             if constexpr (!kWide) {
