@@ -5,12 +5,12 @@
 // those with w >= min_p; each cut is a prefix of that order.  The token is the first index (in index order) whose
 // running sum over kept entries passes u Z.
 //
-// A row is read from HBM once: a cluster of up to 8 CTAs holds it in shared memory (in its own type), and every later
-// pass reads it there.  A cut is found by counting entries in 2048 bins (linear in the logit, later linear in the ordered
+// A row is read from HBM once: a cluster of up to 8 CTAs holds it in shared memory as ordered bits, four to a load, and
+// every later pass compares integers there.  A cut is found by counting entries in 2048 bins (linear in the logit, later linear in the ordered
 // bits).  For a cut by mass, a bin's mass lies between its count times the weights at its two edges, which brackets the
 // crossing to a few bins; the masses above the bracket and of its upper half are then summed exactly, which decides
-// for a half, and that is counted again until it holds few enough entries to rank them one against the other.  The
-// undecided range of ordered bits at least halves every round, so there are at most 33.  (Summing masses into the bins
+// for a half, and that is counted again until it holds few enough entries to sort them.  The
+// undecided range of ordered bits at least halves every round, so there are at most 34.  (Summing masses into the bins
 // took three more shared atomics an entry.)
 // Which token comes out depends on sums of up to 2^18 terms and on comparisons next to a border, so the weights are
 // computed in fp64 and added as integers (units of 2^-45 of the largest weight): sums of integers do not depend on
@@ -30,7 +30,7 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 2048;
-constexpr int kSampleList = 512;          // entries ranked one against the other
+constexpr int kSampleList = 512;          // entries sorted at once
 constexpr int kSampleMaxSlice = 32768;    // entries a CTA holds
 constexpr int kSampleMaxCluster = 8;
 constexpr double kSampleUnit = 35184372088832.0;  // 2^45
@@ -48,10 +48,30 @@ struct SampleArgs {
     float* probs;
 };
 
-// fp32 bits in an order that compares like the numbers (-inf lowest; zeros of both signs arrive as +0).
+// fp32 bits in an order that compares like the numbers; 0 for an entry that cannot be drawn (-inf, NaN, none at all).
 __device__ __forceinline__ uint32_t ordered_bits(float x) {
-    const uint32_t u = __float_as_uint(x);
+    if (!(x > -INFINITY)) return 0;
+    const uint32_t u = __float_as_uint(x + 0.f);  // zeros of both signs are one value
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(uint32_t k) {
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// A CTA's share of a row as ordered bits, with 16-byte loads where the row allows them.
+template <typename T>
+__device__ __forceinline__ void load_keys(const T* src, int have, int slice, uint32_t* keys) {
+    constexpr int kVec = 16 / sizeof(T);
+    const int skip = min(have, int((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / int(sizeof(T)));
+    const int vectors = (have - skip) / kVec, rest = skip + vectors * kVec;
+    for (int i = threadIdx.x; i < vectors; i += kSampleThreads) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src + skip) + i);
+        const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) keys[skip + i * kVec + e] = ordered_bits(to_f32(t[e]));
+    }
+    for (int i = threadIdx.x; i < skip; i += kSampleThreads) keys[i] = ordered_bits(to_f32(src[i]));
+    for (int i = rest + threadIdx.x; i < slice; i += kSampleThreads) keys[i] = i < have ? ordered_bits(to_f32(src[i])) : 0u;
 }
 
 struct SampleShared {
@@ -72,7 +92,7 @@ struct SampleShared {
     uint32_t list_fill;
     // published by rank 0
     int bin_lo, bin_hi;    // the bracket
-    uint32_t before_count;
+    uint32_t before_count, bracket;  // entries above it, in it
     uint64_t cut;          // last kept (ordered bits, ~index)
 };
 
@@ -112,42 +132,39 @@ template <typename T>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t sample_raw[];
     SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_raw);
-    T* xs = reinterpret_cast<T*>(sample_raw + ((sizeof(SampleShared) + 15) & ~size_t(15)));
+    uint32_t* keys = reinterpret_cast<uint32_t*>(sample_raw + ((sizeof(SampleShared) + 15) & ~size_t(15)));
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), ranks = int(cluster.num_blocks());
     const int row = int(blockIdx.x) / ranks;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int base = rank * a.slice, have = max(0, min(a.slice, a.vocab - base));
-    const int per_warp = a.slice / kSampleWarps;  // a multiple of 32; a warp owns consecutive entries
-    const int w0 = warp * per_warp, w1 = min(w0 + per_warp, have);
-
-    // An entry: a NaN counts as -inf, zeros of both signs are one value.
-    auto entry_value = [](T raw) -> float {
-        const float v = to_f32(raw);
-        return v != v ? -INFINITY : v + 0.f;
+    const int per_warp = a.slice / kSampleWarps;  // a multiple of 128; a warp owns consecutive entries, a lane four at a time
+    const int w0 = warp * per_warp, w1 = min(w0 + per_warp, (have + 127) & ~127);
+    auto each = [&](auto&& f) {  // this lane's entries: f(index in the slice, ordered bits)
+        for (int i = w0 + lane * 4; i < w1; i += 128) {
+            const uint4 k4 = *reinterpret_cast<const uint4*>(keys + i);
+            f(i, k4.x), f(i + 1, k4.y), f(i + 2, k4.z), f(i + 3, k4.w);
+        }
     };
-    auto x = [&](int i) { return entry_value(xs[i]); };
+    auto entry_of = [&](int i, uint32_t key) { return uint64_t(key) << 32 | uint32_t(~uint32_t(base + i)); };
 
-    // ---- the row into shared memory; its best entry and its lowest finite one
+    // ---- the row into shared memory; its best entry and its lowest one
     if (tid < 64) sh.power[tid] = exp2(double(tid) / 64.0);
-    const T* src = static_cast<const T*>(a.logits) + int64_t(row) * a.row_stride + base;
-    uint64_t best = 0;
-    uint32_t low = 0xffffffffu;
-    for (int i = tid; i < have; i += kSampleThreads) {
-        const T raw = src[i];
-        xs[i] = raw;
-        const float v = entry_value(raw);
-        const uint32_t key = ordered_bits(v);
-        const uint64_t entry = uint64_t(key) << 32 | uint32_t(~uint32_t(base + i));
-        best = best > entry ? best : entry;
-        if (v > -INFINITY) low = min(low, key);
-    }
+    load_keys(static_cast<const T*>(a.logits) + int64_t(row) * a.row_stride + base, have, a.slice, keys);
+    __syncthreads();
+    uint32_t top = 0, low = 0xffffffffu;
+    int top_at = 0;
+    each([&](int i, uint32_t key) {
+        if (key > top) top = key, top_at = i;  // ascending indexes: the first of equals
+        if (key) low = min(low, key);
+    });
+    uint64_t best = top ? entry_of(top_at, top) : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const uint64_t y = __shfl_xor_sync(0xffffffffu, best, o);
         best = best > y ? best : y;
-        low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
     }
+    low = __reduce_min_sync(0xffffffffu, low);
     if (lane == 0) sh.warp_u64[warp] = best, sh.warp_u32[warp] = low;
     __syncthreads();
     if (tid == 0) {
@@ -166,40 +183,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         low = r == 0 ? p->low : min(low, p->low);
     }
     const uint32_t best_key = uint32_t(best >> 32);
-    const int best_index = int(~uint32_t(best));
-    auto from_ordered = [](uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); };
-    const float m = from_ordered(best_key);
     const float temp = a.temperature[row];
-    const bool empty = !(m > -INFINITY);
-    if (empty || !(temp > 0.f)) {
+    if (best_key == 0 || !(temp > 0.f)) {
         if (rank == 0 && tid == 0) {
-            a.tokens[row] = empty ? -1 : best_index;
-            if (a.probs) a.probs[row] = empty ? 0.f : 1.f;
+            a.tokens[row] = best_key == 0 ? -1 : int(~uint32_t(best));
+            if (a.probs) a.probs[row] = best_key == 0 ? 0.f : 1.f;
         }
         cluster.sync();  // peers may still be reading this CTA's shared memory
         return;
     }
+    const float m = from_ordered(best_key);
     const double inv_t = 1.0 / double(temp);
-    auto weight = [&](float v) -> uint64_t {
-        if (v == m) return uint64_t(kSampleUnit);
-        const double t = (double(v) - double(m)) * inv_t;
-        if (!(t > -31.9) || v == -INFINITY) return 0;  // under half a unit
+    auto weight = [&](uint32_t key) -> uint64_t {
+        if (key == best_key) return uint64_t(kSampleUnit);
+        const double t = (double(from_ordered(key)) - double(m)) * inv_t;
+        if (!(t > -31.9)) return 0;  // under half a unit
         return exp_units(t, sh.power);
     };
 
     uint64_t cut = 0;  // entries at or above it (as (ordered bits, ~index)) are kept
-    auto entry_of = [&](int i) { return uint64_t(ordered_bits(x(i))) << 32 | uint32_t(~uint32_t(base + i)); };
-
-    // Sum over the cluster of the kept entries' weights (at least `least` units each).  Every thread gets the total
-    // and the sum of the ranks before; warp_u64 keeps the warps' running sums.
-    auto kept_mass = [&](uint64_t least, uint64_t& before) -> uint64_t {
-        uint64_t sum = 0;
-        for (int i = w0 + lane; i < w1; i += 32)
-            if (entry_of(i) >= cut) {
-                const uint64_t w = weight(x(i));
-                sum += w >= least ? w : 0;
-            }
-        sum = warp_add_u64(sum);
+    // Is entry i kept so far?  (Absent entries, of bits 0, never are.)
+    auto kept = [&](int i, uint32_t key) {
+        const uint32_t ck = uint32_t(cut >> 32);
+        return key > ck || (key == ck && key != 0 && uint32_t(~uint32_t(base + i)) >= uint32_t(cut));
+    };
+    // This thread's warp's mass into running sums of the CTA (warp_u64[w] = before warp w), its total into sh.total.
+    auto running_sums = [&](uint64_t sum) {
         __syncthreads();
         if (lane == 0) sh.warp_u64[warp + 1] = sum;
         __syncthreads();
@@ -209,7 +218,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             for (int i = 1; i <= kSampleWarps; ++i) sh.warp_u64[i] = run += sh.warp_u64[i];
             sh.total = run;
         }
-        cluster.sync();
+    };
+    auto over_ranks = [&](uint64_t& before) -> uint64_t {  // after a cluster.sync: sum of the totals, and of those before
         uint64_t all = 0;
         before = 0;
         for (int r = 0; r < ranks; ++r) {
@@ -219,36 +229,50 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         }
         return all;
     };
+    bool summed = false;  // warp_u64 and total already hold the kept mass
 
     // Lowers `cut` to the last entry of the prefix that holds `want` entries (by_mass false), or of which the mass
-    // before it is below `target` units (by_mass true).
-    auto find_cut = [&](bool by_mass, uint32_t want, uint64_t target) {
-        const float span = fminf(32.f * temp, m - from_ordered(low));
+    // before it is below `part` of the mass kept so far (by_mass true).
+    auto find_cut = [&](bool by_mass, uint32_t want, float part, bool sum_up) {
+        const float span = fminf(16.f * temp, m - from_ordered(low));  // the last bin takes what lies deeper
         const float per_unit = span > 0.f ? float(kSampleBins) / span : 0.f;
-        uint32_t key_lo = 0, key_hi = 0xffffffffu;  // what is still undecided
+        uint32_t key_lo = 1, key_hi = 0xffffffffu;  // what is still undecided
         uint32_t before_count = 0;                  // kept for certain: everything above key_hi
-        uint64_t before_mass = 0;
+        uint64_t before_mass = 0, target = 0;
         SampleShared* lead = cluster.map_shared_rank(&sh, 0);
         for (int round = 0; round < 40; ++round) {
             int shift = 0;
             while (((key_hi - key_lo) >> shift) >= uint32_t(kSampleBins)) ++shift;
-            auto bin_of = [&](float v, uint32_t key) -> int {
-                if (round == 0) return min(kSampleBins - 1, max(0, int((m - v) * per_unit)));
+            auto bin_of = [&](uint32_t key) -> int {
+                if (round == 0) return min(kSampleBins - 1, max(0, int((m - from_ordered(key)) * per_unit)));
                 return int((key_hi - key) >> shift);
             };
-            auto active = [&](int i, float v, uint32_t& key) {
-                key = ordered_bits(v);
-                return key >= key_lo && key <= key_hi && (uint64_t(key) << 32 | uint32_t(~uint32_t(base + i))) >= cut;
-            };
+            auto active = [&](int i, uint32_t key) { return key >= key_lo && key <= key_hi && kept(i, key); };
             for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.count[i] = 0;
             if (tid < 2) sh.list_fill = 0, sh.key_lo[tid] = 0xffffffffu, sh.key_hi[tid] = 0, sh.inside[tid] = 0;
             __syncthreads();
-            for (int i = tid; i < have; i += kSampleThreads) {
-                const float v = x(i);
-                uint32_t key;
-                if (active(i, v, key)) atomicAdd(&sh.count[bin_of(v, key)], 1u);
+            uint64_t all = 0;
+            each([&](int i, uint32_t key) {
+                if (!active(i, key)) return;
+                atomicAdd(&sh.count[bin_of(key)], 1u);
+                if (by_mass && round == 0) all += weight(key);
+            });
+            if (by_mass && round == 0) {
+                all = warp_add_u64(all);
+                if (lane == 0) sh.warp_u64[warp] = all;
+                __syncthreads();
+                if (tid == 0) {
+                    for (int i = 1; i < kSampleWarps; ++i) all += sh.warp_u64[i];
+                    sh.total = all;
+                }
             }
             cluster.sync();
+            if (by_mass && round == 0) {
+                uint64_t none;
+                const uint64_t z = over_ranks(none);
+                target = part > 0.f ? uint64_t(ceil(double(part) * double(z))) : 1u;
+                if (target == 0) target = 1;
+            }
             if (rank == 0) {
                 // every thread sums four consecutive bins over the ranks, then the bins are scanned in order
                 static_assert(kSampleBins == 4 * kSampleThreads, "four bins a thread");
@@ -261,22 +285,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 double least[4], most[4];
                 uint32_t own_c = 0;
                 double own_l = 0, own_m = 0;
+                // weights at the edges b / per_unit below m (round 0), give or take their rounding
+                const double step = round == 0 && per_unit > 0.f ? inv_t / double(per_unit) : 0.0;
+                const double ratio = by_mass && round == 0 ? exp(-step) : 0.0;
+                double edge = by_mass && round == 0 ? kSampleUnit * exp(-step * (tid * 4)) : 0.0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int b = tid * 4 + e;
                     least[e] = most[e] = 0;
                     if (by_mass && cnt[e] > 0) {
-                        if (round == 0) {  // edges b / per_unit below m, give or take their rounding
-                            const double step = per_unit > 0.f ? inv_t / double(per_unit) : 0.0;
-                            most[e] = cnt[e] * kSampleUnit * exp(-step * b) * 1.001;
-                            least[e] = b == kSampleBins - 1 ? 0.0 : cnt[e] * kSampleUnit * exp(-step * (b + 1)) * 0.999;
+                        if (round == 0) {
+                            most[e] = cnt[e] * edge * 1.001;
+                            least[e] = b == kSampleBins - 1 ? 0.0 : cnt[e] * edge * ratio * 0.999;
                         } else {
-                            const uint32_t top = key_hi - (uint32_t(b) << shift);
-                            const uint32_t end = (1u << shift) - 1u, bottom = top - key_lo < end ? key_lo : top - end;
-                            most[e] = double(cnt[e]) * double(weight(from_ordered(top)));
-                            least[e] = double(cnt[e]) * double(weight(from_ordered(bottom)));
+                            const uint32_t top_key = key_hi - (uint32_t(b) << shift), end = (1u << shift) - 1u;
+                            const uint32_t bottom = top_key - key_lo < end ? key_lo : top_key - end;
+                            most[e] = double(cnt[e]) * double(weight(top_key));
+                            least[e] = double(cnt[e]) * double(weight(bottom));
                         }
                     }
+                    edge *= ratio;
                     own_c += cnt[e];
                     own_l += least[e];
                     own_m += most[e];
@@ -324,32 +352,110 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 if (tid == 0) sh.bin_lo = by_mass ? min(sh.bin_lo, sh.bin_hi) : sh.bin_hi;
                 __syncthreads();
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int e = 0; e < 4; ++e) {
                     if (tid * 4 + e == sh.bin_lo) sh.before_count = at[e];
-            }
-            cluster.sync();
-            const int bin_lo = lead->bin_lo, bin_hi = lead->bin_hi, middle = (bin_lo + bin_hi) >> 1;
-            before_count = lead->before_count;
-            // ---- exactly: the masses above the bracket and of its upper half, its entries by halves and their ranges
-            uint64_t above = 0, upper = 0;
-            uint32_t inside[2] = {0, 0}, lo_key[2] = {0xffffffffu, 0xffffffffu}, hi_key[2] = {0, 0};
-            for (int i = tid; i < have; i += kSampleThreads) {
-                const float v = x(i);
-                uint32_t key;
-                if (!active(i, v, key)) continue;
-                const int b = bin_of(v, key);
-                if (b > bin_hi) continue;
-                if (b >= bin_lo) {
-                    const bool second = b > middle;
-                    inside[0] += second ? 0u : 1u;
-                    inside[1] += second ? 1u : 0u;
-                    if (second) lo_key[1] = min(lo_key[1], key), hi_key[1] = max(hi_key[1], key);
-                    else lo_key[0] = min(lo_key[0], key), hi_key[0] = max(hi_key[0], key);
-                    if (by_mass && !second && bin_hi > bin_lo) upper += weight(v);
-                } else if (by_mass) {
-                    above += weight(v);
+                    if (tid * 4 + e == sh.bin_hi) sh.bracket = at[e] + cnt[e];
                 }
             }
+            cluster.sync();
+            const int bin_lo = lead->bin_lo, bin_hi = lead->bin_hi;
+            before_count = lead->before_count;
+            const uint32_t bracket = lead->bracket - before_count;
+            if (bracket <= uint32_t(kSampleList)) {
+                // ---- the mass above the bracket, exactly, and the bracket's entries into rank 0's list (in any order)
+                uint64_t above = 0;
+                each([&](int i, uint32_t key) {
+                    if (!active(i, key)) return;
+                    const int b = bin_of(key);
+                    if (b > bin_hi) return;
+                    if (b >= bin_lo) {
+                        const uint32_t at = atomicAdd(&lead->list_fill, 1u);
+                        lead->list_entry[at] = entry_of(i, key);
+                        lead->list_weight[at] = by_mass ? weight(key) : 0;
+                    } else if (by_mass) {
+                        above += weight(key);
+                    }
+                });
+                above = by_mass ? warp_add_u64(above) : 0;
+                running_sums(above);
+                cluster.sync();
+                uint64_t none;
+                before_mass += over_ranks(none);
+                if (rank == 0) {
+                    // the list in order (bitonic, an entry a thread; pairs within a warp by shuffles), then its running
+                    // sums: the last entry whose rank / mass before it still qualifies is the cut
+                    static_assert(kSampleList == kSampleThreads, "one entry a thread");
+                    const bool there = uint32_t(tid) < bracket;
+                    uint64_t e = there ? sh.list_entry[tid] : 0, w = there ? sh.list_weight[tid] : 0;
+                    for (int size = 2; size <= kSampleList; size *= 2) {
+                        for (int step = size / 2; step > 0; step /= 2) {
+                            uint64_t oe, ow;
+                            if (step >= 32) {
+                                __syncthreads();
+                                sh.list_entry[tid] = e, sh.list_weight[tid] = w;
+                                __syncthreads();
+                                oe = sh.list_entry[tid ^ step], ow = sh.list_weight[tid ^ step];
+                            } else {
+                                oe = __shfl_xor_sync(0xffffffffu, e, step), ow = __shfl_xor_sync(0xffffffffu, w, step);
+                            }
+                            // descending overall: the lower of a pair of threads keeps the larger in even runs
+                            const bool larger = ((tid & step) == 0) == ((tid & size) == 0);
+                            if ((oe > e) == larger && oe != e) e = oe, w = ow;
+                        }
+                    }
+                    const uint64_t upto = warp_scan_u64(w, lane);
+                    __syncthreads();
+                    if (lane == 31) sh.list_weight[warp] = upto;
+                    if (tid == 0) sh.cut = ~uint64_t(0);
+                    __syncthreads();
+                    uint64_t ms = before_mass + upto - w;
+                    for (int i = 0; i < warp; ++i) ms += sh.list_weight[i];
+                    __syncthreads();
+                    sh.list_entry[tid] = e, sh.list_weight[tid] = w;  // the other ranks read them
+                    const bool keep = there && (by_mass ? ms < target : before_count + uint32_t(tid) < want);
+                    if (keep) atomicMin(reinterpret_cast<unsigned long long*>(&sh.cut), (unsigned long long)e);
+                }
+                cluster.sync();
+                cut = lead->cut;
+                if (by_mass && sum_up && round == 0) {
+                    // what is kept: the entries above the bracket, summed just now, and the list's down to the cut
+                    if (uint32_t(tid) < bracket) {
+                        const uint64_t e = lead->list_entry[tid];
+                        const int i = int(~uint32_t(e)) - base;
+                        if (e >= cut && i >= 0 && i < a.slice) {
+                            const unsigned long long w = lead->list_weight[tid];
+                            for (int o = i / per_warp + 1; o <= kSampleWarps; ++o)
+                                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.warp_u64[o]), w);
+                        }
+                    }
+                    __syncthreads();
+                    if (tid == 0) sh.total = sh.warp_u64[kSampleWarps];
+                    summed = true;
+                }
+                return;
+            }
+            // ---- too many for the list.  Exactly: the masses above the bracket and of its upper half, its entries by
+            // halves and their ranges
+            const int middle = (bin_lo + bin_hi) >> 1;
+            uint64_t above = 0, upper = 0;
+            uint32_t inside[2] = {0, 0}, lo_key[2] = {0xffffffffu, 0xffffffffu}, hi_key[2] = {0, 0};
+            each([&](int i, uint32_t key) {
+                if (!active(i, key)) return;
+                const int b = bin_of(key);
+                if (b > bin_hi) return;
+                if (b >= bin_lo) {
+                    if (b > middle) {
+                        ++inside[1];
+                        lo_key[1] = min(lo_key[1], key), hi_key[1] = max(hi_key[1], key);
+                    } else {
+                        ++inside[0];
+                        lo_key[0] = min(lo_key[0], key), hi_key[0] = max(hi_key[0], key);
+                        if (by_mass && bin_hi > bin_lo) upper += weight(key);
+                    }
+                } else if (by_mass) {
+                    above += weight(key);
+                }
+            });
             if (by_mass) above = warp_add_u64(above), upper = warp_add_u64(upper);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -378,66 +484,30 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             }
             // the last kept entry is in the lower half if something behind the upper one is kept
             const int half = by_mass && bin_hi > bin_lo && before_mass + upper_all < target ? 1 : 0;
-            uint32_t offset = 0, inside_all = 0, low_key = 0xffffffffu, high_key = 0;
+            uint32_t inside_all = 0;
+            key_lo = 0xffffffffu;
+            key_hi = 0;
             for (int r = 0; r < ranks; ++r) {
                 const SampleShared* p = cluster.map_shared_rank(&sh, r);
-                if (r < rank) offset += p->inside[half];
                 inside_all += p->inside[half];
-                low_key = min(low_key, p->key_lo[half]);
-                high_key = max(high_key, p->key_hi[half]);
+                key_lo = min(key_lo, p->key_lo[half]);
+                key_hi = max(key_hi, p->key_hi[half]);
                 if (half) before_count += p->inside[0];
             }
             if (half) before_mass += upper_all;
-            if (inside_all <= uint32_t(kSampleList)) {
-                for (int i = tid; i < have; i += kSampleThreads) {
-                    const float v = x(i);
-                    uint32_t key;
-                    if (!active(i, v, key) || key < low_key || key > high_key) continue;
-                    const uint32_t at = offset + atomicAdd(&sh.list_fill, 1u);
-                    lead->list_entry[at] = uint64_t(key) << 32 | uint32_t(~uint32_t(base + i));
-                    lead->list_weight[at] = by_mass ? weight(v) : 0;
-                }
-                cluster.sync();
-                if (rank == 0) {
-                    // the list's last kept entry: the lowest one whose rank / mass before it still qualifies
-                    uint64_t kept = ~uint64_t(0);
-                    if (uint32_t(tid) < inside_all) {
-                        const uint64_t e = sh.list_entry[tid];
-                        uint32_t c = before_count;
-                        uint64_t ms = before_mass;
-                        for (uint32_t j = 0; j < inside_all; ++j)
-                            if (sh.list_entry[j] > e) ++c, ms += sh.list_weight[j];
-                        if (by_mass ? ms < target : c < want) kept = e;
-                    }
-                    static_assert(kSampleList <= kSampleThreads, "one entry a thread");
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) {
-                        const uint64_t y = __shfl_xor_sync(0xffffffffu, kept, o);
-                        kept = y < kept ? y : kept;
-                    }
-                    if (lane == 0) sh.warp_u64[warp] = kept;
-                    __syncthreads();
-                    if (tid == 0) {
-                        for (int i = 1; i < kSampleWarps; ++i) kept = sh.warp_u64[i] < kept ? sh.warp_u64[i] : kept;
-                        // none in the bracket: everything above it
-                        sh.cut = kept != ~uint64_t(0) ? kept : (uint64_t(high_key) + 1) << 32;
-                    }
-                }
-                cluster.sync();
-                cut = lead->cut;
-                return;
-            }
             cluster.sync();  // read by every rank before it is written again
-            key_lo = low_key;
-            key_hi = high_key;
             if (key_lo != key_hi) continue;
             // one value fills the bracket: its first entries by index are kept
             uint32_t need = want - before_count;
             if (by_mass) {
-                const uint64_t w = weight(from_ordered(key_lo));
+                const uint64_t w = weight(key_lo);
                 const uint64_t left = target > before_mass ? target - before_mass : 0;
                 const uint64_t n = w ? (left + w - 1) / w : (left ? inside_all : 0);
                 need = uint32_t(n < inside_all ? n : inside_all);
+            }
+            if (need >= inside_all) {  // all of them
+                cut = max(cut, uint64_t(key_lo) << 32);
+                return;
             }
             if (need == 0) {
                 cut = (uint64_t(key_hi) + 1) << 32;
@@ -445,10 +515,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             }
             // ties in the ranks, then the warps, before this one
             uint32_t mine = 0;
-            for (int i = w0 + lane; i < w1; i += 32) {
-                uint32_t key;
-                mine += active(i, x(i), key) ? 1u : 0u;
-            }
+            each([&](int i, uint32_t key) { mine += active(i, key) ? 1u : 0u; });
             mine = __reduce_add_sync(0xffffffffu, mine);
             __syncthreads();
             if (lane == 0) sh.warp_u32[warp] = mine;
@@ -465,11 +532,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             if (run < need && need <= run + mine) {
                 for (int i0 = w0; i0 < w1; i0 += 32) {
                     const int i = i0 + lane;
-                    uint32_t key = 0;
-                    const bool hit = i < w1 && active(i, x(i), key);
+                    const bool hit = active(i, keys[i]);
                     const uint32_t vote = __ballot_sync(0xffffffffu, hit);
                     const uint32_t nth = run + __popc(vote & ((2u << lane) - 1u));
-                    if (hit && nth == need) lead->cut = entry_of(i);
+                    if (hit && nth == need) lead->cut = entry_of(i, keys[i]);
                     run += __popc(vote);
                 }
             }
@@ -480,41 +546,61 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     };
 
     const int k = a.top_k ? a.top_k[row] : 0;
-    if (k > 0 && k < a.vocab) find_cut(false, uint32_t(k), 0);
-    const float p = a.top_p ? a.top_p[row] : 1.f;
-    uint64_t before = 0;
-    if (p < 1.f) {
-        cluster.sync();  // the last cut has been read by every rank
-        const uint64_t z = kept_mass(0, before);
-        const uint64_t target = p > 0.f ? uint64_t(ceil(double(p) * double(z))) : 1u;
-        cluster.sync();
-        find_cut(true, 0, target > 0 ? target : 1u);
+    const float p = a.top_p ? a.top_p[row] : 1.f, floor_p = a.min_p ? a.min_p[row] : 0.f;
+    if (k > 0 && k < a.vocab) {
+        find_cut(false, uint32_t(k), 0.f, false);
+        cluster.sync();  // the cut has been read by every rank
     }
-    const float floor_p = a.min_p ? a.min_p[row] : 0.f;
+    if (p < 1.f) find_cut(true, 0, p, !(floor_p > 0.f));
     const uint64_t least = floor_p > 0.f ? uint64_t(ceil(double(fminf(floor_p, 1.f)) * kSampleUnit)) : 0;
+    if (!summed) {
+        uint64_t sum = 0;
+        each([&](int i, uint32_t key) {
+            if (!kept(i, key)) return;
+            const uint64_t w = weight(key);
+            sum += w >= least ? w : 0;
+        });
+        sum = warp_add_u64(sum);
+        cluster.sync();  // the totals of the last cut have been read by every rank
+        running_sums(sum);
+    }
     cluster.sync();
-    const uint64_t z = kept_mass(least, before);
+    uint64_t before;
+    const uint64_t z = over_ranks(before);
     float u = a.uniform[row];
     u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
     uint64_t goal = uint64_t(double(u) * double(z));  // the token is the first whose running sum is above it
     if (goal >= z) goal = z - 1;
     if (goal >= before && goal < before + sh.total) {
-        const uint64_t warp_before = before + sh.warp_u64[warp], warp_after = before + sh.warp_u64[warp + 1];
-        if (goal >= warp_before && goal < warp_after) {
-            uint64_t run = warp_before;
-            for (int i0 = w0; i0 < w1; i0 += 32) {
-                const int i = i0 + lane;
-                uint64_t w = 0;
-                if (i < w1 && entry_of(i) >= cut) {
-                    w = weight(x(i));
-                    if (w < least) w = 0;
-                }
-                const uint64_t upto = run + warp_scan_u64(w, lane);
-                if (w > 0 && goal < upto && goal >= upto - w) {
-                    a.tokens[row] = base + i;
+        // this CTA's: first the warp whose share holds the goal, then that share is cut among all warps, then one of them
+        // looks at its few entries one by one
+        auto mass = [&](int i) -> uint64_t {
+            if (!kept(i, keys[i])) return 0;
+            const uint64_t w = weight(keys[i]);
+            return w >= least ? w : 0;
+        };
+        int owner = 0;
+        while (goal >= before + sh.warp_u64[owner + 1]) ++owner;
+        const int first = owner * per_warp, part = per_warp / kSampleWarps;  // a multiple of 8
+        const int mine = first + warp * part;
+        uint64_t sum = 0;
+        for (int j = lane; j < part; j += 32) sum += mass(mine + j);
+        sum = warp_add_u64(sum);
+        const uint64_t start = before + sh.warp_u64[owner];
+        __syncthreads();
+        if (lane == 0) sh.warp_u64[warp] = sum;
+        __syncthreads();
+        uint64_t run = start;
+        for (int w = 0; w < warp; ++w) run += sh.warp_u64[w];
+        if (goal >= run && goal < run + sum) {
+            for (int j = 0; j < part; j += 32) {
+                const uint64_t w = j + lane < part ? mass(mine + j + lane) : 0;
+                const uint64_t end = run + warp_scan_u64(w, lane);
+                if (w > 0 && goal < end && goal >= end - w) {
+                    a.tokens[row] = base + mine + j + lane;
                     if (a.probs) a.probs[row] = float(double(w) / double(z));
                 }
-                run = __shfl_sync(0xffffffffu, upto, 31);
+                run = __shfl_sync(0xffffffffu, end, 31);
             }
         }
     }

@@ -398,9 +398,9 @@ void sample_tokens(const ServeDevice&, const b2d_sample_request* rq, cudaStream_
     a.probs = rq->probs;
     int ranks = 1;
     while (ranks < kSampleMaxCluster && a.vocab > 4096 * ranks) ranks *= 2;
-    a.slice = ((a.vocab + ranks - 1) / ranks + kSampleThreads - 1) / kSampleThreads * kSampleThreads;
-    const size_t elem = rq->logits_type == B2D_TYPE_F32 ? 4 : 2;
-    const size_t smem = ((sizeof(SampleShared) + 15) & ~size_t(15)) + size_t(a.slice) * elem;
+    constexpr int kStep = kSampleWarps * 128;  // a warp's share is whole steps of four entries a lane
+    a.slice = ((a.vocab + ranks - 1) / ranks + kStep - 1) / kStep * kStep;
+    const size_t smem = ((sizeof(SampleShared) + 15) & ~size_t(15)) + size_t(a.slice) * 4;
     constexpr int kLimit = int((sizeof(SampleShared) + 15) & ~size_t(15)) + kSampleMaxSlice * 4;
     auto go = [&](auto kernel) {
         set_smem_limit(kernel, kLimit);
