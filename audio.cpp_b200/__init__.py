@@ -36,7 +36,7 @@ EXPORTED = ["b2d_create", "b2d_destroy", "b2d_last_error", "b2d_sync", "b2d_vers
             "b2d_saocond_load", "b2d_saocond_encode", "b2d_saocond_encode_device",
             "b2d_vvlm_load", "b2d_vvlm_prefill", "b2d_vvlm_step", "b2d_vvlm_prefill_device", "b2d_vvlm_step_device",
             "b2d_kv_check", "b2d_kv_append", "b2d_kv_gather", "b2d_paged_attention_workspace", "b2d_paged_attention",
-            "b2d_sample_tokens"]
+            "b2d_vvlm_paged_workspace", "b2d_vvlm_forward_paged", "b2d_sample_tokens"]
 
 
 class B2DError(RuntimeError):
@@ -206,6 +206,9 @@ def lib() -> C.CDLL:
         L.b2d_paged_attention_workspace.restype = C.c_size_t
         L.b2d_paged_attention.argtypes = [P, C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), I32, P, I64, P, I64, I32, F,
                                           I32, P, C.c_size_t, P]
+        L.b2d_vvlm_paged_workspace.argtypes = [P, C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc)]
+        L.b2d_vvlm_paged_workspace.restype = C.c_size_t
+        L.b2d_vvlm_forward_paged.argtypes = [P, C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), P, P, P, P, C.c_size_t, P]
         L.b2d_sample_tokens.argtypes = [P, C.POINTER(SampleRequest), P]
         _lib = L
     return _lib
@@ -798,6 +801,40 @@ class VibeVoiceLanguageModel:
         """One cached position from a device embedding [hidden]; outputs as prefill_device."""
         self.ctx.check(lib().b2d_vvlm_step_device(self.ctx.handle, _ptr(embedding), _ptr(logits), _ptr(hidden),
                                                   C.c_void_p(stream)))
+
+
+    # ---- many sequences over paged caches (one PagedCache a layer), see b2d_vvlm_forward_paged
+    def _paged(self, caches, batch: PagedBatch):
+        if len(caches) != self.cfg.layers:
+            raise B2DError(-1, "the decoder has %d layers, got %d paged caches" % (self.cfg.layers, len(caches)))
+        for cache in caches:
+            batch.fits(cache)
+            if cache.device != self.ctx.device or batch.device != self.ctx.device:
+                raise self.ctx._elsewhere("a cache or batch tensor")
+        return (KvCacheDesc * len(caches))(*[cache.desc for cache in caches])
+
+    def paged_workspace(self, caches, batch: PagedBatch) -> int:
+        """Bytes of workspace forward_paged needs for batches of these bounds."""
+        need = lib().b2d_vvlm_paged_workspace(self.ctx.handle, self._paged(caches, batch), batch.ref)
+        if need == 0:
+            raise B2DError(-1, lib().b2d_last_error(self.ctx.handle).decode())
+        return need
+
+    def forward_paged(self, embeddings, caches, batch: PagedBatch, logits, hidden=None, workspace=None,
+                      stream: int = 0) -> None:
+        """The batch's new tokens (embeddings [rows, hidden]) through the decoder over paged caches: logits
+        [seqs, vocab] and, unless None, hidden [seqs, hidden] of each sequence's last new token.  Device float32."""
+        descs = self._paged(caches, batch)
+        seqs = batch.context.shape[0]
+        for name, t, shape in (("embeddings", embeddings, (batch.rows, self.cfg.hidden)),
+                               ("logits", logits, (seqs, self.cfg.vocab)), ("hidden", hidden, (seqs, self.cfg.hidden))):
+            if t is not None:
+                _want(t, name, shape, TYPE_F32)
+                if t.get_device() != self.ctx.device:
+                    raise self.ctx._elsewhere(name)
+        self.ctx.check(lib().b2d_vvlm_forward_paged(
+            self.ctx.handle, descs, batch.ref, _ptr(embeddings), _ptr(logits), _ptr(hidden) if hidden is not None else None,
+            _ptr(workspace) if workspace is not None else None, workspace.nbytes if workspace is not None else 0, stream))
 
 
 class VibeVoiceDiffusionHead:

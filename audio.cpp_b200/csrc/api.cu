@@ -8,6 +8,7 @@
 #include <cstdlib>
 #include <cstdio>
 #include <cstring>
+#include <algorithm>
 #include <atomic>
 #include <map>
 #include <mutex>
@@ -1614,6 +1615,30 @@ b2d_status b2d_paged_attention(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2
     return guarded(ctx, [&] {
         paged_attention(serve_device(ctx), cache, batch, bf16 != 0, q, q_row, o, o_row, heads, scale, window, workspace,
                         workspace_bytes, static_cast<cudaStream_t>(stream));
+    });
+}
+
+size_t b2d_vvlm_paged_workspace(b2d_ctx* ctx, const b2d_kv_cache* caches, const b2d_kv_batch* batch) {
+    size_t bytes = 0;
+    guarded(ctx, [&] {
+        if (!ctx->lm) fail(B2D_ESTATE, "VibeVoice decoder weights are not loaded");
+        lm_check_paged(*ctx->lm, caches, batch);
+        size_t attention = 0;
+        for (int64_t l = 0; l < ctx->lm->cfg.layers; ++l)
+            attention = std::max(attention, paged_attention_workspace(serve_device(ctx), &caches[l], batch,
+                                                                      int(ctx->lm->cfg.heads)));
+        bytes = std::max<size_t>(16, LmPagedPlan<__half>(*ctx->lm, batch->rows, batch->seqs, attention).bytes);
+    });
+    return bytes;
+}
+
+b2d_status b2d_vvlm_forward_paged(b2d_ctx* ctx, const b2d_kv_cache* caches, const b2d_kv_batch* batch,
+                                  const float* embeddings, float* logits, float* last_hidden, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+    return guarded(ctx, [&] {
+        if (!ctx->lm) fail(B2D_ESTATE, "VibeVoice decoder weights are not loaded");
+        lm_forward_paged<__half>(ctx, caches, batch, embeddings, logits, last_hidden, workspace, workspace_bytes,
+                                 static_cast<cudaStream_t>(stream));
     });
 }
 

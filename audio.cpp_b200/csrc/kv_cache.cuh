@@ -320,4 +320,41 @@ __global__ void __launch_bounds__(256, 8) kv_gather_kernel(KvView kv, BatchView 
     }
 }
 
+// NEOX RoPE of the batch's projected rows at their positions (a row without a place is not turned): q to fp16, k in place
+// in fp32, as the append takes it.  One thread per (row, head of q or k, pair); bound by HBM.
+__global__ void __launch_bounds__(256) rope_rows_kernel(BatchView b, float* __restrict__ qkv, int heads, int kv_heads,
+                                                        int head_dim, const float* __restrict__ cs,
+                                                        const float* __restrict__ sn, __half* __restrict__ q16) {
+    extern __shared__ int kv_batch_sm[];
+    int* start = kv_batch_sm;
+    int* context = kv_batch_sm + b.seqs + 1;
+    stage_batch(b, start, context);
+    const int half = head_dim >> 1, slots = heads + kv_heads, ld = (heads + 2 * kv_heads) * head_dim;
+    const int64_t total = int64_t(b.rows) * slots * half;
+    for (int64_t i = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; i < total; i += int64_t(gridDim.x) * blockDim.x) {
+        const int j = int(i % half), slot = int(i / half % slots), row = int(i / (int64_t(half) * slots));
+        const RowPlace at = place_row(b, start, context, row);
+        const int64_t t = int64_t(max(at.pos, 0)) * half + j;
+        const float c = cs[t], s = sn[t];
+        float* x = qkv + int64_t(row) * ld + slot * head_dim + j;
+        const float x0 = x[0], x1 = x[half];
+        const float y0 = x0 * c - x1 * s, y1 = x0 * s + x1 * c;
+        if (slot < heads) {
+            __half* q = q16 + (int64_t(row) * heads + slot) * head_dim + j;
+            q[0] = __float2half_rn(y0);
+            q[half] = __float2half_rn(y1);
+        } else {
+            x[0] = y0;
+            x[half] = y1;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) last_rows_kernel(BatchView b, const float* __restrict__ x, int width,
+                                                        float* __restrict__ out) {
+    const SeqSpan s = seq_span(b, int(blockIdx.x), false);
+    const float* src = x + int64_t(s.first + s.n - 1) * width;
+    for (int j = threadIdx.x; j < width; j += blockDim.x) out[int64_t(blockIdx.x) * width + j] = s.n > 0 ? src[j] : 0.f;
+}
+
 }  // namespace b2d

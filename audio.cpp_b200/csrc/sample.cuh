@@ -96,18 +96,15 @@ struct SampleShared {
     uint64_t cut;          // last kept (ordered bits, ~index)
 };
 
-// exp(t) in units of 2^-45 for -32 < t <= 0, to the nearest unit but for some 2^-46: t log2 e = n + i / 64 + r with
-// |r| <= 1 / 128, 2^r by its Taylor polynomial of degree 4 (the next term is below 2^-44.5), 2^(i / 64) from a table.
-__device__ __forceinline__ uint64_t exp_units(double t, const double* power) {
+// 2^(y / 64) in units of 2^-45 for -32 < y ln 2 / 64 <= 0, to within two units: y = 64 n + i + f with |f| <= 1 / 2,
+// 2^(f / 64) by its Taylor polynomial of degree 4 (the next term is below 2^-44.5), 2^(i / 64) from a table.
+__device__ __forceinline__ uint64_t exp_units(double y, const double* power) {
     constexpr double kMagic = 6755399441055744.0;  // 1.5 x 2^52: adding it rounds to an integer in the low bits
-    const double y = t * 92.33248261689366;        // 64 log2 e
+    constexpr double c1 = 0.010830424696249145, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6, c4 = c2 * c2 / 6;  // ln 2 / 64
     const double z = y + kMagic;
     const int i = __double2loint(z);
-    const double r = (y - (z - kMagic)) * 0.010830424696249145;  // ln 2 / 64
-    double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
-    p = fma(r, p, 0.5);
-    p = fma(r, p, 1.0);
-    p = fma(r, p, 1.0);
+    const double f = y - (z - kMagic);
+    const double p = fma(f, fma(f, fma(f, fma(f, c4, c3), c2), c1), 1.0);
     const double w = p * power[i & 63];
     // times 2^(n + 45) by the exponent bits, then to an integer by the same trick
     const double u = __hiloint2double(__double2hiint(w) + (((i >> 6) + 45) << 20), __double2loint(w)) + kMagic;
@@ -193,12 +190,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         return;
     }
     const float m = from_ordered(best_key);
-    const double inv_t = 1.0 / double(temp);
+    const double inv_t = 1.0 / double(temp), scale = inv_t * 92.33248261689366;  // 64 log2 e / T
+    const float deepest = m - 31.93f * temp;  // weights below it are under half a unit
     auto weight = [&](uint32_t key) -> uint64_t {
         if (key == best_key) return uint64_t(kSampleUnit);
-        const double t = (double(from_ordered(key)) - double(m)) * inv_t;
-        if (!(t > -31.9)) return 0;  // under half a unit
-        return exp_units(t, sh.power);
+        const float v = from_ordered(key);
+        if (!(v >= deepest)) return 0;
+        return exp_units((double(v) - double(m)) * scale, sh.power);
     };
 
     uint64_t cut = 0;  // entries at or above it (as (ordered bits, ~index)) are kept

@@ -182,6 +182,25 @@ void kv_gather(const ServeDevice& dev, const b2d_kv_cache* cache, const b2d_kv_b
     else gather_as<__nv_bfloat16>(kind, kv, b, k, v, row_stride, grid, st);
 }
 
+void rope_rows(const ServeDevice& dev, const b2d_kv_cache* cache, const b2d_kv_batch* batch, float* qkv, int heads,
+               const float* cos, const float* sin, void* q16, cudaStream_t st) {
+    const KvView kv = cache_view(cache);
+    const BatchView b = batch_view(batch, cache, dev.status);
+    if (b.rows == 0 || b.seqs == 0) return;
+    set_smem_limit(rope_rows_kernel, int((2 * kMaxSeqs + 1) * sizeof(int)));
+    const int64_t pairs = int64_t(b.rows) * (heads + kv.kv_heads) * (kv.head_dim / 2);
+    const int grid = int(std::min<int64_t>((pairs + 255) / 256, int64_t(dev.num_sms) * 8));
+    launch_k(rope_rows_kernel, dim3(unsigned(grid)), dim3(256), batch_smem(b), st, 1, b, qkv, heads, kv.kv_heads, kv.head_dim,
+             cos, sin, static_cast<__half*>(q16));
+}
+
+void last_rows(const ServeDevice& dev, const b2d_kv_cache* cache, const b2d_kv_batch* batch, const float* x, int width,
+               float* out, cudaStream_t st) {
+    const BatchView b = batch_view(batch, cache, dev.status);
+    if (b.seqs == 0) return;
+    launch_k(last_rows_kernel, dim3(unsigned(b.seqs)), dim3(256), 0, st, 1, b, x, width, out);
+}
+
 // ------------------------------------------------------------------------------------------------- attention
 namespace {
 

@@ -496,6 +496,23 @@ B2D_API b2d_status b2d_paged_attention(b2d_ctx* ctx, const b2d_kv_cache* cache, 
                                        const void* q, int64_t q_row, void* o, int64_t o_row, int32_t heads, float scale,
                                        int32_t window, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------ serving the language model: paged forward */
+/* The loaded decoder (b2d_vvlm_load) over paged caches that the caller owns: what b2d_vvlm_prefill and b2d_vvlm_step do
+ * for one sequence and the context's own cache, for the new tokens of many sequences at once (whole prompts, chunks of
+ * them, single tokens, mixed).  The calls of either kind do not touch the other's cache.
+ *   caches: [layers] (host array), kv_heads and head_dim the model's, type F16, I8 or E4M3; layer l's keys and values of
+ *     the batch's rows are appended to caches[l] and attended to there, positions from the batch's contexts
+ *     (max_context at most the model's max_positions).
+ *   embeddings [rows, hidden], logits [seqs, vocab] and last_hidden [seqs, hidden] (may be NULL): device fp32; outputs
+ *     are those of each sequence's last new token (zeros in, so the logits of a zero row, for one without new tokens).
+ *   workspace: 16-byte aligned, b2d_vvlm_paged_workspace bytes for batches of these bounds (0: refused); calls that may
+ *     overlap need one each.
+ * Asynchronous on `stream`, allocates nothing, can be captured.  Check b2d_sync for device-side status. */
+B2D_API size_t b2d_vvlm_paged_workspace(b2d_ctx* ctx, const b2d_kv_cache* caches, const b2d_kv_batch* batch);
+B2D_API b2d_status b2d_vvlm_forward_paged(b2d_ctx* ctx, const b2d_kv_cache* caches, const b2d_kv_batch* batch,
+                                          const float* embeddings, float* logits, float* last_hidden, void* workspace,
+                                          size_t workspace_bytes, void* stream);
+
 /* --------------------------------------------------- serving the language model: sampling */
 /* The next token of each row of logits (the reference samples on the host, src/framework/sampling).  With m the
  * row's largest logit and w_i = exp((x_i - m) / temperature), entries ordered by (logit descending, index ascending):
@@ -503,8 +520,8 @@ B2D_API b2d_status b2d_paged_attention(b2d_ctx* ctx, const b2d_kv_cache* cache, 
  *   top-k left (the best entry always stays); min_p > 0 keeps those with w_i >= min(min_p, 1);
  *   the token is the first index whose running sum of kept weights, in index order, exceeds uniform times their sum.
  * temperature <= 0 takes the best entry.  A NaN logit counts as -infinity, +infinity as certain; a row without an
- * entry above -infinity gives token -1.  Weights are computed in fp64 and summed exactly in units of 2^-45 of the
- * largest, so the token depends on nothing but the arguments. */
+ * entry above -infinity gives token -1.  Weights are computed in fp64 to within 2^-44 of the largest and summed
+ * exactly in units of 2^-45 of it, so the token depends on nothing but the arguments. */
 typedef struct {
     int32_t logits_type;        /* B2D_TYPE_F32, B2D_TYPE_F16 or B2D_TYPE_BF16 */
     int64_t rows, vocab;        /* vocab 1 to 262144 */
