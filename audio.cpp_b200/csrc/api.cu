@@ -351,12 +351,14 @@ namespace {
 
 struct DeviceGuard {
     int prev = -1;
+    bool moved = false;
     explicit DeviceGuard(int dev) {
         cudaGetDevice(&prev);
-        if (prev != dev) cudaSetDevice(dev);
+        moved = prev != dev;
+        if (moved) cudaSetDevice(dev);
     }
     ~DeviceGuard() {
-        if (prev >= 0) cudaSetDevice(prev);
+        if (moved && prev >= 0) cudaSetDevice(prev);
     }
 };
 

@@ -605,4 +605,324 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     cluster.sync();
 }
 
+// ---- many rows of bf16 logits: weights by value
+// bf16 rows repeat a few thousand values, so a row is counted by value and every later step works on the counts: one fp64
+// weight a value instead of two an entry, exact masses without a search (a cut falls on one value and keeps its first
+// entries by index).  One CTA a row; the row is read once from HBM and twice more from L2 (to count it, and to find the
+// token).  Values are ordered bits of 16; those that differ only in the low 8 form a group, and the groups that occur
+// and weigh anything get 256 counters each, 32 groups at a time (a row has some twenty; more take further rounds).
+constexpr int kValueThreads = 512;
+constexpr int kValueWarps = kValueThreads / 32;
+constexpr int kValueGroups = 32;
+constexpr int kValueBins = kValueGroups * 256;
+
+struct ValueShared {
+    uint32_t count[kValueBins];   // of the window's values, descending
+    uint64_t weight[kValueBins];  // of one entry of the value
+    uint8_t present[256];
+    int slot[256];          // place of a group among those that count, descending, or -1
+    uint8_t group[256];     // .. and back
+    double power[64];
+    uint64_t best;
+    uint64_t warp_u64[kValueWarps];
+    uint32_t warp_u32[kValueWarps];
+    int groups;
+    int cut;                // place of the last kept value
+    uint32_t need;          // how many of its entries are kept, the first by index
+    uint64_t mass;          // kept
+};
+
+__device__ __forceinline__ uint32_t ordered_bits_16(uint32_t b) {  // 0: cannot be drawn
+    if ((b & 0x7fffu) > 0x7f80u || b == 0xff80u) return 0;
+    if (b == 0x8000u) b = 0;
+    return (b & 0x8000u) ? b ^ 0xffffu : b | 0x8000u;
+}
+__device__ __forceinline__ float value_of_16(uint32_t k) {
+    return __uint_as_float((k & 0x8000u ? k & 0x7fffu : k ^ 0xffffu) << 16);
+}
+
+__global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const SampleArgs a) {
+    extern __shared__ __align__(16) uint8_t sample_raw[];
+    ValueShared& sh = *reinterpret_cast<ValueShared*>(sample_raw);
+    const int row = int(blockIdx.x), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint16_t* src = static_cast<const uint16_t*>(a.logits) + int64_t(row) * a.row_stride;
+    const int skip = min(a.vocab, int((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / 2);
+    const int vectors = (a.vocab - skip) / 8;
+    // A warp owns consecutive vectors of eight entries; what lies before the first and behind the last belongs to the
+    // first and the last warp.
+    const int v0 = int(int64_t(vectors) * warp / kValueWarps), v1 = int(int64_t(vectors) * (warp + 1) / kValueWarps);
+    const int e0 = warp == 0 ? 0 : skip + v0 * 8, e1 = warp == kValueWarps - 1 ? a.vocab : skip + v1 * 8;
+    auto each = [&](auto&& f) {  // this lane's entries of its warp's share: f(index, ordered bits)
+        if (warp == 0)
+            for (int i = lane; i < skip; i += 32) f(i, ordered_bits_16(src[i]));
+#pragma unroll 2
+        for (int v = v0 + lane; v < v1; v += 32) {
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src + skip) + v);
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f(skip + v * 8 + 2 * e, ordered_bits_16(w[e] & 0xffffu));
+                f(skip + v * 8 + 2 * e + 1, ordered_bits_16(w[e] >> 16));
+            }
+        }
+        if (warp == kValueWarps - 1)
+            for (int i = skip + vectors * 8 + lane; i < a.vocab; i += 32) f(i, ordered_bits_16(src[i]));
+    };
+
+    // ---- the best entry, and the groups that occur
+    if (tid < 64) sh.power[tid] = exp2(double(tid) / 64.0);
+    if (tid < 256) sh.present[tid] = 0;
+    if (tid == 0) sh.best = 0;
+    __syncthreads();
+    uint32_t top = 0;
+    int top_at = 0;
+    each([&](int i, uint32_t key) {
+        if (key > top || (key == top && i < top_at)) top = key, top_at = i;
+        if (key) sh.present[key >> 8] = 1;
+    });
+    uint64_t best = top ? uint64_t(top) << 32 | uint32_t(~uint32_t(top_at)) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t y = __shfl_xor_sync(0xffffffffu, best, o);
+        best = best > y ? best : y;
+    }
+    if (lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&sh.best), (unsigned long long)best);
+    __syncthreads();
+    best = sh.best;
+    const uint32_t best_key = uint32_t(best >> 32);
+    const float temp = a.temperature[row];
+    if (best_key == 0 || !(temp > 0.f)) {
+        if (tid == 0) {
+            a.tokens[row] = best_key == 0 ? -1 : int(~uint32_t(best));
+            if (a.probs) a.probs[row] = best_key == 0 ? 0.f : 1.f;
+        }
+        return;
+    }
+    const float m = value_of_16(best_key);
+    const double scale = 1.0 / double(temp) * 92.33248261689366;  // 64 log2 e / T
+    const float deepest = m - 31.93f * temp;                      // weights below it are under half a unit
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const uint32_t want = k > 0 && k < a.vocab ? uint32_t(k) : 0xffffffffu;
+    // groups that count: those that occur, and reach above `deepest` (with top-k all of them: it counts entries of any weight)
+    if (tid < 256) {
+        const int g = 255 - tid;  // descending
+        const float v = g == 0xff ? INFINITY : value_of_16(uint32_t(g) << 8 | 0xffu);  // the largest value of the group
+        const bool there = sh.present[g] && (v >= deepest || want != 0xffffffffu || uint32_t(g) == best_key >> 8);
+        const uint32_t vote = __ballot_sync(0xffffffffu, there);
+        sh.warp_u32[warp] = __popc(vote);
+        sh.slot[g] = there ? __popc(vote & ((1u << lane) - 1u)) : -1;
+    }
+    __syncthreads();
+    if (tid < 256) {
+        const int g = 255 - tid;
+        int before = 0;
+        for (int w = 0; w < warp; ++w) before += int(sh.warp_u32[w]);
+        if (sh.slot[g] >= 0) {
+            sh.slot[g] += before;
+            sh.group[sh.slot[g]] = uint8_t(g);
+        }
+        if (tid == 255) sh.groups = before + int(sh.warp_u32[warp]);
+    }
+    __syncthreads();
+    const int windows = (sh.groups + kValueGroups - 1) / kValueGroups;
+    auto place_of = [&](uint32_t key) -> int {  // among all values that count, descending; negative: does not count
+        const int s = sh.slot[key >> 8];
+        return s < 0 ? -1 : s * 256 + int(255u - (key & 255u));
+    };
+    auto weight_of = [&](uint32_t key) -> uint64_t {
+        if (key == best_key) return uint64_t(kSampleUnit);
+        const float v = value_of_16(key);
+        return v >= deepest ? exp_units((double(v) - double(m)) * scale, sh.power) : 0;
+    };
+    int built = -1;
+    auto build = [&](int win) {  // counts and weights of a window's values
+        if (built == win) return;
+        built = win;
+        __syncthreads();
+        for (int i = tid; i < kValueBins; i += kValueThreads) sh.count[i] = 0;
+        __syncthreads();
+        each([&](int, uint32_t key) {
+            const int at = place_of(key) - win * kValueBins;
+            if (key && at >= 0 && at < kValueBins) atomicAdd(&sh.count[at], 1u);
+        });
+        __syncthreads();
+        for (int i = tid; i < kValueBins; i += kValueThreads) {
+            const int g = win * kValueGroups + (i >> 8);
+            sh.weight[i] = sh.count[i] ? weight_of(uint32_t(sh.group[g]) << 8 | (255u - uint32_t(i & 255))) : 0;
+        }
+        __syncthreads();
+    };
+    // Walks the values in order until one ends the prefix: by counts the one that holds entry `want`, by mass the one that
+    // holds the last entry with less than `target` before it; entries behind (cut, need) are gone already.  Leaves the
+    // new (cut, need) and the kept mass.
+    auto find_cut = [&](uint32_t entries, bool by_mass, uint64_t target) {
+        const int old_cut = sh.cut;
+        const uint32_t old_need = sh.need;
+        uint32_t run_c = 0;
+        uint64_t run_m = 0;
+        __syncthreads();
+        if (tid == 0) sh.cut = -1;
+        __syncthreads();
+        constexpr int kEach = kValueBins / kValueThreads;
+        for (int win = 0; win < windows; ++win) {
+            build(win);
+            uint32_t own_c = 0;
+            uint64_t own_m = 0;
+            auto counted = [&](int i) -> uint32_t {  // entries of the window's value i that are still there
+                const int at = win * kValueBins + i;
+                return at < old_cut ? sh.count[i] : at == old_cut ? min(old_need, sh.count[i]) : 0u;
+            };
+            for (int e = 0; e < kEach; ++e) {
+                const uint32_t c = counted(tid * kEach + e);
+                own_c += c;
+                own_m += c ? c * sh.weight[tid * kEach + e] : 0;
+            }
+            uint32_t c = own_c;
+            uint64_t ms = warp_scan_u64(own_m, lane);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, c, o);
+                if (lane >= o) c += y;
+            }
+            if (lane == 31) sh.warp_u64[warp] = ms, sh.warp_u32[warp] = c;
+            __syncthreads();
+            c += run_c - own_c;
+            ms += run_m - own_m;
+            for (int w = 0; w < kValueWarps; ++w) {
+                if (w < warp) c += sh.warp_u32[w], ms += sh.warp_u64[w];
+                run_c += sh.warp_u32[w], run_m += sh.warp_u64[w];
+            }
+            int last = -1;
+            for (int e = 0; e < kEach; ++e) {
+                const int i = tid * kEach + e;
+                const uint32_t n = counted(i);
+                if (n > 0 && (by_mass ? ms < target : c < entries)) last = win * kValueBins + i;
+                c += n;
+                ms += n ? n * sh.weight[i] : 0;
+            }
+            last = __reduce_max_sync(0xffffffffu, last);
+            if (lane == 0 && last >= 0) atomicMax(&sh.cut, last);
+            __syncthreads();
+            // the thread that holds the window's last such value says how many of its entries are kept, and the mass
+            const int i = sh.cut - win * kValueBins;
+            if (i >= 0 && i / kEach == tid) {
+                for (int e = kEach - 1; e >= i % kEach; --e) {
+                    const uint32_t n = counted(tid * kEach + e);
+                    c -= n;
+                    ms -= n ? n * sh.weight[tid * kEach + e] : 0;
+                }
+                const uint32_t n = counted(i);
+                const uint64_t w = sh.weight[i];
+                const uint64_t most = by_mass ? (w ? (target - ms + w - 1) / w : n) : entries - c;
+                sh.need = uint32_t(most < n ? most : n);
+                sh.mass = ms + sh.need * w;
+            }
+            __syncthreads();
+            // behind a window that the prefix ends in, nothing is kept
+            if (by_mass ? run_m >= target : run_c >= entries) break;
+        }
+    };
+    __syncthreads();
+    if (tid == 0) sh.cut = 0x7fffffff, sh.need = 0xffffffffu;
+    __syncthreads();
+    find_cut(want, false, 0);  // without top-k: everything, for its mass
+    const float p = a.top_p ? a.top_p[row] : 1.f, floor_p = a.min_p ? a.min_p[row] : 0.f;
+    if (p < 1.f) {
+        const uint64_t target = p > 0.f ? uint64_t(ceil(double(p) * double(sh.mass))) : 1u;
+        find_cut(0, true, target > 0 ? target : 1u);
+    }
+    const uint64_t least = floor_p > 0.f ? uint64_t(ceil(double(fminf(floor_p, 1.f)) * kSampleUnit)) : 0;
+    const int cut = sh.cut;
+    const uint32_t need = sh.need;
+
+    // ---- the token: the kept mass of every warp's share, of its sixteen parts, of single entries
+    // Mass of an entry above the cut value (a window's at a time), and whether it is one of the cut value's.
+    auto share = [&](int first, int last, bool vector, uint64_t& mass, uint32_t& ties) {
+        mass = 0;
+        ties = 0;
+        for (int win = 0; win < windows; ++win) {
+            if (win * kValueBins > cut) break;
+            build(win);
+            auto add = [&](int, uint32_t key) {
+                const int at = place_of(key), i = at - win * kValueBins;
+                if (!key || i < 0 || i >= kValueBins || at > cut) return;
+                if (at == cut) {
+                    ++ties;
+                } else {
+                    const uint64_t w = sh.weight[i];
+                    mass += w >= least ? w : 0;
+                }
+            };
+            if (vector) {
+                each(add);
+            } else {
+                for (int i = first + lane; i < last; i += 32) add(i, ordered_bits_16(src[i]));
+            }
+        }
+        mass = warp_add_u64(mass);
+        ties = __reduce_add_sync(0xffffffffu, ties);
+    };
+    const uint32_t cut_key = uint32_t(sh.group[cut >> 8]) << 8 | (255u - uint32_t(cut & 255));
+    const uint64_t raw_cut = weight_of(cut_key), cut_weight = raw_cut >= least ? raw_cut : 0;
+    uint64_t mass;
+    uint32_t ties;
+    share(e0, e1, true, mass, ties);
+    __syncthreads();
+    if (lane == 0) sh.warp_u64[warp] = mass, sh.warp_u32[warp] = ties;
+    __syncthreads();
+    auto kept_ties = [&](uint32_t seen, uint32_t here) { return seen >= need ? 0u : min(need - seen, here); };
+    uint64_t z = 0;
+    uint32_t seen = 0;
+    for (int w = 0; w < kValueWarps; ++w) {
+        z += sh.warp_u64[w] + kept_ties(seen, sh.warp_u32[w]) * cut_weight;
+        seen += sh.warp_u32[w];
+    }
+    float u = a.uniform[row];
+    u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+    uint64_t goal = uint64_t(double(u) * double(z));  // the token is the first whose running sum is above it
+    if (goal >= z) goal = z - 1;
+    auto descend = [&](uint64_t& run, uint32_t& before) -> int {  // the part of the sixteen that holds the goal
+        for (int w = 0; w < kValueWarps; ++w) {
+            const uint64_t next = run + sh.warp_u64[w] + kept_ties(before, sh.warp_u32[w]) * cut_weight;
+            if (goal < next) return w;
+            run = next;
+            before += sh.warp_u32[w];
+        }
+        return kValueWarps - 1;
+    };
+    uint64_t run = 0;
+    uint32_t before = 0;
+    const int owner = descend(run, before);
+    const int o0 = owner == 0 ? 0 : skip + int(int64_t(vectors) * owner / kValueWarps) * 8;
+    const int o1 = owner == kValueWarps - 1 ? a.vocab : skip + int(int64_t(vectors) * (owner + 1) / kValueWarps) * 8;
+    auto bound = [&](int w) { return o0 + int(int64_t(o1 - o0) * w / kValueWarps); };
+    share(bound(warp), bound(warp + 1), false, mass, ties);
+    __syncthreads();
+    if (lane == 0) sh.warp_u64[warp] = mass, sh.warp_u32[warp] = ties;
+    __syncthreads();
+    const int part = descend(run, before);
+    if (warp != part) return;
+    for (int i0 = bound(part); i0 < bound(part + 1); i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t key = i < bound(part + 1) ? ordered_bits_16(src[i]) : 0u;
+        const int at = key ? place_of(key) : -1;
+        const bool tie = at == cut && at >= 0;
+        const uint32_t vote = __ballot_sync(0xffffffffu, tie);
+        uint64_t w = 0;
+        if (at >= 0 && at < cut) {
+            w = weight_of(key);
+            w = w >= least ? w : 0;
+        } else if (tie && before + __popc(vote & ((1u << lane) - 1u)) < need) {
+            w = cut_weight;
+        }
+        const uint64_t end = run + warp_scan_u64(w, lane);
+        if (w > 0 && goal < end && goal >= end - w) {
+            a.tokens[row] = i;
+            if (a.probs) a.probs[row] = float(double(w) / double(z));
+        }
+        run = __shfl_sync(0xffffffffu, end, 31);
+        before += __popc(vote);
+    }
+}
+
 }  // namespace b2d

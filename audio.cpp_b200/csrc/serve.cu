@@ -388,6 +388,9 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
 }
 
 // -------------------------------------------------------------------------------------------------- sampling
+// bf16 rows from which a CTA each, counting values, is faster than a cluster each, weighing entries.
+constexpr int64_t kValueRows = 24;
+
 void sample_tokens(const ServeDevice&, const b2d_sample_request* rq, cudaStream_t st) {
     if (!rq) fail(B2D_EINVAL, "sampling request is missing");
     if (rq->logits_type != B2D_TYPE_F32 && rq->logits_type != B2D_TYPE_F16 && rq->logits_type != B2D_TYPE_BF16)
@@ -415,6 +418,12 @@ void sample_tokens(const ServeDevice&, const b2d_sample_request* rq, cudaStream_
     a.uniform = rq->uniform;
     a.tokens = rq->tokens;
     a.probs = rq->probs;
+    if (rq->logits_type == B2D_TYPE_BF16 && rq->rows >= kValueRows) {
+        constexpr int bytes = int(sizeof(ValueShared));
+        set_smem_limit(sample_values_kernel, bytes);
+        launch_k(sample_values_kernel, dim3(unsigned(rq->rows)), dim3(kValueThreads), bytes, st, 1, a);
+        return;
+    }
     int ranks = 1;
     while (ranks < kSampleMaxCluster && a.vocab > 4096 * ranks) ranks *= 2;
     constexpr int kStep = kSampleWarps * 128;  // a warp's share is whole steps of four entries a lane

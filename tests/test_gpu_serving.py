@@ -106,6 +106,9 @@ def draw_token(logits, t, k, p, mp, u):
         return int(np.argmax(z)), 1.0
     with np.errstate(invalid="ignore"):
         w = np.where(z == m, 1.0, np.where(z == -np.inf, 0.0, np.exp((z - m) / t)))
+    # half a unit: an entry below 2^-46 of the best is never drawn, not even by u = 0 (its probability is below 2^-46, which
+    # no other u of 24 bits can tell from none)
+    w = np.where(w < 2.0 ** -46, 0.0, w)
     order = np.argsort(-z, kind="stable")
     if k is not None and k > 0:
         order = order[:k]
@@ -564,6 +567,49 @@ def test_sampling_largest_vocabulary_and_strides(b2d, ctx):
     wide = torch.tensor(rng.standard_normal((3, 262144 + 7)), dtype=torch.float32, device=DEV)
     sample(ctx, wide[:, 3:262144 + 3], 1.0, k=[0, 2000, 0], p=[1.0, 1.0, 0.97], u=rng.random(3))
     sample(ctx, wide[:, 1:1000].bfloat16()[:, 1:], 1.0, p=0.5, u=rng.random(3))
+
+
+@pytest.mark.parametrize("vocab", [1, 7, 300, 4099, 70001, 262144])
+def test_sampling_many_bf16_rows(b2d, ctx, vocab):
+    """Batches of bf16 rows, which are counted by value: every cut and their combinations, rows that begin off a 16-byte
+    boundary, few values with many ties, masks, infinities, NaN, values over the whole range of exponents (more groups
+    of values than are counted at a time), extreme temperatures."""
+    rows = 48
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((rows, vocab + 3)) * 3
+    x[1] = 0.0
+    x[2] = rng.integers(-3, 4, vocab + 3)
+    x[3] = np.where(rng.random(vocab + 3) < 0.9, -np.inf, x[3])
+    x[4, 1:] = float(torch.finfo(torch.bfloat16).min)
+    x[5] = float(torch.finfo(torch.bfloat16).min)
+    x[6, ::3] = np.nan
+    x[7, vocab // 2:] = np.inf
+    x[8] = -np.inf
+    x[9] = np.nan
+    x[10] = rng.choice([-1, 1], vocab + 3) * 2.0 ** rng.uniform(-120, 100, vocab + 3)
+    x[11] = rng.choice([-1, 1], vocab + 3) * 2.0 ** rng.uniform(-120, 3, vocab + 3)
+    x[12] = -np.abs(x[12])
+    x[13, ::2] = -0.0
+    x[13, 1::2] = 0.0
+    x[14] = 1e5 + x[14]
+    x[15] = 200.0 + rng.integers(0, 2, vocab + 3)
+    logits = torch.tensor(x, dtype=torch.float32, device=DEV).bfloat16()[:, 1:vocab + 1]
+    t = rng.uniform(0.3, 1.5, rows).astype(np.float32)
+    t[[16, 17, 18, 19, 20]] = [0.0, 1e-20, 1e20, np.inf, -3.0]
+    t[10], t[11] = 2.0 ** 90, 1.0
+    u = rng.random(rows).astype(np.float32)
+    u[21:24] = [0.0, 1 - 2.0 ** -24, 1.0]
+    k = rng.integers(0, max(2, vocab // 3), rows)
+    k[[1, 2]] = max(1, vocab // 2)
+    p = rng.uniform(0, 1, rows).astype(np.float32)
+    p[[24, 25]] = [0.0, 1.0]
+    mp = rng.uniform(0, 0.5, rows).astype(np.float32)
+    sample(ctx, logits, t, u=u)
+    sample(ctx, logits, t, k=k, u=u)
+    sample(ctx, logits, t, p=p, u=u)
+    sample(ctx, logits, t, mp=mp, u=u)
+    sample(ctx, logits, t, k=k, p=p, mp=mp * 0.1, u=u)
+    sample(ctx, logits, t, k=np.minimum(k, 40), p=np.maximum(p, 0.5), u=u)
 
 
 # ------------------------------------------------------------------------------------------------ together
