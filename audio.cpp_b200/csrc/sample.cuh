@@ -611,6 +611,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
 // entries by index).  One CTA a row; the row is read once from HBM and twice more from L2 (to count it, and to find the
 // token).  Values are ordered bits of 16; those that differ only in the low 8 form a group, and the groups that occur
 // and weigh anything get 256 counters each, 32 groups at a time (a row has some twenty; more take further rounds).
+// Bound by integer instructions (a pass over 256 x 151937 entries took 40 an entry, 80 us, when it turned each into ordered
+// bits): a table of the 256 high bytes gives an entry's counter from its raw bits in one lookup and one logic operation.
 constexpr int kValueThreads = 512;
 constexpr int kValueWarps = kValueThreads / 32;
 constexpr int kValueGroups = 32;
@@ -621,6 +623,7 @@ struct ValueShared {
     uint64_t weight[kValueBins];  // of one entry of the value
     uint8_t present[256];
     int slot[256];          // place of a group among those that count, descending, or -1
+    int table[256];         // by raw high byte: slot x 256 + what turns the low byte; kNotCounted; kSpecial
     uint8_t group[256];     // .. and back
     double power[64];
     uint64_t best;
@@ -631,6 +634,8 @@ struct ValueShared {
     uint32_t need;          // how many of its entries are kept, the first by index
     uint64_t mass;          // kept
 };
+
+constexpr int kNotCounted = -1, kSpecial = -2;  // kSpecial: NaN, infinities and -0 among them, looked at one by one
 
 __device__ __forceinline__ uint32_t ordered_bits_16(uint32_t b) {  // 0: cannot be drawn
     if ((b & 0x7fffu) > 0x7f80u || b == 0xff80u) return 0;
@@ -652,21 +657,26 @@ __global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const S
     // first and the last warp.
     const int v0 = int(int64_t(vectors) * warp / kValueWarps), v1 = int(int64_t(vectors) * (warp + 1) / kValueWarps);
     const int e0 = warp == 0 ? 0 : skip + v0 * 8, e1 = warp == kValueWarps - 1 ? a.vocab : skip + v1 * 8;
-    auto each = [&](auto&& f) {  // this lane's entries of its warp's share: f(index, ordered bits)
+    auto each = [&](auto&& f, auto&& f2) {  // this lane's entries of its warp's share: f(index, bits), f2(index, two of them)
         if (warp == 0)
-            for (int i = lane; i < skip; i += 32) f(i, ordered_bits_16(src[i]));
-#pragma unroll 2
-        for (int v = v0 + lane; v < v1; v += 32) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src + skip) + v);
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            for (int i = lane; i < skip; i += 32) f(i, uint32_t(src[i]));
+        for (int v = v0 + lane; v < v1; v += 128) {
+            uint4 raw[4];  // 64 bytes a lane on their way
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                f(skip + v * 8 + 2 * e, ordered_bits_16(w[e] & 0xffffu));
-                f(skip + v * 8 + 2 * e + 1, ordered_bits_16(w[e] >> 16));
+            for (int d = 0; d < 4; ++d)
+                if (v + 32 * d < v1) raw[d] = __ldg(reinterpret_cast<const uint4*>(src + skip) + v + 32 * d);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                if (v + 32 * d >= v1) break;
+                const int i = skip + (v + 32 * d) * 8;
+                f2(i, raw[d].x), f2(i + 2, raw[d].y), f2(i + 4, raw[d].z), f2(i + 6, raw[d].w);
             }
         }
         if (warp == kValueWarps - 1)
-            for (int i = skip + vectors * 8 + lane; i < a.vocab; i += 32) f(i, ordered_bits_16(src[i]));
+            for (int i = skip + vectors * 8 + lane; i < a.vocab; i += 32) f(i, uint32_t(src[i]));
+    };
+    auto one_by_one = [&](auto&& f) {
+        each(f, [&](int i, uint32_t two) { f(i, two & 0xffffu), f(i + 1, two >> 16); });
     };
 
     // ---- the best entry, and the groups that occur
@@ -674,26 +684,36 @@ __global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const S
     if (tid < 256) sh.present[tid] = 0;
     if (tid == 0) sh.best = 0;
     __syncthreads();
-    uint32_t top = 0;
-    int top_at = 0;
-    each([&](int i, uint32_t key) {
-        if (key > top || (key == top && i < top_at)) top = key, top_at = i;
-        if (key) sh.present[key >> 8] = 1;
+    __nv_bfloat162 most2 = __float2bfloat162_rn(-INFINITY);  // the larger of each pair; NaN only against NaN
+    auto look = [&](int, uint32_t b) {
+        sh.present[b >> 8] = 1;
+        const __nv_bfloat16 v = __ushort_as_bfloat16((unsigned short)b);
+        most2 = __hmax2(most2, __halves2bfloat162(v, v));
+    };
+    each(look, [&](int, uint32_t two) {
+        sh.present[(two >> 8) & 0xffu] = 1;
+        sh.present[two >> 24] = 1;
+        most2 = __hmax2(most2, *reinterpret_cast<const __nv_bfloat162*>(&two));
     });
-    uint64_t best = top ? uint64_t(top) << 32 | uint32_t(~uint32_t(top_at)) : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t y = __shfl_xor_sync(0xffffffffu, best, o);
-        best = best > y ? best : y;
-    }
-    if (lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&sh.best), (unsigned long long)best);
+    uint32_t top = max(ordered_bits_16(__bfloat16_as_ushort(__low2bfloat16(most2))),
+                       ordered_bits_16(__bfloat16_as_ushort(__high2bfloat16(most2))));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&sh.best), (unsigned long long)top);
     __syncthreads();
-    best = sh.best;
-    const uint32_t best_key = uint32_t(best >> 32);
+    const uint32_t best_key = uint32_t(sh.best);
     const float temp = a.temperature[row];
     if (best_key == 0 || !(temp > 0.f)) {
+        __syncthreads();
+        if (tid == 0) sh.best = 0xffffffffu;
+        __syncthreads();
+        uint32_t at = 0xffffffffu;  // the first of the best
+        if (best_key)
+            one_by_one([&](int i, uint32_t b) { at = ordered_bits_16(b) == best_key ? min(at, uint32_t(i)) : at; });
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) atomicMin(reinterpret_cast<unsigned long long*>(&sh.best), (unsigned long long)at);
+        __syncthreads();
         if (tid == 0) {
-            a.tokens[row] = best_key == 0 ? -1 : int(~uint32_t(best));
+            a.tokens[row] = best_key == 0 ? -1 : int(sh.best);
             if (a.probs) a.probs[row] = best_key == 0 ? 0.f : 1.f;
         }
         return;
@@ -707,7 +727,9 @@ __global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const S
     if (tid < 256) {
         const int g = 255 - tid;  // descending
         const float v = g == 0xff ? INFINITY : value_of_16(uint32_t(g) << 8 | 0xffu);  // the largest value of the group
-        const bool there = sh.present[g] && (v >= deepest || want != 0xffffffffu || uint32_t(g) == best_key >> 8);
+        // raw high byte of the group; 0x80 also holds -0, which counts with +0
+        const bool occurs = sh.present[g & 0x80 ? g & 0x7f : g ^ 0xff] || (g == 0x80 && sh.present[0x80]);
+        const bool there = occurs && (v >= deepest || want != 0xffffffffu || uint32_t(g) == best_key >> 8);
         const uint32_t vote = __ballot_sync(0xffffffffu, there);
         sh.warp_u32[warp] = __popc(vote);
         sh.slot[g] = there ? __popc(vote & ((1u << lane) - 1u)) : -1;
@@ -721,6 +743,10 @@ __global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const S
             sh.slot[g] += before;
             sh.group[sh.slot[g]] = uint8_t(g);
         }
+        const int raw = g & 0x80 ? g & 0x7f : g ^ 0xff;
+        sh.table[raw] = raw == 0x7f || raw == 0xff || raw == 0x80 ? kSpecial
+                        : sh.slot[g] < 0                          ? kNotCounted
+                                                                  : sh.slot[g] * 256 + (g & 0x80 ? 0xff : 0);
         if (tid == 255) sh.groups = before + int(sh.warp_u32[warp]);
     }
     __syncthreads();
@@ -728,6 +754,13 @@ __global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const S
     auto place_of = [&](uint32_t key) -> int {  // among all values that count, descending; negative: does not count
         const int s = sh.slot[key >> 8];
         return s < 0 ? -1 : s * 256 + int(255u - (key & 255u));
+    };
+    auto place_of_raw = [&](uint32_t b) -> int {
+        const int t = sh.table[b >> 8];
+        if (t >= 0) return (t & ~0xff) | ((t ^ int(b)) & 0xff);
+        if (t == kNotCounted) return -1;
+        const uint32_t key = ordered_bits_16(b);
+        return key ? place_of(key) : -1;
     };
     auto weight_of = [&](uint32_t key) -> uint64_t {
         if (key == best_key) return uint64_t(kSampleUnit);
@@ -741,9 +774,9 @@ __global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const S
         __syncthreads();
         for (int i = tid; i < kValueBins; i += kValueThreads) sh.count[i] = 0;
         __syncthreads();
-        each([&](int, uint32_t key) {
-            const int at = place_of(key) - win * kValueBins;
-            if (key && at >= 0 && at < kValueBins) atomicAdd(&sh.count[at], 1u);
+        one_by_one([&](int, uint32_t b) {
+            const uint32_t at = uint32_t(place_of_raw(b) - win * kValueBins);
+            if (at < uint32_t(kValueBins)) atomicAdd(&sh.count[at], 1u);
         });
         __syncthreads();
         for (int i = tid; i < kValueBins; i += kValueThreads) {
@@ -760,67 +793,63 @@ __global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const S
         const uint32_t old_need = sh.need;
         uint32_t run_c = 0;
         uint64_t run_m = 0;
-        __syncthreads();
-        if (tid == 0) sh.cut = -1;
-        __syncthreads();
-        constexpr int kEach = kValueBins / kValueThreads;
+        constexpr int kShare = kValueBins / kValueWarps;  // consecutive values a warp looks at
         for (int win = 0; win < windows; ++win) {
             build(win);
-            uint32_t own_c = 0;
-            uint64_t own_m = 0;
             auto counted = [&](int i) -> uint32_t {  // entries of the window's value i that are still there
                 const int at = win * kValueBins + i;
                 return at < old_cut ? sh.count[i] : at == old_cut ? min(old_need, sh.count[i]) : 0u;
             };
-            for (int e = 0; e < kEach; ++e) {
-                const uint32_t c = counted(tid * kEach + e);
-                own_c += c;
-                own_m += c ? c * sh.weight[tid * kEach + e] : 0;
+            uint32_t own_c = 0;
+            uint64_t own_m = 0;
+            for (int i = warp * kShare + lane; i < (warp + 1) * kShare; i += 32) {
+                const uint32_t n = counted(i);
+                own_c += n;
+                own_m += n ? n * sh.weight[i] : 0;
             }
-            uint32_t c = own_c;
-            uint64_t ms = warp_scan_u64(own_m, lane);
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xffffffffu, c, o);
-                if (lane >= o) c += y;
-            }
-            if (lane == 31) sh.warp_u64[warp] = ms, sh.warp_u32[warp] = c;
+            own_c = __reduce_add_sync(0xffffffffu, own_c);
+            own_m = warp_add_u64(own_m);
             __syncthreads();
-            c += run_c - own_c;
-            ms += run_m - own_m;
+            if (lane == 0) sh.warp_u64[warp] = own_m, sh.warp_u32[warp] = own_c;
+            __syncthreads();
+            // the last warp with an entry that begins below the limit holds the prefix's last value
+            int holder = -1;
+            uint32_t c = 0;
+            uint64_t ms = 0;
             for (int w = 0; w < kValueWarps; ++w) {
-                if (w < warp) c += sh.warp_u32[w], ms += sh.warp_u64[w];
+                if (sh.warp_u32[w] > 0 && (by_mass ? run_m < target : run_c < entries)) holder = w, c = run_c, ms = run_m;
                 run_c += sh.warp_u32[w], run_m += sh.warp_u64[w];
             }
-            int last = -1;
-            for (int e = 0; e < kEach; ++e) {
-                const int i = tid * kEach + e;
-                const uint32_t n = counted(i);
-                if (n > 0 && (by_mass ? ms < target : c < entries)) last = win * kValueBins + i;
-                c += n;
-                ms += n ? n * sh.weight[i] : 0;
-            }
-            last = __reduce_max_sync(0xffffffffu, last);
-            if (lane == 0 && last >= 0) atomicMax(&sh.cut, last);
-            __syncthreads();
-            // the thread that holds the window's last such value says how many of its entries are kept, and the mass
-            const int i = sh.cut - win * kValueBins;
-            if (i >= 0 && i / kEach == tid) {
-                for (int e = kEach - 1; e >= i % kEach; --e) {
-                    const uint32_t n = counted(tid * kEach + e);
-                    c -= n;
-                    ms -= n ? n * sh.weight[tid * kEach + e] : 0;
+            if (warp == holder) {
+                for (int i0 = warp * kShare; i0 < (warp + 1) * kShare; i0 += 32) {
+                    const int i = i0 + lane;
+                    const uint32_t n = counted(i);
+                    const uint64_t w = sh.weight[i], all = n ? n * w : 0, upto = warp_scan_u64(all, lane);
+                    uint32_t upto_c = n;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const uint32_t y = __shfl_up_sync(0xffffffffu, upto_c, o);
+                        if (lane >= o) upto_c += y;
+                    }
+                    const uint64_t begin = ms + upto - all;
+                    const uint32_t begin_c = c + upto_c - n;
+                    const bool below = n > 0 && (by_mass ? begin < target : begin_c < entries);
+                    const uint32_t vote = __ballot_sync(0xffffffffu, below);
+                    if (vote && lane == 31 - __clz(vote)) {
+                        const uint64_t most = by_mass ? (w ? (target - begin + w - 1) / w : n) : entries - begin_c;
+                        sh.cut = win * kValueBins + i;
+                        sh.need = uint32_t(most < n ? most : n);
+                        sh.mass = begin + sh.need * w;
+                    }
+                    __syncwarp();
+                    c += __shfl_sync(0xffffffffu, upto_c, 31);
+                    ms += __shfl_sync(0xffffffffu, upto, 31);
                 }
-                const uint32_t n = counted(i);
-                const uint64_t w = sh.weight[i];
-                const uint64_t most = by_mass ? (w ? (target - ms + w - 1) / w : n) : entries - c;
-                sh.need = uint32_t(most < n ? most : n);
-                sh.mass = ms + sh.need * w;
             }
-            __syncthreads();
             // behind a window that the prefix ends in, nothing is kept
             if (by_mass ? run_m >= target : run_c >= entries) break;
         }
+        __syncthreads();
     };
     __syncthreads();
     if (tid == 0) sh.cut = 0x7fffffff, sh.need = 0xffffffffu;
@@ -843,9 +872,9 @@ __global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const S
         for (int win = 0; win < windows; ++win) {
             if (win * kValueBins > cut) break;
             build(win);
-            auto add = [&](int, uint32_t key) {
-                const int at = place_of(key), i = at - win * kValueBins;
-                if (!key || i < 0 || i >= kValueBins || at > cut) return;
+            auto add = [&](int, uint32_t b) {
+                const int at = place_of_raw(b), i = at - win * kValueBins;
+                if (uint32_t(i) >= uint32_t(kValueBins) || at > cut) return;
                 if (at == cut) {
                     ++ties;
                 } else {
@@ -854,9 +883,9 @@ __global__ void __launch_bounds__(kValueThreads, 2) sample_values_kernel(const S
                 }
             };
             if (vector) {
-                each(add);
+                one_by_one(add);
             } else {
-                for (int i = first + lane; i < last; i += 32) add(i, ordered_bits_16(src[i]));
+                for (int i = first + lane; i < last; i += 32) add(i, uint32_t(src[i]));
             }
         }
         mass = warp_add_u64(mass);
