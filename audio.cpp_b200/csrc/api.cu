@@ -1588,6 +1588,9 @@ b2d_status b2d_kv_check(const b2d_kv_cache* cache, const b2d_kv_batch* batch, in
     } catch (const Fail& e) {
         if (err && err_len) std::snprintf(err, err_len, "%s", e.msg.c_str());
         return e.code;
+    } catch (const std::exception& e) {
+        if (err && err_len) std::snprintf(err, err_len, "%s", e.what());
+        return B2D_EINVAL;
     }
 }
 

@@ -665,11 +665,15 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a, int
     __shared__ int64_t red[16];
     __shared__ float sm_x[8][HD];
     __shared__ float2 sm_ml[8];
+    pdl_trigger();  // the tensor-tile kernel, if there is one, has other sequences
     const int seq = blockIdx.x / (row_tiles * a.kv.kv_heads), unit = blockIdx.x % (row_tiles * a.kv.kv_heads);
     const UnitSpan u = unit_span<ROWS>(a, seq, false);
     const int rt = unit / a.kv.kv_heads, head = unit % a.kv.kv_heads;
     const int r = blockIdx.y, row = rt * ROWS + r;
-    if (rt >= u.row_tiles || row >= u.s.n * a.group) return;
+    if (rt >= u.row_tiles || row >= u.s.n * a.group) {
+        if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();  // the grid is not done before the runs are
+        return;
+    }
     CT* out = static_cast<CT*>(a.o) + int64_t(u.s.first + row / a.group) * a.o_row +
               int64_t(head * a.group + row % a.group) * HD;
     int64_t total, first;

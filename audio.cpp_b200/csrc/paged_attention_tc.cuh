@@ -12,7 +12,7 @@
 //   one warp a tile issues, per half, O += P V of two halves before and S = Q K^T (P from TMEM; K K-major, V MN-major
 //     in shared memory).  The tensor pipe runs them in order, so S may overwrite that P; the half in between is the
 //     softmax's meanwhile.  (With one 128-key S a tile the softmax waited for its own products: 2.6 us a block in
-//     place of SUBBLOCK_US, although N = 64 reads Q from shared memory twice as often.)
+//     place of 2.3, and 2.0 with exponentials on two pipes, although N = 64 reads Q from shared memory twice as often.)
 //   16-bit caches: one warp loads K / V pages with TMA, one box per page and 64-dim panel (128-byte swizzle).
 //   8-bit caches: three pairs of warps read the codes and write them as fp16 in the same layout.  fp16 queries: the codes
 //     stay exact and scales are applied as in paged_stream_kernel: y = s + log2 vs is the logarithm of t = p vs, m
@@ -135,10 +135,15 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     PairPlace at;
-    if (!find_pair(a, int(blockIdx.x), at, blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && warp == 0)) return;
+    const bool first_cta = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
+    if (!find_pair(a, int(blockIdx.x), at, first_cta && warp == 0)) {
+        if (first_cta) pdl_wait();  // as at the end
+        return;
+    }
     const int head = int(blockIdx.y), split = int(blockIdx.z);
     const int seq_rows = at.s.n * a.group;
     const int p_base = at.s.context - at.s.n;  // position of the sequence's first new token
+    const int seen = a.window > 0 ? max(0, p_base - a.window + 1) : 0;  // no row of the sequence sees a key before this one
 
     // halves (64 keys) that each tile sees, cut to this split's share of the pair's blocks jb .. je - 1
     int lo[2], hi[2];
@@ -351,7 +356,10 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                     y0 = kApart ? add_x2(y0, base2) : fma_x2(y0, f2, base2);
                     y1 = kApart ? add_x2(y1, base2) : fma_x2(y1, f2, base2);
                     y0.x = ex2_approx(y0.x), y0.y = ex2_approx(y0.y);
-                    y1.x = ex2_approx(y1.x), y1.y = ex2_approx(y1.y);
+                    // A quarter of them off MUFU: 145 -> 131 us for 2047 + 1098 rows of 12 / 2 heads over 8191 keys.  Not with
+                    // 8-bit caches, whose code warps want the issue slots (2.35 -> 2.54 ms for four int8 prompts).
+                    if (kWide && (e & 4)) y1 = ex2_fma_x2(y1);
+                    else y1.x = ex2_approx(y1.x), y1.y = ex2_approx(y1.y);
                     if constexpr (kApart) {
                         const float4 i4 = *reinterpret_cast<const float4*>(sc + 128 + h * 64 + c * 32 + e);
                         sum[0] = fma_x2(y0, make_float2(i4.x, i4.y), sum[0]);
@@ -468,13 +476,14 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         // ------------------------------------------------------------------------------------ pages by TMA
         const int per_page = 1 << a.kv.page_shift, boxes = 128 >> a.kv.page_shift;  // pages of a block
         bool ok = true;
+        uint32_t patched = 0;  // phase of v_tail
         for (int j = jb; ok && j < je; ++j) {
             const int i = j - jb, s = i % kPtStages;
             const uint32_t ph = uint32_t(i / kPtStages) & 1u;
-            // lane b < boxes: its page; outside the context or the pool one that TMA fills with zeros
+            // lane b < boxes: its page; where no row sees a key of it, or outside the pool, one that TMA fills with zeros
             int page = int(a.kv.pages);
             const int pos = (j << 7) + lane * per_page;
-            if (lane < boxes && pos < at.s.context) {
+            if (lane < boxes && pos < at.s.context && pos + per_page > seen) {
                 page = __ldg(table + (pos >> a.kv.page_shift));
                 if (page < 0 || page >= a.kv.pages) {
                     batch_error(a.b);
@@ -490,11 +499,11 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                     tma_load_4d(smem + Sh::kK + s * Sh::kTile + d * Sh::kPanel + lane * per_page * 128, &tmK, &k_full[s],
                                 d * 64, 0, head, page);
             if (!(ok = warp_wait(&v_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
-            // the block that holds the context's end: rows behind it are zeroed before they are announced (they may hold
-            // anything, and P = 0 times NaN is NaN)
-            const int used = at.s.context - (j << 7);
-            const bool tail = used < 128 && (used & (per_page - 1)) != 0;
-            uint64_t* bar = tail ? v_tail : &v_full[s];
+            // a page that holds the context's end, or the first key that a row sees: its rows outside are zeroed before
+            // they are announced (they may hold anything, and P = 0 times NaN is NaN)
+            const int used = at.s.context - (j << 7), hidden = seen - (j << 7);
+            const bool tail = used < 128 && (used & (per_page - 1)) != 0, front = hidden > 0 && (hidden & (per_page - 1)) != 0;
+            uint64_t* bar = tail || front ? v_tail : &v_full[s];
             if (lane == 0) mbar_arrive_expect_tx(bar, Sh::kTile);
             __syncwarp();
             if (lane < boxes)
@@ -502,14 +511,18 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 for (int d = 0; d < HD / 64; ++d)
                     tma_load_4d(smem + Sh::kV + s * Sh::kTile + d * Sh::kPanel + lane * per_page * 128, &tmV, bar, d * 64, 0,
                                 head, page);
-            if (tail) {  // the last block of the range: v_tail is used once
-                if (!(ok = warp_wait(v_tail, 0u, abort_flag, a.b.status, kErrTimeoutProducer))) break;
-                const int end = (used + per_page - 1) & ~(per_page - 1);
-                for (int b = used * 8 + lane; b < end * 8; b += 32)
+            if (tail || front) {  // at most two blocks of the range
+                if (!(ok = warp_wait(v_tail, patched, abort_flag, a.b.status, kErrTimeoutProducer))) break;
+                patched ^= 1u;
+                auto clear = [&](int from, int to) {  // rows of the block: 8 pieces of a panel each
+                    for (int b = from * 8 + lane; b < to * 8; b += 32)
 #pragma unroll
-                    for (int d = 0; d < HD / 64; ++d)
-                        *reinterpret_cast<uint4*>(smem + Sh::kV + s * Sh::kTile + d * Sh::kPanel + b * 16) =
-                            make_uint4(0u, 0u, 0u, 0u);
+                        for (int d = 0; d < HD / 64; ++d)
+                            *reinterpret_cast<uint4*>(smem + Sh::kV + s * Sh::kTile + d * Sh::kPanel + b * 16) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                };
+                if (front) clear(hidden & ~(per_page - 1), hidden);
+                if (tail) clear(used, (used + per_page - 1) & ~(per_page - 1));
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[s]);
@@ -526,16 +539,17 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         const int units = 4 * (je - jb);
         const int page_mask = (1 << a.kv.page_shift) - 1;
         // Row r of the warp: key unit_key + r.  Lane g (mod 2) holds the page of the 16 rows g (pages are multiples of
-        // 16 rows), -1 behind the context.
+        // 16 rows), -1 where no row of the sequence sees a key.
         auto unit_key = [&](int n) { return ((jb + (n >> 2)) << 7) + ((n & 1) << 6) + (sub << 5); };
         auto load_page = [&](int n) -> int {
             const int pos = unit_key(n) + ((lane & 1) << 4);
-            return n < units && pos < at.s.context ? __ldg(table + (pos >> a.kv.page_shift)) : -1;
+            return n < units && pos < at.s.context && pos + 15 >= seen ? __ldg(table + (pos >> a.kv.page_shift)) : -1;
         };
-        // An out-of-range page becomes -1; reported when it lies inside the context.
+        // An out-of-range page becomes -1; reported when a row may see it.
         auto check_page = [&](int n, int pg) -> int {
             if (pg >= 0 && pg < a.kv.pages) return pg;
-            if (n < units && unit_key(n) + ((lane & 1) << 4) < at.s.context) batch_error(a.b);
+            const int pos = unit_key(n) + ((lane & 1) << 4);
+            if (n < units && pos < at.s.context && pos + 15 >= seen) batch_error(a.b);
             return -1;
         };
         uint4 w[kPieces];
@@ -569,10 +583,10 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         for (; ok && n < units; n += Sh::kCodePairs) {
             const int i = n >> 2, s = i % kPtStages, slot = i % kPtScaleSlots, group = 2 * (n & 1) + sub;
             const bool is_v = (n & 2) != 0;
-            const int used = at.s.context - unit_key(n);  // rows from here on are behind the context
+            const int used = at.s.context - unit_key(n), hidden = seen - unit_key(n);  // rows hidden .. used - 1 are seen
             const uint32_t ph = uint32_t(i / kPtStages) & 1u;
             // a row without a page: zero codes; its probability is 0 or its block reported
-            const bool there = __shfl_sync(0xffffffffu, pg, lane >> 4) >= 0 && lane < used;
+            const bool there = __shfl_sync(0xffffffffu, pg, lane >> 4) >= 0 && lane < used && lane >= hidden;
             int e_k = 0, e_v = 0;
             uint32_t parts = 0;
             if constexpr (kFold) {
@@ -590,7 +604,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
 #pragma unroll
             for (int e = 0; e < kPieces; ++e) {
                 const int row = row0 + e * kRowStep;
-                const bool zero = __shfl_sync(0xffffffffu, pg, row >> 4) < 0 || row >= used;
+                const bool zero = __shfl_sync(0xffffffffu, pg, row >> 4) < 0 || row >= used || row < hidden;
                 const uint4 c4 = zero ? make_uint4(0u, 0u, 0u, 0u) : w[e];
                 uint32_t h[8];
                 codes_to_f16<POOL>(c4.x, h[0], h[1]);
@@ -647,6 +661,8 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+    // Launched while the stream kernel's join, which has other sequences, may still run: done only when that is.
+    if (first_cta && threadIdx.x == 0) pdl_wait();
 }
 
 // Joins the splits of the tensor-tile kernel: one warp per packed row.

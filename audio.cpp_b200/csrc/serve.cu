@@ -290,8 +290,14 @@ void launch_tc(const AttentionLaunch& x) {
         ta.part_o = static_cast<float*>(x.tc_workspace);
         ta.part_ml = reinterpret_cast<float2*>(ta.part_o + slots * HD);
     }
-    launch_k(kernel, dim3(unsigned(x.tc.pairs), kvh, unsigned(x.tc.splits)), dim3(Sh::kThreads), Sh::kSmem, x.st, 1, tk, tv,
-             ta);
+    {
+        // behind the stream kernel and its join, which have other sequences: beside them (the kernel ends after them)
+        const bool outer = tl_pdl;
+        tl_pdl = x.row_tiles > 0;
+        launch_k(kernel, dim3(unsigned(x.tc.pairs), kvh, unsigned(x.tc.splits)), dim3(Sh::kThreads), Sh::kSmem, x.st, 1, tk,
+                 tv, ta);
+        tl_pdl = outer;
+    }
     if (x.tc.splits > 1)
         launch_k(paged_join_kernel<CT, HD>, dim3(unsigned(x.tc.pairs), kvh, 32u), dim3(256), 0, x.st, 1, ta);
 }
@@ -347,6 +353,7 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
     const int kind = pool_kind(cache->type);
     if ((kind == kPoolF16 && bf16) || (kind == kPoolBf16 && !bf16))
         fail(B2D_EINVAL, "a 16-bit paged cache must have the queries' type");
+    if (int64_t(a.b.rows) * heads > kMaxVectors) fail(B2D_EINVAL, "paged attention batch is too large");
     if (a.b.rows == 0 || a.b.seqs == 0 || a.b.max_new == 0) return;
     if (!q || !o || misaligned(q, 16) || misaligned(o, 16) || q_row % 8 || o_row % 8)
         fail(B2D_EINVAL, "paged attention rows must be 16-byte aligned device memory");
@@ -361,7 +368,7 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
     a.q_row = q_row;
     a.o_row = o_row;
     a.heads = heads;
-    a.window = window;
+    a.window = window < a.b.max_context ? window : 0;  // one that holds every context hides nothing
     a.scale_log2 = scale * 1.4426950408889634f;
     a.min_rows = stream_most_rows(a.kv.head_dim);
     x.cache = cache;

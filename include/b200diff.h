@@ -486,8 +486,9 @@ B2D_API size_t b2d_paged_attention_workspace(b2d_ctx* ctx, const b2d_kv_cache* c
  * scale is positive and finite.
  * q, o: [rows, heads, head_dim] fp16 (bf16 = 0) or bf16 (bf16 = 1), row strides q_row / o_row in elements, 16-byte
  * aligned; a 16-bit cache has the queries' type.  heads is 1 to 128 times kv_heads.  A row that sees no key gives
- * zeros.  Keys and values at the positions of a context that a new row may see must be finite (what lies behind a
- * context, in its last page, may be anything).  Scores, softmax sums and the output's sums are fp32; probabilities
+ * zeros.  Keys and values at the positions that a new row of the sequence sees must be finite; what lies behind the
+ * context in its last page, or before the window of the sequence's first new row, may be anything, and pages that hold
+ * nothing else need no valid table entry.  Scores, softmax sums and the output's sums are fp32; probabilities
  * enter the second product rounded to the queries' type, or, times the value's scale, to fp16 for an 8-bit cache (bf16
  * queries: the cache's values may be rounded to fp16 as well).  The same batch gives the same bits whenever it runs.
  * workspace: 16-byte aligned, contents neither read nor kept; calls that may overlap (two streams, two graphs) need
@@ -519,9 +520,10 @@ B2D_API b2d_status b2d_vvlm_forward_paged(b2d_ctx* ctx, const b2d_kv_cache* cach
  *   top_k > 0 keeps the first top_k; top_p < 1 keeps an entry while the mass before it is below top_p times the mass
  *   top-k left (the best entry always stays); min_p > 0 keeps those with w_i >= min(min_p, 1);
  *   the token is the first index whose running sum of kept weights, in index order, exceeds uniform times their sum.
- * temperature <= 0 takes the best entry.  A NaN logit counts as -infinity, +infinity as certain; a row without an
+ * temperature <= 0 (or NaN) takes the best entry.  A NaN logit counts as -infinity, +infinity as certain; a row without an
  * entry above -infinity gives token -1.  Weights are computed in fp64 to within 2^-44 of the largest and summed
- * exactly in units of 2^-45 of it (an entry below half a unit is never drawn), so the token depends on nothing but the arguments. */
+ * exactly in units of 2^-45 of it (an entry below half a unit is never drawn), so the token depends on nothing but the
+ * arguments. */
 typedef struct {
     int32_t logits_type;        /* B2D_TYPE_F32, B2D_TYPE_F16 or B2D_TYPE_BF16 */
     int64_t rows, vocab;        /* vocab 1 to 262144 */

@@ -353,6 +353,24 @@ def test_attention(b2d, ctx, case, pool, dtype, kv_heads, group, head_dim, page,
     assert torch.equal(out, attend(ctx, s, q, window))  # the same bits again
 
 
+@pytest.mark.parametrize("pool", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("new,context,window", [
+    (1, 1, 0), (2, 3000, 0), (33, 33, 0), (300, 20, 0), (300, 0, 0), (129, 4000, 0), (64, 4001, 130), (500, 700, 2 ** 31 - 1),
+    (300, 20, 2 ** 31 - 1), (1000, 1000, 1)])
+def test_attention_one_sequence(b2d, ctx, pool, new, context, window):
+    """One sequence, whose keys are spread over many CTAs; also when its rows turn out fewer than the bounds allow."""
+    s = Setup(b2d, [new], [context], 2, 128, 32, pool, gap=1)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q = (2 * torch.randn(s.rows, 14, 128, generator=g, device=DEV)).bfloat16()
+    check_attention(s, q, attend(ctx, s, q, window), window)
+    if new > 2:  # the same bounds, two rows
+        s.row_start[1] = s.start[0] + 2
+        s.start[1] = s.start[0] + 2
+        out = attend(ctx, s, q, window)
+        check_attention(s, q, out, window)
+    ctx.sync(stream())
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_attention_growing_and_extreme_scores(b2d, ctx, dtype):
     """Scores that keep rising along the context (the running maximum moves at every step), a large scale that makes
@@ -397,6 +415,53 @@ def test_attention_reads_no_stale_slots(b2d, ctx):
                 t[~used] = float("inf")
         assert torch.equal(first, attend(ctx, s, q))
         ctx.sync(stream())
+
+
+@pytest.mark.parametrize("pool", ["f16", "bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("head_dim,page,window", [(128, 32, 70), (64, 128, 33), (128, 128, 5), (128, 16, 256), (32, 64, 40)])
+def test_attention_reads_nothing_before_the_window(b2d, ctx, pool, dtype, head_dim, page, window):
+    """Slots before the window of a sequence's first new row are NaN or garbage, and pages that hold nothing else were
+    given back: their table entries are -7."""
+    if pool in WIDE and pool != dtype:
+        pytest.skip("a 16-bit cache has the queries' type")
+    new, context = [1, 9, 50, 300, 513], [533, 477, 350, 1029, 5000]
+    s = Setup(b2d, new, context, 2, head_dim, page, pool)
+    q = torch.randn(s.rows, 14, head_dim, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).to(WIDE[dtype])
+    first = attend(ctx, s, q, window)
+    check_attention(s, q, first, window)
+    for i, (n, c) in enumerate(zip(new, context)):
+        lo = max(0, c - n - window + 1)
+        pos = torch.arange(lo, device=DEV)
+        at = s.table[i, pos // page].long()
+        for t in (s.k, s.v):
+            bits = torch.full_like(t[at, :, pos % page], float("nan")) if pool in WIDE else None
+            if bits is None:
+                t.view(torch.uint8)[at, :, pos % page] = 0x7f if pool == "e4m3" else 0x80
+            else:
+                t[at, :, pos % page] = bits
+        for t in (s.ks, s.vs):
+            if t is not None:
+                t[at, :, pos % page] = float("nan")
+        s.table[i, :lo // page] = -7
+    assert torch.equal(first, attend(ctx, s, q, window))
+    ctx.sync(stream())
+
+
+@pytest.mark.parametrize("pool", ["bf16", "int8"])
+def test_attention_queries_that_are_not_finite(b2d, ctx, pool):
+    """A NaN or an infinity in a query makes that row's head NaN and no other."""
+    s = Setup(b2d, [1, 9, 300], [533, 477, 1029], 2, 128, 32, pool)
+    q = torch.randn(s.rows, 14, 128, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV).bfloat16()
+    first = attend(ctx, s, q)
+    bad = torch.zeros(s.rows, 14, dtype=torch.bool, device=DEV)
+    for n, (row, head, x) in enumerate([(0, 3, "nan"), (5, 0, "inf"), (40, 13, "nan"), (200, 7, "-inf"), (309, 2, "nan")]):
+        q[row, head, 11 * n] = float(x)
+        bad[row, head] = True
+    out = attend(ctx, s, q)
+    assert torch.isnan(out[bad]).all()
+    assert torch.equal(out[~bad], first[~bad])
+    ctx.sync(stream())
 
 
 def test_bad_indexes_are_reported_and_not_followed(b2d, ctx):
@@ -453,6 +518,9 @@ def test_refusals(b2d, ctx):
     for wrong in (q.float(), q[:, :3], q[..., :32], q[:1], q.cpu()):
         with pytest.raises(b2d.B2DError):
             ctx.paged_attention(wrong, s.cache, s.batch, torch.empty_like(wrong), workspace=work)
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(b2d.B2DError, match="scale"):
+            ctx.paged_attention(q, s.cache, s.batch, torch.empty_like(q), scale=scale, workspace=work)
     rows = torch.zeros(2, 2, 64, device=DEV)
     for wrong in (rows.double(), rows[:1], rows[..., :32], rows[:, :1], rows.cpu(), rows.transpose(0, 1)):
         with pytest.raises(b2d.B2DError):
