@@ -6,12 +6,14 @@
 // running sum over kept entries passes u Z.
 //
 // A row is read from HBM once: a cluster of up to 8 CTAs holds it in shared memory as ordered bits, four to a load, and
-// every later pass compares integers there.  A cut is found by counting entries in 2048 bins (linear in the logit, later linear in the ordered
-// bits).  For a cut by mass, a bin's mass lies between its count times the weights at its two edges, which brackets the
-// crossing to a few bins; the masses above the bracket and of its upper half are then summed exactly, which decides
-// for a half, and that is counted again until it holds few enough entries to sort them.  The
-// undecided range of ordered bits at least halves every round, so there are at most 34.  (Summing masses into the bins
-// took three more shared atomics an entry.)
+// every later pass compares integers there.  A cut is found by counting entries in 2048 bins (linear in the logit, later
+// linear in the ordered bits).  For a cut by mass, a bin's mass lies between its count times the weights at its two edges,
+// which brackets the crossing to a few bins; the masses above the bracket and of its upper half are then summed exactly,
+// which decides for a half, and that is counted again until it holds few enough entries to sort them.  The undecided
+// range of ordered bits at least halves every round, so there are at most 34.  (Summing masses into the bins took three
+// more shared atomics an entry.)
+// One row of 32003 fp32 entries takes 17 us, its cluster's barriers and rounds one after the other; 64 x 128256 of mixed
+// requests 93 us (0.4 TB/s): the passes that weigh entries in fp64, two CTAs an SM.
 // Which token comes out depends on sums of up to 2^18 terms and on comparisons next to a border, so the weights are
 // computed in fp64 and added as integers (units of 2^-45 of the largest weight): sums of integers do not depend on
 // the order of threads, warps or CTAs, so neither does the token.

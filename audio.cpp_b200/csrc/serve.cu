@@ -70,7 +70,7 @@ KvView cache_view(const b2d_kv_cache* c) {
 BatchView batch_view(const b2d_kv_batch* b, const b2d_kv_cache* c, int* status) {
     if (!b) fail(B2D_EINVAL, "paged cache batch is missing");
     if (b->seqs < 0 || b->seqs > kMaxSeqs) fail(B2D_EINVAL, "paged cache batch of %d sequences (0 to %d)", b->seqs, kMaxSeqs);
-    if (b->rows < 0 || b->rows * c->kv_heads > kMaxVectors || b->max_new < 0 || b->max_context < 0)
+    if (b->rows < 0 || b->rows > kMaxVectors / c->kv_heads || b->max_new < 0 || b->max_context < 0)
         fail(B2D_EINVAL, "paged cache batch sizes are negative or too large");
     if (b->seqs > 0 && (!b->row_start || !b->context || !b->page_table))
         fail(B2D_EINVAL, "paged cache batch needs row_start, context and page_table");
@@ -362,7 +362,7 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
     const size_t need = attention_bytes(a.b, a.kv, a.group, dev.num_sms);
     if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
         fail(B2D_EINVAL, "paged attention needs a 16-byte aligned workspace of %zu bytes", need);
-    if (!(scale > 0.f) || !std::isfinite(scale)) fail(B2D_EINVAL, "paged attention scale must be positive and finite");
+    if (!(scale > 0.f) || !std::isfinite(2.f * scale)) fail(B2D_EINVAL, "paged attention scale must be positive and finite");
     a.q = q;
     a.o = o;
     a.q_row = q_row;

@@ -518,7 +518,7 @@ def test_refusals(b2d, ctx):
     for wrong in (q.float(), q[:, :3], q[..., :32], q[:1], q.cpu()):
         with pytest.raises(b2d.B2DError):
             ctx.paged_attention(wrong, s.cache, s.batch, torch.empty_like(wrong), workspace=work)
-    for scale in (0.0, -1.0, float("nan"), float("inf")):
+    for scale in (0.0, -1.0, 2.0 ** 127, float("nan"), float("inf")):
         with pytest.raises(b2d.B2DError, match="scale"):
             ctx.paged_attention(q, s.cache, s.batch, torch.empty_like(q), scale=scale, workspace=work)
     rows = torch.zeros(2, 2, 64, device=DEV)
@@ -635,6 +635,21 @@ def test_sampling_largest_vocabulary_and_strides(b2d, ctx):
     wide = torch.tensor(rng.standard_normal((3, 262144 + 7)), dtype=torch.float32, device=DEV)
     sample(ctx, wide[:, 3:262144 + 3], 1.0, k=[0, 2000, 0], p=[1.0, 1.0, 0.97], u=rng.random(3))
     sample(ctx, wide[:, 1:1000].bfloat16()[:, 1:], 1.0, p=0.5, u=rng.random(3))
+
+
+def test_sampling_does_not_depend_on_the_batch(b2d, ctx):
+    """A row gives the same token and the same probability, bit for bit, alone, among few rows and among many."""
+    rng = np.random.default_rng(11)
+    x = torch.tensor(rng.standard_normal((40, 50021)) * 4, device=DEV).bfloat16()
+    t = rng.uniform(0.5, 2.0, 40).astype(np.float32)
+    k, p = rng.integers(0, 400, 40), rng.uniform(0.2, 1.1, 40).astype(np.float32)
+    u = rng.random(40).astype(np.float32)
+    many = sample(ctx, x, t, k=k, p=p, u=u)
+    for part in (slice(0, 1), slice(3, 10), slice(17, 40)):
+        few = sample(ctx, x[part], t[part], k=k[part], p=p[part], u=u[part])
+        assert torch.equal(few[0], many[0][part]) and torch.equal(few[1], many[1][part])
+        wide = sample(ctx, x[part].float(), t[part], k=k[part], p=p[part], u=u[part])
+        assert torch.equal(wide[0], many[0][part]) and torch.equal(wide[1], many[1][part])
 
 
 @pytest.mark.parametrize("vocab", [1, 7, 300, 4099, 70001, 262144])

@@ -47,7 +47,7 @@ def test_eight_bit_cache_needs_scales(b2d):
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(seqs=-1), "sequences"), (dict(seqs=8193), "sequences"), (dict(rows=-1), "sizes"), (dict(rows=1 << 31), "sizes"),
+    (dict(seqs=-1), "sequences"), (dict(seqs=8193), "sequences"), (dict(rows=-1), "sizes"), (dict(rows=1 << 31), "sizes"), (dict(rows=1 << 62), "sizes"),
     (dict(max_new=-1), "sizes"), (dict(max_context=-1), "sizes"), (dict(max_context=49), "max_context"),
     (dict(table_stride=2), "max_context"), (dict(context=None), "needs row_start"), (dict(page_table=None), "needs row_start"),
 ])
