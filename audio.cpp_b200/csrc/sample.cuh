@@ -11,9 +11,12 @@
 // which brackets the crossing to a few bins; the masses above the bracket and of its upper half are then summed exactly,
 // which decides for a half, and that is counted again until it holds few enough entries to sort them.  The undecided
 // range of ordered bits at least halves every round, so there are at most 34.  (Summing masses into the bins took three
-// more shared atomics an entry.)
-// One row of 32003 fp32 entries takes 17 us, its cluster's barriers and rounds one after the other; 64 x 128256 of mixed
-// requests 93 us (0.4 TB/s): the passes that weigh entries in fp64, two CTAs an SM.
+// more shared atomics an entry.)  When all entries down to the first cut fit in the list (any top-k up to some 500, a
+// small nucleus), one CTA finishes the row there: the later cuts, the sums and the draw (a row with top-k and top-p 105k
+// -> 48k clocks).
+// One row of 32003 fp32 entries takes 15 us, its cluster's barriers and passes one after the other; 64 x 128256 of mixed
+// requests 91 us (0.4 TB/s): the passes that weigh entries in fp64, 33k clocks of the 120k that a row with top-p alone
+// takes, and its second round.
 // Which token comes out depends on sums of up to 2^18 terms and on comparisons next to a border, so the weights are
 // computed in fp64 and added as integers (units of 2^-45 of the largest weight): sums of integers do not depend on
 // the order of threads, warps or CTAs, so neither does the token.
@@ -194,11 +197,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const float m = from_ordered(best_key);
     const double inv_t = 1.0 / double(temp), scale = inv_t * 92.33248261689366;  // 64 log2 e / T
     const float deepest = m - 31.93f * temp;  // weights below it are under half a unit
-    auto weight = [&](uint32_t key) -> uint64_t {
-        if (key == best_key) return uint64_t(kSampleUnit);
+    auto weight = [&](uint32_t key) -> uint64_t {  // without branches, so that a lane's entries go side by side
         const float v = from_ordered(key);
-        if (!(v >= deepest)) return 0;
-        return exp_units((double(v) - double(m)) * scale, sh.power);
+        const bool most = key == best_key, some = v >= deepest;  // bits 0 are a NaN here
+        const uint64_t w = exp_units(some && !most ? (double(v) - double(m)) * scale : 0.0, sh.power);
+        return most || some ? w : 0;
     };
 
     uint64_t cut = 0;  // entries at or above it (as (ordered bits, ~index)) are kept
@@ -231,9 +234,46 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     };
     bool summed = false;  // warp_u64 and total already hold the kept mass
 
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.f, floor_p = a.min_p ? a.min_p[row] : 0.f;
+    const uint64_t least_kept = floor_p > 0.f ? uint64_t(ceil(double(fminf(floor_p, 1.f)) * kSampleUnit)) : 0;
+    auto mass_goal = [](float part, uint64_t z) -> uint64_t {  // top-p keeps entries while the mass before them is below it
+        const uint64_t t = part > 0.f ? uint64_t(ceil(double(part) * double(z))) : 1u;
+        return t ? t : 1;
+    };
+    auto draw_goal = [&](uint64_t z) -> uint64_t {  // the token is the first whose running sum is above it
+        float u = a.uniform[row];
+        u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+        const uint64_t goal = uint64_t(double(u) * double(z));
+        return goal >= z ? z - 1 : goal;
+    };
+
     // Lowers `cut` to the last entry of the prefix that holds `want` entries (by_mass false), or of which the mass
-    // before it is below `part` of the mass kept so far (by_mass true).
-    auto find_cut = [&](bool by_mass, uint32_t want, float part, bool sum_up) {
+    // before it is below `part` of the mass kept so far (by_mass true).  Where all entries down to the cut fit in the
+    // list, rank 0 finishes the row from there, and true is returned.
+    auto find_cut = [&](bool by_mass, uint32_t want, float part, bool sum_up) -> bool {
+        // Rank 0's list in order (bitonic, an entry a thread; pairs within a warp by shuffles).
+        auto sort_list = [&](uint32_t n, uint64_t& e, uint64_t& w) {
+            static_assert(kSampleList == kSampleThreads, "one entry a thread");
+            const bool there = uint32_t(tid) < n;
+            e = there ? sh.list_entry[tid] : 0, w = there ? sh.list_weight[tid] : 0;
+            for (int size = 2; size <= kSampleList; size *= 2) {
+                for (int step = size / 2; step > 0; step /= 2) {
+                    uint64_t oe, ow;
+                    if (step >= 32) {
+                        __syncthreads();
+                        sh.list_entry[tid] = e, sh.list_weight[tid] = w;
+                        __syncthreads();
+                        oe = sh.list_entry[tid ^ step], ow = sh.list_weight[tid ^ step];
+                    } else {
+                        oe = __shfl_xor_sync(0xffffffffu, e, step), ow = __shfl_xor_sync(0xffffffffu, w, step);
+                    }
+                    // descending overall: the lower of a pair of threads keeps the larger in even runs
+                    const bool larger = ((tid & step) == 0) == ((tid & size) == 0);
+                    if ((oe > e) == larger && oe != e) e = oe, w = ow;
+                }
+            }
+        };
         const float span = fminf(16.f * temp, m - from_ordered(low));  // the last bin takes what lies deeper
         const float per_unit = span > 0.f ? float(kSampleBins) / span : 0.f;
         uint32_t key_lo = 1, key_hi = 0xffffffffu;  // what is still undecided
@@ -253,11 +293,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             __syncthreads();
             uint64_t all = 0;
             each([&](int i, uint32_t key) {
-                if (!active(i, key)) return;
-                atomicAdd(&sh.count[bin_of(key)], 1u);
-                if (by_mass && round == 0) all += weight(key);
+                if (active(i, key)) atomicAdd(&sh.count[bin_of(key)], 1u);
             });
-            if (by_mass && round == 0) {
+            if (by_mass && target == 0) {
+                each([&](int i, uint32_t key) { all += kept(i, key) ? weight(key) : 0; });
                 all = warp_add_u64(all);
                 if (lane == 0) sh.warp_u64[warp] = all;
                 __syncthreads();
@@ -267,11 +306,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 }
             }
             cluster.sync();
-            if (by_mass && round == 0) {
+            if (by_mass && target == 0) {
                 uint64_t none;
-                const uint64_t z = over_ranks(none);
-                target = part > 0.f ? uint64_t(ceil(double(part) * double(z))) : 1u;
-                if (target == 0) target = 1;
+                target = mass_goal(part, over_ranks(none));
             }
             if (rank == 0) {
                 // every thread sums four consecutive bins over the ranks, then the bins are scanned in order
@@ -361,6 +398,55 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             const int bin_lo = lead->bin_lo, bin_hi = lead->bin_hi;
             before_count = lead->before_count;
             const uint32_t bracket = lead->bracket - before_count;
+            if (lead->bracket <= uint32_t(kSampleList)) {
+                // ---- all entries down to the cut into rank 0's list (in any order), which finishes the row
+                each([&](int i, uint32_t key) {
+                    if (!kept(i, key) || key < key_lo || (key <= key_hi && bin_of(key) > bin_hi)) return;
+                    const uint32_t at = atomicAdd(&lead->list_fill, 1u);
+                    lead->list_entry[at] = entry_of(i, key);
+                    lead->list_weight[at] = weight(key);
+                });
+                cluster.sync();
+                if (rank != 0) return true;  // nobody reads this CTA's shared memory any more
+                uint64_t e, w;
+                sort_list(sh.bracket, e, w);
+                // what top-k, then top-p leaves, then min-p
+                auto running = [&](uint64_t x, uint64_t& all) -> uint64_t {  // sums up to this thread, over all
+                    const uint64_t upto = warp_scan_u64(x, lane);
+                    __syncthreads();
+                    if (lane == 31) sh.warp_u64[warp] = upto;
+                    __syncthreads();
+                    uint64_t run = upto;
+                    all = 0;
+                    for (int i = 0; i < kSampleWarps; ++i) {
+                        if (i < warp) run += sh.warp_u64[i];
+                        all += sh.warp_u64[i];
+                    }
+                    return run;
+                };
+                uint64_t all_mass;
+                if (!by_mass && uint32_t(tid) >= want) w = 0;
+                const uint64_t upto = running(w, all_mass);
+                if (!by_mass && p < 1.f) target = mass_goal(p, all_mass);
+                if (p < 1.f && upto - w >= target) w = 0;
+                if (w < least_kept) w = 0;
+                uint64_t z;
+                running(w, z);
+                const uint64_t goal = draw_goal(z);
+                sh.list_entry[tid] = e, sh.list_weight[tid] = w;
+                __syncthreads();
+                // the running sum in the order of the indexes: what of the list lies before this entry
+                if (w > 0) {
+                    uint64_t run = 0;
+                    for (uint32_t j = 0; j < sh.bracket; ++j)
+                        run += uint32_t(sh.list_entry[j]) > uint32_t(e) ? sh.list_weight[j] : 0;  // (~index)
+                    if (goal >= run && goal < run + w) {
+                        a.tokens[row] = int(~uint32_t(e));
+                        if (a.probs) a.probs[row] = float(double(w) / double(z));
+                    }
+                }
+                return true;
+            }
             if (bracket <= uint32_t(kSampleList)) {
                 // ---- the mass above the bracket, exactly, and the bracket's entries into rank 0's list (in any order)
                 uint64_t above = 0;
@@ -382,27 +468,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 uint64_t none;
                 before_mass += over_ranks(none);
                 if (rank == 0) {
-                    // the list in order (bitonic, an entry a thread; pairs within a warp by shuffles), then its running
-                    // sums: the last entry whose rank / mass before it still qualifies is the cut
-                    static_assert(kSampleList == kSampleThreads, "one entry a thread");
+                    // the list's running sums in order: the last entry whose rank / mass before it still qualifies is the cut
                     const bool there = uint32_t(tid) < bracket;
-                    uint64_t e = there ? sh.list_entry[tid] : 0, w = there ? sh.list_weight[tid] : 0;
-                    for (int size = 2; size <= kSampleList; size *= 2) {
-                        for (int step = size / 2; step > 0; step /= 2) {
-                            uint64_t oe, ow;
-                            if (step >= 32) {
-                                __syncthreads();
-                                sh.list_entry[tid] = e, sh.list_weight[tid] = w;
-                                __syncthreads();
-                                oe = sh.list_entry[tid ^ step], ow = sh.list_weight[tid ^ step];
-                            } else {
-                                oe = __shfl_xor_sync(0xffffffffu, e, step), ow = __shfl_xor_sync(0xffffffffu, w, step);
-                            }
-                            // descending overall: the lower of a pair of threads keeps the larger in even runs
-                            const bool larger = ((tid & step) == 0) == ((tid & size) == 0);
-                            if ((oe > e) == larger && oe != e) e = oe, w = ow;
-                        }
-                    }
+                    uint64_t e, w;
+                    sort_list(bracket, e, w);
                     const uint64_t upto = warp_scan_u64(w, lane);
                     __syncthreads();
                     if (lane == 31) sh.list_weight[warp] = upto;
@@ -432,7 +501,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                     if (tid == 0) sh.total = sh.warp_u64[kSampleWarps];
                     summed = true;
                 }
-                return;
+                return false;
             }
             // ---- too many for the list.  Exactly: the masses above the bracket and of its upper half, its entries by
             // halves and their ranges
@@ -440,22 +509,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             uint64_t above = 0, upper = 0;
             uint32_t inside[2] = {0, 0}, lo_key[2] = {0xffffffffu, 0xffffffffu}, hi_key[2] = {0, 0};
             each([&](int i, uint32_t key) {
-                if (!active(i, key)) return;
-                const int b = bin_of(key);
-                if (b > bin_hi) return;
-                if (b >= bin_lo) {
-                    if (b > middle) {
-                        ++inside[1];
-                        lo_key[1] = min(lo_key[1], key), hi_key[1] = max(hi_key[1], key);
-                    } else {
-                        ++inside[0];
-                        lo_key[0] = min(lo_key[0], key), hi_key[0] = max(hi_key[0], key);
-                        if (by_mass && bin_hi > bin_lo) upper += weight(key);
-                    }
-                } else if (by_mass) {
-                    above += weight(key);
+                const int b = active(i, key) ? bin_of(key) : kSampleBins;
+                if (b >= bin_lo && b <= middle) {
+                    ++inside[0];
+                    lo_key[0] = min(lo_key[0], key), hi_key[0] = max(hi_key[0], key);
+                } else if (b > middle && b <= bin_hi) {
+                    ++inside[1];
+                    lo_key[1] = min(lo_key[1], key), hi_key[1] = max(hi_key[1], key);
                 }
             });
+            if (by_mass)
+                each([&](int i, uint32_t key) {
+                    const int b = active(i, key) ? bin_of(key) : kSampleBins;
+                    const uint64_t w = b <= middle ? weight(key) : 0;
+                    above += b < bin_lo ? w : 0;
+                    upper += b >= bin_lo && bin_hi > bin_lo ? w : 0;
+                });
             if (by_mass) above = warp_add_u64(above), upper = warp_add_u64(upper);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -507,11 +576,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             }
             if (need >= inside_all) {  // all of them
                 cut = max(cut, uint64_t(key_lo) << 32);
-                return;
+                return false;
             }
             if (need == 0) {
                 cut = (uint64_t(key_hi) + 1) << 32;
-                return;
+                return false;
             }
             // ties in the ranks, then the warps, before this one
             uint32_t mine = 0;
@@ -541,24 +610,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             }
             cluster.sync();
             cut = lead->cut;
-            return;
+            return false;
         }
+        return false;
     };
 
-    const int k = a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.f, floor_p = a.min_p ? a.min_p[row] : 0.f;
     if (k > 0 && k < a.vocab) {
-        find_cut(false, uint32_t(k), 0.f, false);
+        if (find_cut(false, uint32_t(k), 0.f, false)) return;
         cluster.sync();  // the cut has been read by every rank
     }
-    if (p < 1.f) find_cut(true, 0, p, !(floor_p > 0.f));
-    const uint64_t least = floor_p > 0.f ? uint64_t(ceil(double(fminf(floor_p, 1.f)) * kSampleUnit)) : 0;
+    if (p < 1.f && find_cut(true, 0, p, !(floor_p > 0.f))) return;
     if (!summed) {
         uint64_t sum = 0;
         each([&](int i, uint32_t key) {
-            if (!kept(i, key)) return;
             const uint64_t w = weight(key);
-            sum += w >= least ? w : 0;
+            sum += kept(i, key) && w >= least_kept ? w : 0;
         });
         sum = warp_add_u64(sum);
         cluster.sync();  // the totals of the last cut have been read by every rank
@@ -567,17 +633,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     cluster.sync();
     uint64_t before;
     const uint64_t z = over_ranks(before);
-    float u = a.uniform[row];
-    u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
-    uint64_t goal = uint64_t(double(u) * double(z));  // the token is the first whose running sum is above it
-    if (goal >= z) goal = z - 1;
+    const uint64_t goal = draw_goal(z);
     if (goal >= before && goal < before + sh.total) {
         // this CTA's: first the warp whose share holds the goal, then that share is cut among all warps, then one of them
         // looks at its few entries one by one
         auto mass = [&](int i) -> uint64_t {
             if (!kept(i, keys[i])) return 0;
             const uint64_t w = weight(keys[i]);
-            return w >= least ? w : 0;
+            return w >= least_kept ? w : 0;
         };
         int owner = 0;
         while (goal >= before + sh.warp_u64[owner + 1]) ++owner;
