@@ -24,6 +24,9 @@
 // The keys of all units form one list of 64-key tiles, cut into equal runs, one per CTA: ragged batches load every
 // SM alike whatever the lengths.  A run that holds only part of a unit leaves (O, m, l) in the workspace and
 // paged_merge_kernel joins the parts in their order in the list, so results do not depend on timing.
+//
+// 3 sequences of up to 131071 keys, bf16, 28 / 4 heads of 128: 103 us, 6.1 TB/s (94 % of a copy's rate).  64 of up to 8190,
+// int8: 91 us, 3.8 TB/s, bound by issue (half of the slots) and latency: some 490 instructions for 16 keys, three CTAs an SM.
 #pragma once
 
 #include "kv_cache.cuh"

@@ -52,8 +52,8 @@ KvView cache_view(const b2d_kv_cache* c) {
     KvView v{};
     v.k = static_cast<uint8_t*>(c->k);
     v.v = static_cast<uint8_t*>(c->v);
-    v.ks = c->k_scale;
-    v.vs = c->v_scale;
+    v.ks = elem == 1 ? c->k_scale : nullptr;
+    v.vs = elem == 1 ? c->v_scale : nullptr;
     v.page_stride = c->page_stride * elem;
     v.head_stride = c->head_stride * elem;
     v.token_stride = c->token_stride * elem;
@@ -208,9 +208,11 @@ namespace {
 int stream_rows(const BatchView& b, int group) { return int64_t(b.max_new) * group <= 8 ? 8 : 16; }
 
 // Packed rows (tokens x heads per kv head) up to which a sequence goes through the stream kernel.  Its cost grows with
-// every tile of 16 rows that reads the keys again, the tensor-tile kernel's with every pair of 128; head_dim 32 has no
-// tensor-tile kernel.
-int stream_most_rows(int head_dim) { return head_dim == 32 ? 0x7fffffff : 16; }
+// every tile of 16 rows that reads the keys again, the tensor-tile kernel's with every pair of 128; with 8-bit caches that
+// one also waits for its codes, whatever the rows.  64 sequences of up to 3 tokens over up to 8192 keys, 28 / 4 heads of
+// 128 (21 packed rows at most): stream 253 us, tensor tiles 187 with bf16 caches, 207 and 345 with int8; of up to 5 over
+// 2048 (35 rows): 138 and 64, 132 and 106.  head_dim 32 has no tensor-tile kernel.
+int stream_most_rows(const KvView& kv) { return kv.head_dim == 32 ? 0x7fffffff : kv.ks ? 32 : 16; }
 
 int64_t batch_packed_rows(const BatchView& b, int group) { return int64_t(std::min(b.max_new, b.rows)) * group; }
 
@@ -220,7 +222,7 @@ struct TcPlan {
     int pairs, splits;
 };
 TcPlan tc_plan(const BatchView& b, const KvView& kv, int group, int num_sms) {
-    const int most = stream_most_rows(kv.head_dim);
+    const int most = stream_most_rows(kv);
     if (batch_packed_rows(b, group) <= most) return {0, 0};
     const int64_t packed = int64_t(b.rows) * group;
     const int64_t pairs = packed / 256 + std::min<int64_t>(b.seqs, packed / (most + 1) + 1);
@@ -370,7 +372,7 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
     a.heads = heads;
     a.window = window < a.b.max_context ? window : 0;  // one that holds every context hides nothing
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.min_rows = stream_most_rows(a.kv.head_dim);
+    a.min_rows = stream_most_rows(a.kv);
     x.cache = cache;
     x.tc = tc_plan(a.b, a.kv, a.group, dev.num_sms);
     x.tc_workspace = static_cast<uint8_t*>(workspace) + stream_bytes(a.b, a.kv, a.group, dev.num_sms);
@@ -395,8 +397,9 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
 }
 
 // -------------------------------------------------------------------------------------------------- sampling
-// bf16 rows from which a CTA each, counting values, is faster than a cluster each, weighing entries.
-constexpr int64_t kValueRows = 24;
+// bf16 rows from which a CTA each, counting values, is faster than a cluster each, weighing entries: 8 rows of 128256 take
+// 96 and 124 us with top-p, 75 and 53 with top-k; 16 rows 97 and 153, 76 and 72; 64 rows 99 and 356, 77 and 149.
+constexpr int64_t kValueRows = 16;
 
 void sample_tokens(const ServeDevice&, const b2d_sample_request* rq, cudaStream_t st) {
     if (!rq) fail(B2D_EINVAL, "sampling request is missing");
