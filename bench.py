@@ -872,12 +872,16 @@ def bench_ours(args):
                 "whole_call_tflops": round(flops_call / (ms / 1e3) / 1e12, 1),
                 "clocks": clk.summary()}
         if not args.no_cpu_baseline and world == 1:
-            frames = cfg.frames  # the whole 1024-frame call, as the GPU arm runs it
-            cms, variant = run_cpu_reference(cfg, frames, 4, os.cpu_count() or 1)
-            v = frames / (float(np.median(cms[1:])) / 1e3)
-            line["cpu_baseline"] = {"value": round(v, 2), "unit": UNIT, "cores": os.cpu_count(), "kind": "reference",
-                                    "sample": "the full %d-frame call, 10 DPM steps + CFG, audio.cpp ggml CPU (%s), "
-                                              "1 warm-up + median of 3 timed calls" % (frames, variant)}
+            from oracle import ref_runner
+            if ref_runner.available():
+                frames = cfg.frames  # the whole 1024-frame call, as the GPU arm runs it
+                cms, variant = run_cpu_reference(cfg, frames, 4, os.cpu_count() or 1)
+                v = frames / (float(np.median(cms[1:])) / 1e3)
+                line["cpu_baseline"] = {"value": round(v, 2), "unit": UNIT, "cores": os.cpu_count(), "kind": "reference",
+                                        "sample": "the full %d-frame call, 10 DPM steps + CFG, audio.cpp ggml CPU (%s), "
+                                                  "1 warm-up + median of 3 timed calls" % (frames, variant)}
+            else:
+                line["cpu_baseline"] = {"unavailable": "reference CPU build (oracle/_ref) not present"}
         if dit_res is not None:
             line["dit"] = dit_res
         line.update(extra)
