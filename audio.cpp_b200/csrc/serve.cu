@@ -211,7 +211,8 @@ int stream_rows(const BatchView& b, int group) { return int64_t(b.max_new) * gro
 // every tile of 16 rows that reads the keys again, the tensor-tile kernel's with every pair of 128; with 8-bit caches that
 // one also waits for its codes, whatever the rows.  64 sequences of up to 3 tokens over up to 8192 keys, 28 / 4 heads of
 // 128 (21 packed rows at most): stream 253 us, tensor tiles 187 with bf16 caches, 207 and 345 with int8; of up to 5 over
-// 2048 (35 rows): 138 and 64, 132 and 106.  head_dim 32 has no tensor-tile kernel.
+// 2048 (35 rows): 138 and 64, 132 and 106.  A few ragged int8 sequences on both sides of the border pay for two kernels:
+// 8 of up to 9 tokens over 4096 take 35 us, with a border of 16 rows 27.  head_dim 32 has no tensor-tile kernel.
 int stream_most_rows(const KvView& kv) { return kv.head_dim == 32 ? 0x7fffffff : kv.ks ? 32 : 16; }
 
 int64_t batch_packed_rows(const BatchView& b, int group) { return int64_t(std::min(b.max_new, b.rows)) * group; }
