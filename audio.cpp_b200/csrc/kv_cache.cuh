@@ -70,7 +70,8 @@ __device__ __forceinline__ float div_to_odd(float x, float scale) {
     const float y = __fdiv_rn(x, scale);
     const float e = __fmaf_rn(-y, scale, x);  // exact remainder; its sign says on which side of y the quotient lies
     uint32_t u = __float_as_uint(y);
-    if (e != 0.f && !(u & 1u)) u += ((e > 0.f) == (y > 0.f)) ? 1u : 0xffffffffu;
+    // (x has the quotient's sign also where y has underflowed to zero, whose bits may only go up)
+    if (e != 0.f && !(u & 1u)) u += ((e > 0.f) == (x > 0.f)) ? 1u : 0xffffffffu;
     return __uint_as_float(u);
 }
 

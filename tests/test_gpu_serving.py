@@ -300,6 +300,31 @@ def test_append_special_vectors(b2d, ctx, pool):
         assert torch.equal(back[~nan], held[~nan])
 
 
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("pool", ["int8", "e4m3"])
+def test_append_quotients_that_underflow(b2d, ctx, pool, src):
+    """Entries so small that x / scale underflows to zero in fp32, in the same eight elements as one that lies half-way
+    between two codes: zeros of either sign, whatever their neighbours are."""
+    q, half = QMAX[POOLS[pool]], 1.5 if pool == "int8" else 432.0
+    rows = []
+    for scale, tiny in ((4.0, 2.0 ** -149), (2.0 ** 40, 2.0 ** -130), (2.0 ** 100, 2.0 ** -66), (2.0 ** 100, 2.0 ** -51)):
+        for at in range(8):
+            x = torch.zeros(64)
+            x[:8] = torch.tensor([tiny, -tiny] * 4)
+            x[at], x[63] = half * scale, q * scale
+            rows.append(x)
+            rows.append(-x)
+    x = torch.stack(rows)[:, None].to(WIDE[src]).to(DEV)  # powers of two and short mantissas: exact in bf16
+    s = Setup(b2d, [len(rows)], [len(rows)], 1, 64, 16, pool)
+    ctx.kv_append(s.cache, s.batch, x, x, stream=stream())
+    out = [torch.empty_like(x) for _ in range(2)]
+    ctx.kv_gather(s.cache, s.batch, out[0], out[1], stream=stream())
+    ctx.sync(stream())
+    held = quantise(x, s.dtype)[0].to(WIDE[src])
+    for back in out:
+        assert torch.equal(back.cpu(), held)
+
+
 def test_cache_past_32_bit_offsets(b2d, ctx):
     """Pages more than 2^32 bytes apart (written, read back and attended to)."""
     hd, heads, page = 64, 2, 16
