@@ -14,12 +14,12 @@
 //     softmax's meanwhile.  (With one 128-key S a tile the softmax waited for its own products: 2.6 us a block in
 //     place of 2.3, and 2.0 with exponentials on two pipes, although N = 64 reads Q from shared memory twice as often.)
 //   16-bit caches: one warp loads K / V pages with TMA, one box per page and 64-dim panel (128-byte swizzle).
-//   8-bit caches: three pairs of warps read the codes and write them as fp16 in the same layout.  fp16 queries: the codes
-//     stay exact and scales are applied as in paged_stream_kernel: y = s + log2 vs is the logarithm of t = p vs, m
-//     follows y, t = 2^(y - m) is what is rounded and multiplied with the codes, and the row's sum adds t / vs.  bf16
-//     queries: the warps write round(code x scale / 2^e), 2^e the power of two of the largest of 32 scales, so that the
-//     softmax has one factor of its scores and one exponent to add for 32 keys in place of 48 shared loads a half.
-//     Those roundings are of 2^-11 at most, the queries' and the output's own of 2^-8.
+//   8-bit caches: three pairs of warps read the codes and write them as fp16, which is exact, in the same layout.  Scales
+//     are applied as in paged_stream_kernel: y = s + log2 vs is the logarithm of t = p vs, m follows y, t = 2^(y - m) is
+//     what is rounded and multiplied with the codes, and the row's sum adds t / vs.  (fp16 values of code x scale, with one
+//     power of two for 32 keys, spare the softmax 48 shared loads a half: 2.37 in place of 2.71 ms for four int8 prompts.
+//     But a row then loses bits to a key beside those it sees, even one that is masked, whose scale is far above theirs,
+//     and keys off by 2^-11 change which of two large scores is the larger.)
 // K and V have a ring of two blocks each.  TMEM (512 columns): S (and P) of tile t, half h at 128 t + 64 h, O_t at
 // 256 + 128 t.
 // Few units are spread over more CTAs by cutting the key range into `splits`; paged_join_kernel joins the parts.
@@ -31,8 +31,7 @@ namespace b2d {
 
 constexpr int kPtStages = 2;
 constexpr int kPtScaleSlots = 4;
-// Per block: bf16 queries 4 factors of K and 4 exponents of V, fp16 queries the key scales, 1 / value scales and log2 of
-// the value scales of 128 keys.
+// Per block: the key scales, 1 / value scales and log2 of the value scales of 128 keys.
 constexpr int kPtScaleFloats = 3 * 128;
 
 struct PagedTcArgs {
@@ -113,9 +112,8 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                     const PagedTcArgs ta) {
     using Sh = PagedTcShape<POOL, HD>;
     constexpr bool kWide = Sh::kWide;
-    constexpr bool kFold = !kWide && std::is_same<CT, __nv_bfloat16>::value;  // 8-bit scales are in the fp16 values
-    constexpr bool kApart = !kWide && !kFold;                                 // .. or applied key by key in the softmax
-    using MT16 = typename std::conditional<kWide, CT, __half>::type;          // the products' 16-bit type
+    constexpr bool kScaleQ = !kWide && std::is_same<CT, __nv_bfloat16>::value;  // Q as fp16, a power of two a row
+    using MT16 = typename std::conditional<kWide, CT, __half>::type;            // the products' 16-bit type
     const PagedArgs& a = ta.a;
     extern __shared__ uint8_t pt_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~uintptr_t(1023));
@@ -218,7 +216,6 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             // this row of Q into its tile (128-byte swizzle); for 8-bit caches as fp16, scaled by a power of two
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const CT*>(a.q) +
                                                               int64_t(at.s.first + token) * a.q_row + int64_t(hq) * HD);
-            constexpr bool kScaleQ = !kWide && std::is_same<CT, __nv_bfloat16>::value;
             float f = 1.f;
             if constexpr (kScaleQ) {
                 float big = 0.f;
@@ -282,28 +279,20 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             tmem_ld_32x32b_x32(tS, x[0]);
             tmem_ld_32x32b_x32(tS + 32u, x[1]);
             tmem_ld_wait();
-            // factor of the raw scores, and exponent of V that joins theirs: one each for 32 keys
-            float fk[2] = {rf, rf}, ev[2] = {0.f, 0.f};
-            if constexpr (kFold) {
-                const float2 f2 = *reinterpret_cast<const float2*>(sc + 2 * h);
-                const float2 e2 = *reinterpret_cast<const float2*>(sc + 4 + 2 * h);
-                // not zero: a masked score has to stay -inf when it is multiplied
-                fk[0] = fmaxf(rf * f2.x, 1.17549435e-38f), fk[1] = fmaxf(rf * f2.y, 1.17549435e-38f);
-                ev[0] = e2.x, ev[1] = e2.y;
-            }
+            const float2 rf2 = make_float2(rf, rf);
             float top = -INFINITY;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                if constexpr (kApart) {
+                if constexpr (!kWide) {
                     const float* kf = sc + h * 64 + c * 32;
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         const float4 k4 = *reinterpret_cast<const float4*>(kf + e);
                         const float4 v4 = *reinterpret_cast<const float4*>(kf + 256 + e);
-                        const float2 a0 = fma_x2(make_float2(x[c][e], x[c][e + 1]), make_float2(k4.x, k4.y),
-                                                 make_float2(v4.x, v4.y));
-                        const float2 a1 = fma_x2(make_float2(x[c][e + 2], x[c][e + 3]), make_float2(k4.z, k4.w),
-                                                 make_float2(v4.z, v4.w));
+                        float2 a0 = make_float2(x[c][e], x[c][e + 1]), a1 = make_float2(x[c][e + 2], x[c][e + 3]);
+                        if constexpr (kScaleQ) a0 = mul_x2(a0, rf2), a1 = mul_x2(a1, rf2);
+                        a0 = fma_x2(a0, make_float2(k4.x, k4.y), make_float2(v4.x, v4.y));
+                        a1 = fma_x2(a1, make_float2(k4.z, k4.w), make_float2(v4.z, v4.w));
                         x[c][e] = a0.x, x[c][e + 1] = a0.y, x[c][e + 2] = a1.x, x[c][e + 3] = a1.y;
                     }
                 }
@@ -318,7 +307,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[c][e]);
                 const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                top = fmaxf(top, kApart ? most : fmaf(most, fk[c], ev[c]));  // factors are positive
+                top = fmaxf(top, kWide ? most * rf : most);  // rf > 0
             }
             const bool raise = top > m + 8.f;  // also the first visible key: m is -inf
             if (__any_sync(0xffffffffu, raise)) {
@@ -344,23 +333,23 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 }
             }
             const float base = m == -INFINITY ? 0.f : -m;
+            const float2 base2 = make_float2(base, base);
             float sum_h = 0.f;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float2 f2 = make_float2(fk[c], fk[c]), base2 = make_float2(base + ev[c], base + ev[c]);
                 float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
                 float p[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
                     float2 y0 = make_float2(x[c][e], x[c][e + 1]), y1 = make_float2(x[c][e + 2], x[c][e + 3]);
-                    y0 = kApart ? add_x2(y0, base2) : fma_x2(y0, f2, base2);
-                    y1 = kApart ? add_x2(y1, base2) : fma_x2(y1, f2, base2);
+                    y0 = kWide ? fma_x2(y0, rf2, base2) : add_x2(y0, base2);
+                    y1 = kWide ? fma_x2(y1, rf2, base2) : add_x2(y1, base2);
                     y0.x = ex2_approx(y0.x), y0.y = ex2_approx(y0.y);
                     // A quarter of them off MUFU: 145 -> 131 us for 2047 + 1098 rows of 12 / 2 heads over 8191 keys.  Not with
                     // 8-bit caches, whose code warps want the issue slots (2.35 -> 2.54 ms for four int8 prompts).
                     if (kWide && (e & 4)) y1 = ex2_fma_x2(y1);
                     else y1.x = ex2_approx(y1.x), y1.y = ex2_approx(y1.y);
-                    if constexpr (kApart) {
+                    if constexpr (!kWide) {
                         const float4 i4 = *reinterpret_cast<const float4*>(sc + 128 + h * 64 + c * 32 + e);
                         sum[0] = fma_x2(y0, make_float2(i4.x, i4.y), sum[0]);
                         sum[1] = fma_x2(y1, make_float2(i4.z, i4.w), sum[1]);
@@ -373,8 +362,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 }
                 tmem_st_32x32b_x16(tS + uint32_t(c * 16), p);
                 sum[0] = add_x2(sum[0], sum[1]);
-                const float part = sum[0].x + sum[0].y;
-                sum_h += kFold ? part * ex2_approx(-ev[c]) : part;
+                sum_h += sum[0].x + sum[0].y;
             }
             tmem_st_wait();
             tc_fence_before();
@@ -553,7 +541,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             return -1;
         };
         uint4 w[kPieces];
-        float ks = 0.f, vs = 0.f;  // scales of row `lane`; ks for K only
+        float ks = 0.f, vs = 0.f;  // scales of row `lane`, both taken with K
         // Rows without a page: any that can be read, zeroed when stored.
         auto load = [&](int n, int pg) {
             const int first = unit_key(n) & page_mask;
@@ -566,16 +554,8 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             }
             const int p = max(__shfl_sync(0xffffffffu, pg, lane >> 4), 0);
             const int64_t i = ((int64_t(p) * a.kv.kv_heads + head) << a.kv.page_shift) + ((first + lane) & page_mask);
-            if (!(n & 2)) ks = __ldg(a.kv.ks + i);
-            vs = __ldg(a.kv.vs + i);
+            if (!(n & 2)) ks = __ldg(a.kv.ks + i), vs = __ldg(a.kv.vs + i);
         };
-        // Power of two of the largest of the warp's 32 scales (NaN and infinities, which are to come through, aside).
-        auto exponent = [&](float scale) -> int {
-            const uint32_t u = __float_as_uint(scale);
-            const uint32_t most = __reduce_max_sync(0xffffffffu, u < 0x7f800000u ? u : 0u);
-            return min(max(int(most >> 23) - 127, -101), 126);  // held scales are 0 or at least 2^-100
-        };
-        auto power = [](int e) { return __uint_as_float(uint32_t(e + 127) << 23); };
         bool ok = true;
         int n = pair;
         int pg = check_page(n, load_page(n)), next = load_page(n + Sh::kCodePairs);
@@ -587,17 +567,6 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             const uint32_t ph = uint32_t(i / kPtStages) & 1u;
             // a row without a page: zero codes; its probability is 0 or its block reported
             const bool there = __shfl_sync(0xffffffffu, pg, lane >> 4) >= 0 && lane < used && lane >= hidden;
-            int e_k = 0, e_v = 0;
-            uint32_t parts = 0;
-            if constexpr (kFold) {
-                e_k = exponent(there && !is_v ? ks : 0.f);
-                e_v = exponent(there ? vs : 0.f);
-                const float unit = there ? (is_v ? vs * power(-e_v) : ks * power(-e_k)) : 0.f;
-                // the scale in two fp16 parts: code x high + code x low is rounded once (but for 2^-10 of a step)
-                const __half high = __float2half_rn(unit);
-                const __half2 both = __halves2half2(high, __float2half_rn(unit - __half2float(high)));
-                parts = *reinterpret_cast<const uint32_t*>(&both);
-            }
             if (!(ok = warp_wait(is_v ? &v_empty[s] : &k_empty[s], ph ^ 1u, abort_flag, a.b.status, kErrTimeoutProducer)))
                 break;
             uint8_t* tile = smem + (is_v ? Sh::kV : Sh::kK) + s * Sh::kTile + (piece >> 2) * Sh::kPanel + group * 32 * 128;
@@ -611,17 +580,6 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 codes_to_f16<POOL>(c4.y, h[2], h[3]);
                 codes_to_f16<POOL>(c4.z, h[4], h[5]);
                 codes_to_f16<POOL>(c4.w, h[6], h[7]);
-                if constexpr (kFold) {
-                    const uint32_t hl = __shfl_sync(0xffffffffu, parts, row);
-                    const __half2 both = *reinterpret_cast<const __half2*>(&hl);
-                    const __half2 hi2 = __low2half2(both), lo2 = __high2half2(both);
-#pragma unroll
-                    for (int d = 0; d < 8; ++d) {
-                        const __half2 c2 = *reinterpret_cast<const __half2*>(&h[d]);
-                        const __half2 y = __hfma2(c2, hi2, __hmul2(c2, lo2));
-                        h[d] = *reinterpret_cast<const uint32_t*>(&y);
-                    }
-                }
                 uint8_t* dst = tile + row * 128;
                 const int c = 2 * (piece & 3);
                 // the two panels' lanes store their halves in opposite order: no two on one bank
@@ -633,16 +591,11 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
             if (!is_v) {
                 // K of two blocks ago is consumed, so the softmax of four blocks ago is done with this slot's scales
                 float* sc = reinterpret_cast<float*>(smem + Sh::kScale) + slot * kPtScaleFloats;
-                if constexpr (kApart) {
-                    float v = there ? vs : 1.f;
-                    if (v < 3.944304526105059e-31f) v = 3.944304526105059e-31f;  // 2^-101 for a zero scale (of zero codes)
-                    sc[group * 32 + lane] = there ? ks * a.scale_log2 : 0.f;
-                    sc[128 + group * 32 + lane] = 1.f / v;
-                    sc[256 + group * 32 + lane] = __log2f(v);
-                } else if (lane == 0) {
-                    sc[group] = power(e_k) * a.scale_log2;
-                    sc[4 + group] = float(e_v);
-                }
+                float v = there ? vs : 1.f;
+                if (v < 3.944304526105059e-31f) v = 3.944304526105059e-31f;  // 2^-101 for a zero scale (of zero codes)
+                sc[group * 32 + lane] = there ? ks * a.scale_log2 : 0.f;
+                sc[128 + group * 32 + lane] = 1.f / v;
+                sc[256 + group * 32 + lane] = __log2f(v);
             }
             pg = check_page(n + Sh::kCodePairs, next);
             if (n + Sh::kCodePairs < units) load(n + Sh::kCodePairs, pg);

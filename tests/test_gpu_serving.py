@@ -421,6 +421,106 @@ def test_attention_growing_and_extreme_scores(b2d, ctx, dtype):
             check_attention(s, rise, out, scale=1.0)
 
 
+# 8-bit caches whose scales differ from key to key, in either kernel.  The bound looks at what a row sees alone.  Codes are
+# exact, so a score is off by d = (head_dim + 8) 2^-24 sum |q k_j| scale at most, which moves a probability p_j by p_j
+# (exp(d) - 1) and the output by the sum of that times (|v_j| + |o|).  (Where d is large -- scores of 2^21 beside one another
+# -- the few units that such an fp32 sum is really off by are far below the 40 that d is cut to, so that exp stays finite.)
+# Probabilities (times value scales) are fp16: 2^-11 of A = sum p |v| / sum p, and what falls below 2^-14 is off by 2^-25 of
+# the key's that set the running maximum (see above), here of the largest value seen.  Sums of a score and the logarithm
+# of a scale are below 2^7, so two of them are off by 2^-18 each, less than 2^-17 of p.
+def check_uneven(s, q, out, group, window=0, scale=None):
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    u, hd, worst = torch.finfo(q.dtype).eps / 2, q.shape[2], 0.0
+    for i, c in enumerate(s.context):
+        n, r0 = s.new[i], s.start[i]
+        if n == 0 or c == 0:
+            continue
+        qs = q[r0:r0 + n].double().reshape(n, -1, group, hd)
+        pos = torch.arange(c - n, c, device=q.device)
+        dist = pos[:, None] - torch.arange(c, device=q.device)[None]
+        seen = ((dist >= 0) & (dist < (window if window > 0 else c + 1)))[:, None, None]
+        score = (torch.einsum("nhgd,khd->nhgk", qs, s.dense_k[i]) * scale).masked_fill(~seen, -torch.inf)
+        p = torch.softmax(score, -1)
+        big = torch.einsum("nhgd,khd->nhgk", qs.abs(), s.dense_k[i].abs()) * scale
+        off = p * torch.expm1((big * (hd + 8) * 2.0 ** -24).clamp(max=40.0))
+        v = s.dense_v[i]
+        o, a = (torch.einsum("nhgk,khd->nhgd", p, x) for x in (v, v.abs()))
+        vmax = torch.where(seen, v.abs().amax(-1).T[None, :, None], 0.0).amax(-1, keepdim=True)
+        bound = u * o.abs() + a * (2.0 ** -11 + 2.0 ** -16)
+        bound += 1.01 * (torch.einsum("nhgk,khd->nhgd", off, v.abs()) + o.abs() * off.sum(-1, keepdim=True))
+        bound += c * 2.0 ** -25 * vmax + (2.0 ** -24 if q.dtype == torch.float16 else 0.0) + 1e-30
+        got = out[r0:r0 + n].double().reshape(o.shape)
+        if q.dtype == torch.float16:  # from half a step above its largest number on, fp16 rounds to an infinity
+            over = (o.abs() + bound >= 65520.0) & (torch.isinf(got) & (got * o > 0))
+            got = torch.where(over, o, got)
+        assert torch.isfinite(got).all()
+        worst = max(worst, float(((got - o).abs() / bound).max()))
+    assert worst <= 1.0, "error is %.3g of its bound" % worst
+
+
+def rewrite(s, name, change):
+    """The cache's keys or values (name) become the quantised change(sequence, values) of what they were."""
+    dense, store, scales = (s.dense_k, s.k, s.ks) if name == "k" else (s.dense_v, s.v, s.vs)
+    for i, c in enumerate(s.context):
+        pos = torch.arange(c, device=DEV)
+        rows = s.table[i, pos // s.page].long()
+        held, scale = (t.to(DEV) for t in quantise(change(i, dense[i].float()), s.dtype))
+        code = torch.where(scale[..., None] > 0, held / scale[..., None], torch.zeros_like(held))
+        code = code.round().to(torch.int8) if s.dtype == torch.int8 else code.to(s.dtype)
+        store.view(torch.uint8)[rows, :, pos % s.page] = code.view(torch.uint8)
+        scales[rows, :, pos % s.page] = scale
+        dense[i] = held.double()
+
+
+UNEVEN = ["spread", "late_values", "late_keys", "zero_groups", "rising"]
+
+
+@pytest.mark.parametrize("kind", UNEVEN)
+@pytest.mark.parametrize("pool", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new,context,head_dim,page,window", [
+    ([200], [200], 128, 16, 0), ([64], [3000], 128, 64, 0), ([1, 2, 4], [700, 90, 301], 128, 32, 0),
+    ([40, 70, 1, 16], [600, 300, 400, 333], 64, 128, 0), ([1, 3, 50], [700, 130, 500], 64, 16, 77),
+    ([3, 40], [200, 150], 32, 16, 0)])
+def test_attention_uneven_scales(b2d, ctx, new, context, head_dim, page, window, dtype, pool, kind):
+    """Scales that differ by orders of magnitude between neighbouring keys: spread over 2^20; a key in 32 far above its
+    neighbours, which rows before it do not see; all-zero vectors, 32 together; scores that rise key by key."""
+    kv, group = 2, 4
+    s = Setup(b2d, new, context, kv, head_dim, page, pool, seed=7)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    q = torch.randn(s.rows, kv * group, head_dim, generator=g, device=DEV).to(WIDE[dtype])
+
+    def powers(x, lo, hi):
+        return x * 2.0 ** (lo + (hi - lo) * torch.rand(x.shape[:2], generator=g, device=DEV))[..., None]
+
+    def late(x, power):
+        x = x.clone()
+        x[31::32] *= 2.0 ** power
+        return x
+
+    def zeros(x, at):
+        x = x.clone()
+        x[at(torch.arange(len(x), device=DEV))] = 0
+        return x
+    if kind == "spread":
+        rewrite(s, "k", lambda i, x: powers(x, -10, 2))
+        rewrite(s, "v", lambda i, x: powers(x, -10, 10))
+    elif kind == "late_values":
+        rewrite(s, "v", lambda i, x: late(x, 30))
+    elif kind == "late_keys":
+        rewrite(s, "k", lambda i, x: late(x, 20))
+    elif kind == "zero_groups":
+        rewrite(s, "k", lambda i, x: zeros(x, lambda j: j // 32 % 3 == 1))
+        rewrite(s, "v", lambda i, x: zeros(x, lambda j: j // 32 % 2 == 1))
+    else:
+        ramp = torch.linspace(0, 40, max(context), device=DEV)
+        rewrite(s, "k", lambda i, x: torch.cat([ramp[:len(x), None, None].expand(-1, kv, 1), 0.05 * x[..., 1:]], -1))
+        rewrite(s, "v", lambda i, x: powers(x, -6, 6))
+        q[..., 0] = head_dim ** 0.5
+    check_uneven(s, q, attend(ctx, s, q, window), group, window)
+    ctx.sync(stream())
+
+
 def test_attention_reads_no_stale_slots(b2d, ctx):
     """Codes, scales and values behind a context, in its last page and in other pages, are NaN or garbage (Setup fills them);
     tables are -7 behind the last page.  The result does not change when they do."""
