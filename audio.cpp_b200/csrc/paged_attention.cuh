@@ -36,6 +36,13 @@ namespace b2d {
 constexpr int kPaWarps = 4;
 constexpr int kPaTileKeys = 16 * kPaWarps;
 
+// What a value scale of 0 counts as: its codes are 0, so only the key's p matters, and the running maximum has to stay within
+// 2^126 of its score.  p then survives beside scales of up to 2^41 (what underflows is below 2^-25 of the largest p), and
+// the key takes nothing from values whose scale is 2^-60 or more.  (As 2^-101, the least scale that is held, it lost its
+// share of the sum beside values of 2^24.)
+constexpr float kZeroScale = 8.673617379884035e-19f;  // 2^-60
+constexpr float kZeroScaleLog2 = -60.f;
+
 struct PagedArgs {
     KvView kv;
     BatchView b;
@@ -521,7 +528,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PagedShape<CT, POOL, HD, NT>::k
                 for (int i = 0; i < 2; ++i) {
                     const int key = pos + g + 8 * i;
                     if (key < any_lo || key > any_hi || this_page < 0) vsc[i] = 0.f;  // a slot no row sees
-                    lv[i] = fmaxf(__log2f(vsc[i]), -101.f);  // held scales are 0 or at least 2^-100
+                    lv[i] = vsc[i] == 0.f ? kZeroScaleLog2 : fmaxf(__log2f(vsc[i]), -101.f);  // held scales: at least 2^-100
                 }
             }
             bool exceed = false;

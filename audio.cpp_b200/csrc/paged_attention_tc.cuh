@@ -592,7 +592,8 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                 // K of two blocks ago is consumed, so the softmax of four blocks ago is done with this slot's scales
                 float* sc = reinterpret_cast<float*>(smem + Sh::kScale) + slot * kPtScaleFloats;
                 float v = there ? vs : 1.f;
-                if (v < 3.944304526105059e-31f) v = 3.944304526105059e-31f;  // 2^-101 for a zero scale (of zero codes)
+                if (v == 0.f) v = kZeroScale;
+                else if (v < 3.944304526105059e-31f) v = 3.944304526105059e-31f;  // 2^-101: held scales are above it
                 sc[group * 32 + lane] = there ? ks * a.scale_log2 : 0.f;
                 sc[128 + group * 32 + lane] = 1.f / v;
                 sc[256 + group * 32 + lane] = __log2f(v);

@@ -451,7 +451,7 @@ def check_uneven(s, q, out, group, window=0, scale=None):
         bound += c * 2.0 ** -25 * vmax + (2.0 ** -24 if q.dtype == torch.float16 else 0.0) + 1e-30
         got = out[r0:r0 + n].double().reshape(o.shape)
         if q.dtype == torch.float16:  # from half a step above its largest number on, fp16 rounds to an infinity
-            over = (o.abs() + bound >= 65520.0) & (torch.isinf(got) & (got * o > 0))
+            over = ((got == torch.inf) & (o + bound >= 65520.0)) | ((got == -torch.inf) & (o - bound <= -65520.0))
             got = torch.where(over, o, got)
         assert torch.isfinite(got).all()
         worst = max(worst, float(((got - o).abs() / bound).max()))
@@ -472,7 +472,7 @@ def rewrite(s, name, change):
         dense[i] = held.double()
 
 
-UNEVEN = ["spread", "late_values", "late_keys", "zero_groups", "rising"]
+UNEVEN = ["spread", "late_values", "late_keys", "zeros", "zeros_first", "zero_groups", "rising"]
 
 
 @pytest.mark.parametrize("kind", UNEVEN)
@@ -484,7 +484,8 @@ UNEVEN = ["spread", "late_values", "late_keys", "zero_groups", "rising"]
     ([3, 40], [200, 150], 32, 16, 0)])
 def test_attention_uneven_scales(b2d, ctx, new, context, head_dim, page, window, dtype, pool, kind):
     """Scales that differ by orders of magnitude between neighbouring keys: spread over 2^20; a key in 32 far above its
-    neighbours, which rows before it do not see; all-zero vectors, 32 together; scores that rise key by key."""
+    neighbours, which rows before it do not see; all-zero vectors, alone, 32 together and before all others, beside large
+    values; scores that rise key by key."""
     kv, group = 2, 4
     s = Setup(b2d, new, context, kv, head_dim, page, pool, seed=7)
     g = torch.Generator(device=DEV).manual_seed(8)
@@ -509,6 +510,11 @@ def test_attention_uneven_scales(b2d, ctx, new, context, head_dim, page, window,
         rewrite(s, "v", lambda i, x: late(x, 30))
     elif kind == "late_keys":
         rewrite(s, "k", lambda i, x: late(x, 20))
+    elif kind == "zeros":
+        rewrite(s, "k", lambda i, x: zeros(x, lambda j: j % 7 == 3))
+        rewrite(s, "v", lambda i, x: late(zeros(x, lambda j: j % 5 == 1), 24))
+    elif kind == "zeros_first":
+        rewrite(s, "v", lambda i, x: late(zeros(x, lambda j: j < 64), 40))
     elif kind == "zero_groups":
         rewrite(s, "k", lambda i, x: zeros(x, lambda j: j // 32 % 3 == 1))
         rewrite(s, "v", lambda i, x: zeros(x, lambda j: j // 32 % 2 == 1))
