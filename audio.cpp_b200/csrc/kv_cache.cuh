@@ -45,21 +45,22 @@ struct BatchView {
 
 __device__ __forceinline__ void batch_error(const BatchView& b) { atomicCAS(b.status, 0, int(kErrCacheBatch)); }
 
-// New rows and context of sequence s, forced into the call's bounds (first = its first packed row).
+// A sequence whose rows r0 .. r1 - 1 or context c break one of the call's bounds: it has no rows in any kernel, so that
+// what is written, read back and attended to agree.
+__device__ __forceinline__ bool out_of_bounds(const BatchView& b, int r0, int r1, int c) {
+    return r0 < 0 || r1 < r0 || r1 > b.rows || r1 - r0 > b.max_new || uint32_t(c) > uint32_t(b.max_context);
+}
+
+// New rows and context of sequence s (first = its first packed row).
 struct SeqSpan {
     int first, n, context;
 };
 
 __device__ __forceinline__ SeqSpan seq_span(const BatchView& b, int s, bool report) {
     const int r0 = __ldg(b.row_start + s), r1 = __ldg(b.row_start + s + 1), c = __ldg(b.context + s);
-    SeqSpan v;
-    v.first = min(max(r0, 0), b.rows);
-    v.n = min(max(r1, v.first), b.rows) - v.first;
-    v.context = min(max(c, 0), b.max_context);
-    const bool bad = v.first != r0 || v.first + v.n != r1 || v.context != c || v.n > b.max_new;
-    if (bad) v.n = min(v.n, b.max_new);
+    const bool bad = out_of_bounds(b, r0, r1, c);
     if (bad && report) batch_error(b);
-    return v;
+    return bad ? SeqSpan{0, 0, 0} : SeqSpan{r0, r1 - r0, c};
 }
 
 // ------------------------------------------------------------------------------------ quantisation of one vector
@@ -180,12 +181,8 @@ __device__ __forceinline__ void stage_batch(const BatchView& b, int* start, int*
     __syncthreads();
     // rows that no sequence could own, sequences that overlap: reported once, by the first block
     if (blockIdx.x == 0) {
-        for (int i = threadIdx.x; i < b.seqs; i += blockDim.x) {
-            const int n = start[i + 1] - start[i];
-            if (n < 0 || n > b.max_new || start[i] < 0 || start[i + 1] > b.rows || context[i] < 0 ||
-                context[i] > b.max_context)
-                batch_error(b);
-        }
+        for (int i = threadIdx.x; i < b.seqs; i += blockDim.x)
+            if (out_of_bounds(b, start[i], start[i + 1], context[i])) batch_error(b);
     }
 }
 
@@ -197,10 +194,8 @@ __device__ __forceinline__ RowPlace place_row(const BatchView& b, const int* sta
         else hi = mid;
     }
     const int s = lo - 1;
-    if (s < 0 || row >= start[s + 1]) return {-1, -1};
-    const int c = min(max(context[s], 0), b.max_context);
-    const int pos = c - (start[s + 1] - row);
-    return {s, pos};
+    if (s < 0 || row >= start[s + 1] || out_of_bounds(b, start[s], start[s + 1], context[s])) return {-1, -1};
+    return {s, context[s] - (start[s + 1] - row)};
 }
 
 // Page of a position, or -1 (reported) when the table names one outside the pool.

@@ -443,8 +443,9 @@ typedef struct {
  * position % page_size of page page_table[s * table_stride + position / page_size].  A row at a negative position has
  * no place.  Rows before the first or behind the last sequence are left as they are.
  * The arrays are read on the device and may change between replays of a captured graph, within the bounds given
- * here.  An index outside its bound (a page outside the cache, rows that overlap or exceed max_new or rows, a context
- * above max_context) is not followed; b2d_sync then returns B2D_EINVAL. */
+ * here.  An index outside its bound is not followed, and b2d_sync then returns B2D_EINVAL: a sequence whose row_start
+ * falls, whose rows exceed max_new or rows, or whose context is negative or above max_context, has no rows in that call;
+ * what a page outside the cache would hold is neither written nor read (the rows that would see it are unspecified). */
 typedef struct {
     int32_t seqs;                /* 0 to 8192 */
     int32_t max_new;             /* no sequence has more new rows */

@@ -635,6 +635,55 @@ def test_bad_indexes_are_reported_and_not_followed(b2d, ctx):
     ctx.sync(stream())
 
 
+@pytest.mark.parametrize("pool", ["f16", "int8"])
+@pytest.mark.parametrize("change,bad", [
+    (dict(row_start=[0, 1, 4, 4]), [1]), (dict(row_start=[0, 1, 2, 50]), [2]), (dict(row_start=[-1, 1, 2, 4]), [0]),
+    (dict(row_start=[0, 2, 1, 2]), [1]), (dict(context=[40, 61, 60]), [1]), (dict(context=[40, -3, 60]), [1])])
+def test_a_sequence_outside_its_bounds_has_no_rows(b2d, ctx, pool, change, bad):
+    """Too many rows, rows past the buffer or before it, a row_start that falls, contexts outside their bounds: nothing of
+    such a sequence is written, read back or attended to, the others are done, and b2d_sync refuses."""
+    s = Setup(b2d, [1, 1, 2], [40, 50, 60], 2, 64, 16, pool)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    q = torch.randn(s.rows, 4, 64, generator=g, device=DEV).half()
+    k, v = (torch.randn(s.rows, 2, 64, generator=g, device=DEV).half() for _ in range(2))
+    good = attend(ctx, s, q)
+    ctx.sync(stream())
+    before = [t.clone() for t in (s.k, s.v)]
+    for name, values in change.items():
+        (s.row_start if name == "row_start" else s.context_dev).copy_(torch.tensor(values, dtype=torch.int32))
+    start = change.get("row_start", [0, 1, 2, 4])
+    out = attend(ctx, s, q)
+    with pytest.raises(b2d.B2DError, match="paged cache batch"):
+        ctx.sync(stream())
+    back = [torch.full_like(k, 9.0) for _ in range(2)]
+    ctx.kv_gather(s.cache, s.batch, back[0], back[1], stream=stream())
+    with pytest.raises(b2d.B2DError, match="paged cache batch"):
+        ctx.sync(stream())
+    ctx.kv_append(s.cache, s.batch, k, v, stream=stream())
+    with pytest.raises(b2d.B2DError, match="paged cache batch"):
+        ctx.sync(stream())
+    if "row_start" in change and change["row_start"][1] == 2:
+        return  # which of two sequences a row that both claim belongs to is not said; the calls end and report
+    untouched = torch.ones(s.k.shape[:3], dtype=torch.bool, device=DEV)
+    owned = torch.zeros(s.rows, dtype=torch.bool, device=DEV)
+    for i in range(3):
+        if i in bad:
+            continue
+        n, c = start[i + 1] - start[i], s.context[i]
+        pos = torch.arange(c - n, c, device=DEV)
+        at = s.table[i, pos // 16].long()
+        untouched[at, :, pos % 16] = False
+        owned[start[i]:start[i + 1]] = True
+        if start[i:i + 2] == s.start[i:i + 2]:
+            assert torch.equal(out[start[i]:start[i + 1]], good[start[i]:start[i + 1]])
+            for t, x in zip(back, (s.dense_k, s.dense_v)):
+                assert torch.equal(t[start[i]:start[i + 1]], x[i][pos].half())
+    assert (out[~owned] == 77.0).all()
+    for t, store, old in zip(back, (s.k, s.v), before):
+        assert (t[~owned] == 9.0).all()
+        assert torch.equal(store.view(torch.uint8)[untouched], old.view(torch.uint8)[untouched])
+
+
 def test_refusals(b2d, ctx):
     s = Setup(b2d, [2], [20], 2, 64, 16, "f16")
     q = torch.zeros(2, 4, 64, device=DEV, dtype=torch.float16)
