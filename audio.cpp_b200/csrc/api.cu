@@ -336,7 +336,7 @@ struct b2d_ctx {
     int device = 0;
     int num_sms = 148;
     std::string err;
-    DevBuf status;  // int device-side status word
+    DevBuf status;  // device-side status words (StatusWord)
     cudaStream_t load_stream = nullptr;
     std::unique_ptr<HeadModel> head;
     std::unique_ptr<DitModel> dit;
@@ -379,17 +379,25 @@ b2d_status guarded(b2d_ctx* ctx, F&& f) {
     }
 }
 
-void check_status_word(b2d_ctx* ctx, cudaStream_t st) {
-    int s = 0;
-    CK(cudaMemcpyAsync(&s, ctx->status.p, sizeof(int), cudaMemcpyDeviceToHost, st));
-    CK(cudaStreamSynchronize(st));
-    if (s != 0) {
-        CK(cudaMemsetAsync(ctx->status.p, 0, sizeof(int), st));
+// What kernels reported once the stream's work is done.  A word is cleared as it is reported; that of the paged batches
+// is for the caller who asks for it.
+void check_status_word(b2d_ctx* ctx, cudaStream_t st, bool* bad_batch = nullptr) {
+    int s[kStatusWords] = {0, 0};
+    auto clear = [&](StatusWord which) {
+        CK(cudaMemsetAsync(ctx->status.as<int>() + which, 0, sizeof(int), st));
         CK(cudaStreamSynchronize(st));
-        if (s == kErrNonFinite) fail(B2D_ENONFINITE, "VibeVoice diffusion sampler produced non-finite latent");
-        if (s == kErrCacheBatch)
-            fail(B2D_EINVAL, "paged cache batch names a page, rows or a context outside the call's bounds");
-        fail(B2D_ETIMEOUT, "a device-side wait expired (code %d); the kernel unwound", s);
+    };
+    CK(cudaMemcpyAsync(s, ctx->status.p, sizeof(s), cudaMemcpyDeviceToHost, st));
+    CK(cudaStreamSynchronize(st));
+    if (s[kStatusError] != 0) {
+        clear(kStatusError);
+        if (s[kStatusError] == kErrNonFinite)
+            fail(B2D_ENONFINITE, "VibeVoice diffusion sampler produced non-finite latent");
+        fail(B2D_ETIMEOUT, "a device-side wait expired (code %d); the kernel unwound", s[kStatusError]);
+    }
+    if (bad_batch) {
+        *bad_batch = s[kStatusBatch] != 0;
+        if (*bad_batch) clear(kStatusBatch);
     }
 }
 
@@ -1066,13 +1074,16 @@ b2d_status b2d_selftest_wait_timeout(b2d_ctx* ctx, uint32_t polls, void* stream)
 
 b2d_status b2d_sync(b2d_ctx* ctx, void* stream) {
     return guarded(ctx, [&] {
+        bool bad_batch = false;
         try {
-            check_status_word(ctx, static_cast<cudaStream_t>(stream));
+            check_status_word(ctx, static_cast<cudaStream_t>(stream), &bad_batch);
         } catch (...) {
             // an asynchronous decoder forward may have written garbage cache rows: the next call must prefill
             lm_invalidate(ctx);
             throw;
         }
+        // (the caller's own mistake: what the decoder holds in the context's cache is not concerned)
+        if (bad_batch) fail(B2D_EINVAL, "paged cache batch names a page, rows or a context outside the call's bounds");
     });
 }
 

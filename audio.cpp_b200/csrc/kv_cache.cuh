@@ -6,7 +6,7 @@
 // row_start[s] .. row_start[s + 1]; its context (new rows included) is context[s] long, so its row i sits at position
 // context[s] - n + i, in slot position % page_size of page page_table[s][position / page_size].
 // Every index that comes from device memory is checked against the bounds the host gave before it is used; one that
-// is outside raises kErrCacheBatch in the status word and its access is skipped.
+// is outside sets the status word kStatusBatch and its access is skipped.
 #pragma once
 
 #include <cstdint>
@@ -40,10 +40,10 @@ struct BatchView {
     int rows;
     int max_new;
     int max_context;
-    int* status;
+    int* status;  // kStatusWords words
 };
 
-__device__ __forceinline__ void batch_error(const BatchView& b) { atomicCAS(b.status, 0, int(kErrCacheBatch)); }
+__device__ __forceinline__ void batch_error(const BatchView& b) { atomicOr(b.status + kStatusBatch, 1); }
 
 // A sequence whose rows r0 .. r1 - 1 or context c break one of the call's bounds: it has no rows in any kernel, so that
 // what is written, read back and attended to agree.

@@ -22,8 +22,10 @@ enum DeviceError : int {
     kErrTimeoutMma = 2,
     kErrTimeoutEpilogue = 3,
     kErrNonFinite = 4,
-    kErrCacheBatch = 5,
 };
+// The context's status words: what its kernels ran into (one of the above), and whether a batch of a paged cache broke its
+// bounds.  The second is the caller's doing and concerns no other call.
+enum StatusWord : int { kStatusError = 0, kStatusBatch = 1, kStatusWords = 2 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));

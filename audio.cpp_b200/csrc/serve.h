@@ -10,7 +10,7 @@ namespace b2d {
 
 struct ServeDevice {
     int num_sms;
-    int* status;  // the context's device-side status word
+    int* status;  // the context's device-side status words (StatusWord)
 };
 
 void kv_check(const b2d_kv_cache* cache, const b2d_kv_batch* batch, int heads);

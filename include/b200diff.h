@@ -445,7 +445,8 @@ typedef struct {
  * The arrays are read on the device and may change between replays of a captured graph, within the bounds given
  * here.  An index outside its bound is not followed, and b2d_sync then returns B2D_EINVAL: a sequence whose row_start
  * falls, whose rows exceed max_new or rows, or whose context is negative or above max_context, has no rows in that call;
- * what a page outside the cache would hold is neither written nor read (the rows that would see it are unspecified). */
+ * what a page outside the cache would hold is neither written nor read (the rows that would see it are unspecified).
+ * No other call reports it, and b2d_vvlm_prefill's cache and position stay as they are. */
 typedef struct {
     int32_t seqs;                /* 0 to 8192 */
     int32_t max_new;             /* no sequence has more new rows */

@@ -281,3 +281,35 @@ def test_vvlm_paged_refusals(b2d, ctx):
         lm.forward_paged(rows, half, batch, logits, workspace=work)
     lm.forward_paged(rows, caches, batch, logits, workspace=work)
     ctx.sync()
+
+
+def test_vvlm_paged_batch_errors_do_not_reach_the_dense_cache(b2d, ctx):
+    """A paged batch that names a page outside its cache, in the middle of the one-sequence calls: b2d_sync says so, once; the
+    one-sequence calls go on as if it had not been."""
+    import torch
+    cfg, inp, lm, table = _paged_lm(b2d, ctx, "vvlm_tiny")
+    host, prompt, steps = table.cpu().numpy(), inp["prefill_ids"].array(), inp["step_ids"].array()[:3]
+    lm.prefill(host[prompt])
+    want = [lm.step(host[i])[0] for i in steps]
+    caches = _paged_caches(b2d, cfg, 4, 16, "float16")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    bad = b2d.PagedBatch(torch.tensor([0, 2], **i32), torch.tensor([2], **i32), torch.full((1, 2), 99, **i32), 2, 2, 32)
+    work = torch.empty(lm.paged_workspace(caches, bad), dtype=torch.uint8, device="cuda")
+    logits = torch.empty(1, cfg.vocab, device="cuda")
+
+    def break_bounds():
+        lm.forward_paged(table[:2].contiguous(), caches, bad, logits, workspace=work)
+        torch.cuda.synchronize()
+    lm.prefill(host[prompt])
+    break_bounds()
+    got = [lm.step(host[steps[0]])[0]]  # blocking calls look at the status of their own kernels
+    with pytest.raises(b2d.B2DError, match="paged cache batch"):
+        ctx.sync()
+    got.append(lm.step(host[steps[1]])[0])
+    break_bounds()
+    with pytest.raises(b2d.B2DError, match="paged cache batch"):
+        ctx.sync()
+    got.append(lm.step(host[steps[2]])[0])
+    ctx.sync()
+    for a, b in zip(want, got):
+        assert np.array_equal(a, b)
