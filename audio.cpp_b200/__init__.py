@@ -437,6 +437,16 @@ class Context:
     def _elsewhere(self, what: str):
         return B2DError(-1, "%s is not on this context's device cuda:%d" % (what, self.device))
 
+    def _workspace(self, t):
+        """(address, bytes) of a workspace tensor; nothing for None, which the library refuses."""
+        if t is None:
+            return None, 0
+        if t.get_device() != self.device:
+            raise self._elsewhere("a workspace tensor")
+        if not t.is_contiguous():
+            raise B2DError(-1, "a workspace must be a contiguous tensor: its bytes are taken from its size")
+        return t.data_ptr(), t.nbytes
+
     def _cache_rows(self, cache: PagedCache, batch: PagedBatch, k, v):
         """(element type, row stride) of k / v rows [rows, kv_heads, head_dim] whose last two dimensions are packed."""
         batch.fits(cache)
@@ -484,16 +494,14 @@ class Context:
         if out.shape != shape or out.dtype != q.dtype or qs[2] != 1 or qs[1] != hd or os_[2] != 1 or os_[1] != hd:
             raise B2DError(-1, "paged attention q and out must be alike with packed heads")
         dev = self.device
-        if q.get_device() != dev or out.get_device() != dev or cache.device != dev or batch.device != dev or \
-                (workspace is not None and workspace.get_device() != dev):
-            raise self._elsewhere("a cache, batch, query, output or workspace tensor")
+        if q.get_device() != dev or out.get_device() != dev or cache.device != dev or batch.device != dev:
+            raise self._elsewhere("a cache, batch, query or output tensor")
         heads = shape[1]
         many = shape[0] > 1
         st = lib().b2d_paged_attention(
             self._h, cache.ref, batch.ref, 1 if kind == TYPE_BF16 else 0, q.data_ptr(), qs[0] if many else heads * hd,
             out.data_ptr(), os_[0] if many else heads * hd, heads, hd ** -0.5 if scale is None else scale, window,
-            workspace.data_ptr() if workspace is not None else None, workspace.nbytes if workspace is not None else 0,
-            stream)
+            *self._workspace(workspace), stream)
         if st:
             self.check(st)
 
@@ -834,7 +842,7 @@ class VibeVoiceLanguageModel:
                     raise self.ctx._elsewhere(name)
         self.ctx.check(lib().b2d_vvlm_forward_paged(
             self.ctx.handle, descs, batch.ref, _ptr(embeddings), _ptr(logits), _ptr(hidden) if hidden is not None else None,
-            _ptr(workspace) if workspace is not None else None, workspace.nbytes if workspace is not None else 0, stream))
+            *self.ctx._workspace(workspace), stream))
 
 
 class VibeVoiceDiffusionHead:

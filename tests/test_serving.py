@@ -81,3 +81,53 @@ def test_python_layer_refuses_mismatched_tensors(b2d):
             b2d.PagedBatch(*bad, rows=2, max_new=1, max_context=16)
     with pytest.raises(b2d.B2DError, match="max_context"):
         b2d.check_paged(_cache(b2d), b2d.PagedBatch(start, context, table, rows=2, max_new=1, max_context=49))
+
+
+def _no_device_context(b2d):
+    """A context without a library handle, whose device is that of CPU tensors: what the Python layer lets through, the
+    library refuses for the missing handle, with another message."""
+    ctx = object.__new__(b2d.Context)
+    ctx._h, ctx.device = None, torch.zeros(1).get_device()
+    return ctx
+
+
+def test_workspaces_are_checked_before_their_address_is_used(b2d):
+    """A workspace elsewhere, or one whose elements are not one block (an expanded byte has as many nbytes as asked for)."""
+    ctx = _no_device_context(b2d)
+    lm = object.__new__(b2d.VibeVoiceLanguageModel)
+    lm.ctx = ctx
+    lm.cfg = b2d.VvlmConfig(hidden=128, layers=1, vocab=10)
+    cache, batch = _cache(b2d), _batch(b2d)
+    q, rows, logits = torch.zeros(4, 2, 64, dtype=torch.float16), torch.zeros(4, 128), torch.zeros(2, 10)
+
+    def attention(w):
+        ctx.paged_attention(q, cache, batch, torch.empty_like(q), workspace=w)
+
+    def forward(w):
+        lm.forward_paged(rows, [cache], batch, logits, workspace=w)
+    for call in (attention, forward):
+        for w in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 20, dtype=torch.uint8)[::2]):
+            with pytest.raises(b2d.B2DError, match="contiguous"):
+                call(w)
+        ctx.device = 5  # of everything but the workspace
+        cache.device = batch.device = 5
+        elsewhere = torch.zeros(1 << 20, dtype=torch.uint8)
+        tensors = (q, rows, logits)
+
+        class There:  # a tensor of device 5, as far as the checks look
+            def __init__(self, t):
+                self.t = t
+
+            def __getattr__(self, name):
+                return getattr(self.t, name)
+
+            def get_device(self):
+                return 5
+        q, rows, logits = (There(t) for t in tensors)
+        with pytest.raises(b2d.B2DError, match="workspace"):
+            if call is attention:
+                ctx.paged_attention(q, cache, batch, There(torch.empty(4, 2, 64, dtype=torch.float16)), workspace=elsewhere)
+            else:
+                call(elsewhere)
+        q, rows, logits = tensors
+        ctx.device = cache.device = batch.device = torch.zeros(1).get_device()
