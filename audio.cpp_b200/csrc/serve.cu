@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kMaxSeqs = 8192;  // row_start and context are staged in shared memory
 constexpr int64_t kMaxVectors = int64_t(1) << 30;
+constexpr int kMaxContext = 1 << 30;  // positions, rounded up to tiles and less a window and the new rows, stay in 32 bits
 
 int pool_kind(int type) {
     switch (type) {
@@ -72,6 +73,8 @@ BatchView batch_view(const b2d_kv_batch* b, const b2d_kv_cache* c, int* status) 
     if (b->seqs < 0 || b->seqs > kMaxSeqs) fail(B2D_EINVAL, "paged cache batch of %d sequences (0 to %d)", b->seqs, kMaxSeqs);
     if (b->rows < 0 || b->rows > kMaxVectors / c->kv_heads || b->max_new < 0 || b->max_context < 0)
         fail(B2D_EINVAL, "paged cache batch sizes are negative or too large");
+    if (b->max_context > kMaxContext)
+        fail(B2D_EINVAL, "paged cache batch max_context %d is above %d", b->max_context, kMaxContext);
     if (b->seqs > 0 && (!b->row_start || !b->context || !b->page_table))
         fail(B2D_EINVAL, "paged cache batch needs row_start, context and page_table");
     if (misaligned(b->row_start, 4) || misaligned(b->context, 4) || misaligned(b->page_table, 4))

@@ -450,7 +450,7 @@ typedef struct {
 typedef struct {
     int32_t seqs;                /* 0 to 8192 */
     int32_t max_new;             /* no sequence has more new rows */
-    int32_t max_context;         /* no context is longer; table_stride pages hold it */
+    int32_t max_context;         /* no context is longer (at most 2^30); table_stride pages hold it */
     int64_t rows;                /* rows of the packed buffers */
     const int32_t* row_start;    /* [seqs + 1] */
     const int32_t* context;      /* [seqs] */

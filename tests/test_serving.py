@@ -131,3 +131,16 @@ def test_workspaces_are_checked_before_their_address_is_used(b2d):
                 call(elsewhere)
         q, rows, logits = tensors
         ctx.device = cache.device = batch.device = torch.zeros(1).get_device()
+
+
+@pytest.mark.parametrize("most,fits", [(1 << 30, True), ((1 << 30) + 1, False), (2 ** 31 - 1, False)])
+def test_contexts_next_to_2_31_are_refused(b2d, most, fits):
+    """Position arithmetic is 32-bit: 2^31 - 1 positions rounded up to whole tiles would not be."""
+    cache, batch = _cache(b2d), _batch(b2d)
+    batch.desc.max_context, batch.desc.table_stride = most, 1 << 40
+    batch.table_pages = 1 << 40
+    if fits:
+        b2d.check_paged(cache, batch)
+    else:
+        with pytest.raises(b2d.B2DError, match="max_context"):
+            b2d.check_paged(cache, batch)
