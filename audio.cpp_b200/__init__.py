@@ -478,7 +478,10 @@ class Context:
     def paged_attention_workspace(self, cache: PagedCache, batch: PagedBatch, heads: int) -> int:
         """Bytes of workspace paged_attention needs for batches of these bounds."""
         check_paged(cache, batch, heads)
-        return lib().b2d_paged_attention_workspace(self._h, cache.ref, batch.ref, heads)
+        need = lib().b2d_paged_attention_workspace(self._h, cache.ref, batch.ref, heads)
+        if need == 0:
+            raise B2DError(-1, lib().b2d_last_error(self._h).decode())
+        return need
 
     def paged_attention(self, q, cache: PagedCache, batch: PagedBatch, out, scale: Optional[float] = None,
                         window: int = 0, workspace=None, stream: int = 0) -> None:

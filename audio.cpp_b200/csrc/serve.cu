@@ -155,12 +155,6 @@ void gather_as(int kind, const KvView& kv, const BatchView& b, void* k, void* v,
 
 }  // namespace
 
-void kv_check(const b2d_kv_cache* cache, const b2d_kv_batch* batch, int heads) {
-    const KvView kv = cache_view(cache);
-    batch_view(batch, cache, nullptr);
-    if (heads != 0) check_heads(kv, heads);
-}
-
 void kv_append(const ServeDevice& dev, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int src_type, const void* k,
                const void* v, int64_t row_stride, cudaStream_t st) {
     const KvView kv = cache_view(cache);
@@ -236,6 +230,20 @@ TcPlan tc_plan(const BatchView& b, const KvView& kv, int group, int num_sms) {
     return {int(pairs), int(std::max<int64_t>(1, splits))};
 }
 
+// Row tiles of the stream kernel that a sequence may have: 0 when none of them can be its.
+int stream_row_tiles(const BatchView& b, const KvView& kv, int group, bool single_to_tc) {
+    const int64_t most = single_to_tc ? 0 : stream_most_rows(kv);
+    const int rows = stream_rows(b, group);
+    return int((std::min(batch_packed_rows(b, group), most) + rows - 1) / rows);
+}
+
+// Sizes that only attention bounds: its grids'.  Before anything is launched.
+void check_attention_batch(const BatchView& b, const KvView& kv, int group) {
+    if (int64_t(b.rows) * group * kv.kv_heads > kMaxVectors ||
+        int64_t(b.seqs) * stream_row_tiles(b, kv, group, false) * kv.kv_heads > 0x7fffffff)
+        fail(B2D_EINVAL, "paged attention batch is too large");
+}
+
 constexpr int kMaxRunsPerSm = 4;
 
 // One box = one page's slots of one head, 64 dims wide, 128-byte swizzle; pages outside the pool read as zeros.
@@ -272,8 +280,7 @@ void launch_stream(const AttentionLaunch& x) {
     set_smem_limit(kernel, int(Sh::kSmem));
     const int runs = x.num_sms * Sh::kMinBlocks;
     launch_k(kernel, dim3(unsigned(runs)), dim3(kPaWarps * 32), Sh::kSmem, x.st, 1, x.a);
-    const int64_t units = int64_t(x.a.b.seqs) * x.row_tiles * x.a.kv.kv_heads;
-    if (units > 0x7fffffff) fail(B2D_EINVAL, "paged attention batch is too large");
+    const int64_t units = int64_t(x.a.b.seqs) * x.row_tiles * x.a.kv.kv_heads;  // check_attention_batch
     const PdlScope early;  // it gets ready while the runs work, and waits for them before it reads
     launch_k(paged_merge_kernel<CT, HD, Sh::kRows>, dim3(unsigned(units), unsigned(Sh::kRows)), dim3(256), 0, x.st, 1, x.a,
              runs, x.row_tiles);
@@ -342,10 +349,18 @@ static size_t attention_bytes(const BatchView& b, const KvView& kv, int group, i
     return stream_bytes(b, kv, group, num_sms) + tc_rows * (size_t(kv.head_dim) + 2) * 4;
 }
 
+void kv_check(const b2d_kv_cache* cache, const b2d_kv_batch* batch, int heads) {
+    const KvView kv = cache_view(cache);
+    const BatchView b = batch_view(batch, cache, nullptr);
+    if (heads != 0) check_attention_batch(b, kv, check_heads(kv, heads));
+}
+
 size_t paged_attention_workspace(const ServeDevice& dev, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int heads) {
     const KvView kv = cache_view(cache);
     const BatchView b = batch_view(batch, cache, dev.status);
-    return attention_bytes(b, kv, check_heads(kv, heads), dev.num_sms);
+    const int group = check_heads(kv, heads);
+    check_attention_batch(b, kv, group);
+    return attention_bytes(b, kv, group, dev.num_sms);
 }
 
 void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2d_kv_batch* batch, bool bf16,
@@ -359,7 +374,7 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
     const int kind = pool_kind(cache->type);
     if ((kind == kPoolF16 && bf16) || (kind == kPoolBf16 && !bf16))
         fail(B2D_EINVAL, "a 16-bit paged cache must have the queries' type");
-    if (int64_t(a.b.rows) * heads > kMaxVectors) fail(B2D_EINVAL, "paged attention batch is too large");
+    check_attention_batch(a.b, a.kv, a.group);
     if (a.b.rows == 0 || a.b.seqs == 0 || a.b.max_new == 0) return;
     if (!q || !o || misaligned(q, 16) || misaligned(o, 16) || q_row % 8 || o_row % 8)
         fail(B2D_EINVAL, "paged attention rows must be 16-byte aligned device memory");
@@ -384,9 +399,9 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + stream_slots(dev.num_sms) * x.rows * a.kv.head_dim);
     // one sequence that may be long belongs to the tensor-tile kernel whatever its rows turn out to be
-    if (a.b.seqs == 1 && x.tc.pairs > 0) a.min_rows = 0;
-    const int64_t packed = std::min<int64_t>(batch_packed_rows(a.b, a.group), a.min_rows);
-    x.row_tiles = int((packed + x.rows - 1) / x.rows);
+    const bool single_to_tc = a.b.seqs == 1 && x.tc.pairs > 0;
+    if (single_to_tc) a.min_rows = 0;
+    x.row_tiles = stream_row_tiles(a.b, a.kv, a.group, single_to_tc);
     x.num_sms = dev.num_sms;
     x.st = st;
     if (bf16) {

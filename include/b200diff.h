@@ -487,13 +487,14 @@ B2D_API size_t b2d_paged_attention_workspace(b2d_ctx* ctx, const b2d_kv_cache* c
  *   o = sum_j softmax_j(scale q . k_j) v_j  over the positions j <= p, with window > 0 only those above p - window;
  * scale is positive, finite and below 2^127.
  * q, o: [rows, heads, head_dim] fp16 (bf16 = 0) or bf16 (bf16 = 1), row strides q_row / o_row in elements, 16-byte
- * aligned, not overlapping; a 16-bit cache has the queries' type.  heads is 1 to 128 times kv_heads.  A row that sees
- * no key gives zeros.  Keys and values at the positions that a new row of the sequence sees must be finite; what lies
- * behind the context in its last page, or before the window of the sequence's first new row, may be anything, and pages
- * that hold nothing else need no valid table entry.  Value scales of one context lie within 2^100 of each other; beside
- * all-zero value vectors, which count as 2^-60, from 2^-60 to 2^41.  Scores, softmax sums and the output's sums are fp32;
- * probabilities enter the second product rounded to the queries' type, or, times the value's scale, to fp16 for an 8-bit
- * cache, whose codes are multiplied as they are.  The same batch gives the same bits whenever it runs.
+ * aligned, not overlapping; a 16-bit cache has the queries' type.  heads is 1 to 128 times kv_heads, rows x heads at most
+ * 2^30 (head_dim 32: seqs x max_new x heads / 16 below 2^31 too).  A row that sees no key gives zeros.  Keys and values
+ * at the positions that a new row of the sequence sees must be finite; what lies behind the context in its last page, or
+ * before the window of the sequence's first new row, may be anything, and pages that hold nothing else need no valid
+ * table entry.  Value scales of one context lie within 2^100 of each other; beside all-zero value vectors, which count
+ * as 2^-60, from 2^-60 to 2^41.  Scores, softmax sums and the output's sums are fp32; probabilities enter the second
+ * product rounded to the queries' type, or, times the value's scale, to fp16 for an 8-bit cache, whose codes are
+ * multiplied as they are.  The same batch gives the same bits whenever it runs.
  * workspace: 16-byte aligned, contents neither read nor kept; calls that may overlap (two streams, two graphs) need
  * one each. */
 B2D_API b2d_status b2d_paged_attention(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t bf16,

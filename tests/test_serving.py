@@ -144,3 +144,18 @@ def test_contexts_next_to_2_31_are_refused(b2d, most, fits):
     else:
         with pytest.raises(b2d.B2DError, match="max_context"):
             b2d.check_paged(cache, batch)
+
+
+@pytest.mark.parametrize("seqs,rows,dim,fits", [(512, 1 << 18, 32, True), (4096, 1 << 18, 32, False), (8192, 1 << 22, 32, False),
+                                               (8192, 1 << 22, 64, True), (2, 1 << 27, 64, False)])
+def test_attention_batches_too_large_for_a_grid_are_refused_first(b2d, seqs, rows, dim, fits):
+    """Rows of all heads, and what the parts of head_dim 32 are joined by: (sequence, 16 rows of the longest, kv head), which
+    are seqs x (rows x 8 heads a kv head / 16) x 8 kv heads here, at most 2^31 - 1: 2^29, 2^32 and 2^37."""
+    cache, batch = _cache(b2d, heads=8, dim=dim), _batch(b2d)
+    batch.desc.seqs, batch.desc.rows, batch.desc.max_new = seqs, rows, rows
+    b2d.check_paged(cache, batch)  # no attention
+    if fits:
+        b2d.check_paged(cache, batch, heads=64)
+    else:
+        with pytest.raises(b2d.B2DError, match="too large"):
+            b2d.check_paged(cache, batch, heads=64)
