@@ -41,13 +41,16 @@ struct Fail {
 // ------------------------------------------------------ kernel launches
 // Launches inside a PdlScope carry the programmatic-stream-serialization attribute: the next kernel may start
 // its prologue (and its constant-weight loads) while this one finishes; every kernel launched this way calls
-// pdl_wait before touching data of its predecessors.  Per host thread, so concurrent contexts do not interact.
+// pdl_wait before touching data of its predecessors.  Per host thread, so concurrent contexts do not interact.  Set by
+// scopes alone: a launch that fails throws, and must not leave it set for the thread's later calls.
 inline thread_local bool tl_pdl = false;
 
 struct PdlScope {
     bool prev;
-    PdlScope() : prev(tl_pdl) { tl_pdl = true; }
+    explicit PdlScope(bool on = true) : prev(tl_pdl) { tl_pdl = on; }
     ~PdlScope() { tl_pdl = prev; }
+    PdlScope(const PdlScope&) = delete;
+    PdlScope& operator=(const PdlScope&) = delete;
 };
 
 template <typename... KArgs, typename... Args>

@@ -305,11 +305,9 @@ void launch_tc(const AttentionLaunch& x) {
     }
     {
         // behind the stream kernel and its join, which have other sequences: beside them (the kernel ends after them)
-        const bool outer = tl_pdl;
-        tl_pdl = x.row_tiles > 0;
+        const PdlScope beside(x.row_tiles > 0);
         launch_k(kernel, dim3(unsigned(x.tc.pairs), kvh, unsigned(x.tc.splits)), dim3(Sh::kThreads), Sh::kSmem, x.st, 1, tk,
                  tv, ta);
-        tl_pdl = outer;
     }
     if (x.tc.splits > 1)
         launch_k(paged_join_kernel<CT, HD>, dim3(unsigned(x.tc.pairs), kvh, 32u), dim3(256), 0, x.st, 1, ta);

@@ -1,5 +1,9 @@
 """CPU tests of the serving operators' argument checks (the paged cache, its batches, attention heads) through
 b2d_kv_check and the Python layer: what a call would refuse is refused before any device work."""
+import os
+import re
+import subprocess
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -159,3 +163,41 @@ def test_attention_batches_too_large_for_a_grid_are_refused_first(b2d, seqs, row
     else:
         with pytest.raises(b2d.B2DError, match="too large"):
             b2d.check_paged(cache, batch, heads=64)
+
+
+SCOPE_TEST = r"""
+#include "host.cuh"
+int main() {
+    using namespace b2d;
+    auto failed_launch = [](bool on) {  // as a launch that the driver refuses leaves the scope
+        try {
+            const PdlScope scope(on);
+            if (tl_pdl != on) return false;
+            fail(B2D_ECUDA, "kernel launch failed");
+        } catch (const Fail&) {
+        }
+        return true;
+    };
+    if (!failed_launch(true) || tl_pdl) return 1;
+    const PdlScope outer;
+    if (!failed_launch(false) || !tl_pdl) return 2;
+    return 0;
+}
+"""
+
+
+def test_a_failed_launch_leaves_no_launch_attribute_behind(tmp_path):
+    """The thread's programmatic-launch flag is set by scopes alone, which an exception leaves too; otherwise every later
+    launch of the thread could start before its inputs are written."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "audio.cpp_b200", "csrc")
+    for name in sorted(os.listdir(csrc)):
+        with open(os.path.join(csrc, name)) as f:
+            text = f.read()
+        if name == "host.cuh":
+            text = re.sub(r"struct PdlScope \{.*?\n\};", "", text, flags=re.S).replace("tl_pdl = false;", "", 1)
+        assert not re.search(r"\btl_pdl\s*=[^=]", text), name
+    source, program = tmp_path / "scope.cu", tmp_path / "scope"
+    source.write_text(SCOPE_TEST)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    subprocess.run([os.path.join(cuda, "bin", "nvcc"), "-std=c++17", "-I", csrc, "-o", str(program), str(source)], check=True)
+    assert subprocess.run([str(program)]).returncode == 0
