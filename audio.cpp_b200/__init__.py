@@ -322,11 +322,17 @@ class PagedCache:
         self.ref = C.byref(self.desc)
 
 
+_INT32_MAX = 2 ** 31 - 1
+
+
 class PagedBatch:
     """The new tokens of some sequences (b2d_kv_batch): int32 device tensors ``row_start`` [seqs + 1], ``context`` [seqs]
     and ``page_table`` [seqs, pages], with the bounds that hold for this call and every replay of it."""
 
     def __init__(self, row_start, context, page_table, rows: int, max_new: int, max_context: int):
+        for name, bound in (("max_new", max_new), ("max_context", max_context)):  # ctypes would wrap them
+            if not 0 <= bound <= _INT32_MAX:
+                raise B2DError(-1, "paged cache batch %s %d is negative or too large" % (name, bound))
         seqs = context.shape[0]
         _want(context, "context", (seqs,), _INT32)
         _want(row_start, "row_start", (seqs + 1,), _INT32, context.device)
@@ -503,8 +509,8 @@ class Context:
         many = shape[0] > 1
         st = lib().b2d_paged_attention(
             self._h, cache.ref, batch.ref, 1 if kind == TYPE_BF16 else 0, q.data_ptr(), qs[0] if many else heads * hd,
-            out.data_ptr(), os_[0] if many else heads * hd, heads, hd ** -0.5 if scale is None else scale, window,
-            *self._workspace(workspace), stream)
+            out.data_ptr(), os_[0] if many else heads * hd, heads, hd ** -0.5 if scale is None else scale,
+            window if 0 < window <= _INT32_MAX else 0, *self._workspace(workspace), stream)
         if st:
             self.check(st)
 

@@ -165,6 +165,32 @@ def test_attention_batches_too_large_for_a_grid_are_refused_first(b2d, seqs, row
             b2d.check_paged(cache, batch, heads=64)
 
 
+@pytest.mark.parametrize("bound", [-1, 2 ** 31, 2 ** 32 + 2])
+@pytest.mark.parametrize("name", ["max_new", "max_context"])
+def test_bounds_that_do_not_fit_are_refused(b2d, name, bound):
+    """2^32 + 2 as a 32-bit integer would be 2."""
+    with pytest.raises(b2d.B2DError, match=name):
+        _batch(b2d, pages=1, **{name: bound})
+
+
+@pytest.mark.parametrize("window,passed", [(0, 0), (-5, 0), (5 - 2 ** 32, 0), (7, 7), (2 ** 31 - 1, 2 ** 31 - 1),
+                                           (2 ** 31, 0), (2 ** 32 + 5, 0)])
+def test_windows_past_32_bits_are_none(b2d, monkeypatch, window, passed):
+    """A window longer than any context hides nothing; 2^32 + 5 as a 32-bit integer would be 5."""
+    ctx, got = _no_device_context(b2d), []
+
+    class Library:
+        @staticmethod
+        def b2d_paged_attention(*args):
+            got.append(b2d.C.c_int32(args[10]).value)
+            return 0
+    monkeypatch.setattr(b2d, "lib", lambda: Library)
+    q = torch.zeros(4, 2, 64, dtype=torch.float16)
+    ctx.paged_attention(q, _cache(b2d), _batch(b2d), torch.empty_like(q), window=window,
+                        workspace=torch.zeros(16, dtype=torch.uint8))
+    assert got == [passed]
+
+
 SCOPE_TEST = r"""
 #include "host.cuh"
 int main() {
