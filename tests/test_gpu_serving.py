@@ -472,7 +472,7 @@ def rewrite(s, name, change):
         dense[i] = held.double()
 
 
-UNEVEN = ["spread", "late_values", "late_keys", "zeros", "zeros_first", "zero_groups", "rising"]
+UNEVEN = ["even", "spread", "late_values", "late_keys", "zeros", "zeros_first", "zero_groups", "rising"]
 
 
 @pytest.mark.parametrize("kind", UNEVEN)
@@ -483,7 +483,7 @@ UNEVEN = ["spread", "late_values", "late_keys", "zeros", "zeros_first", "zero_gr
     ([40, 70, 1, 16], [600, 300, 400, 333], 64, 128, 0), ([1, 3, 50], [700, 130, 500], 64, 16, 77),
     ([3, 40], [200, 150], 32, 16, 0)])
 def test_attention_uneven_scales(b2d, ctx, new, context, head_dim, page, window, dtype, pool, kind):
-    """Scales that differ by orders of magnitude between neighbouring keys: spread over 2^20; a key in 32 far above its
+    """Scales that are alike, or differ by orders of magnitude between neighbouring keys: spread over 2^20; a key in 32 far above its
     neighbours, which rows before it do not see; all-zero vectors, alone, 32 together and before all others, beside large
     values; scores that rise key by key."""
     kv, group = 2, 4
@@ -518,7 +518,7 @@ def test_attention_uneven_scales(b2d, ctx, new, context, head_dim, page, window,
     elif kind == "zero_groups":
         rewrite(s, "k", lambda i, x: zeros(x, lambda j: j // 32 % 3 == 1))
         rewrite(s, "v", lambda i, x: zeros(x, lambda j: j // 32 % 2 == 1))
-    else:
+    elif kind == "rising":
         ramp = torch.linspace(0, 40, max(context), device=DEV)
         rewrite(s, "k", lambda i, x: torch.cat([ramp[:len(x), None, None].expand(-1, kv, 1), 0.05 * x[..., 1:]], -1))
         rewrite(s, "v", lambda i, x: powers(x, -6, 6))
@@ -949,3 +949,92 @@ def test_overlapping_calls_with_their_own_workspaces(b2d, ctx):
         for o in many:
             assert torch.equal(o, want)
     ctx.sync(stream())
+
+
+@pytest.mark.parametrize("pool", ["bf16", "int8"])
+def test_mixed_batches_in_a_graph(b2d, ctx, pool):
+    """Chunks beside single tokens -- the stream kernel, its join, the tensor-tile kernel and its join in one call -- captured
+    once and replayed as rows move between the sequences, contexts and pages change within the bounds, and a call by itself
+    runs on the same workspace in between; the replays give the eager call's bits."""
+    s = Setup(b2d, [1, 130, 2, 40, 1], [3000, 1000, 40, 2500, 17], 2, 128, 32, pool)
+    q = torch.randn(s.rows, 12, 128, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).bfloat16()
+    work = torch.empty(ctx.paged_attention_workspace(s.cache, s.batch, 12), dtype=torch.uint8, device=DEV)
+    out = torch.empty_like(q)
+    attend(ctx, s, q, out=out, workspace=work)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(ctx, s, q, out=out, workspace=work)
+    full = s.table.clone()
+    rng = np.random.default_rng(5)
+    for i in range(20):
+        s.new = [int(x) for x in (rng.integers(0, 131, 5) if i % 3 else [1, 1, 1, 1, 1])]
+        while sum(s.new) > s.rows:
+            s.new[int(np.argmax(s.new))] //= 2
+        order = rng.permutation(5)
+        s.table.copy_(full[torch.tensor(order, device=DEV)])
+        dense_k, dense_v = s.dense_k, s.dense_v
+        have = [len(dense_k[j]) for j in order]
+        s.context = [int(rng.integers(0, n + 1)) for n in have]
+        s.start = [0] + [int(x) for x in np.cumsum(s.new)]
+        s.row_start.copy_(torch.tensor(s.start, dtype=torch.int32))
+        s.context_dev.copy_(torch.tensor(s.context, dtype=torch.int32))
+        out.fill_(77.0)
+        graph.replay()
+        want = attend(ctx, s, q, workspace=work)
+        assert torch.equal(out, want), i
+        out.fill_(77.0)
+        graph.replay()
+        assert torch.equal(out, want), i
+        if i % 5 == 0:
+            s.dense_k, s.dense_v = ([d[j][:c] for j, c in zip(order, s.context)] for d in (dense_k, dense_v))
+            check_attention(s, q, out)
+            s.dense_k, s.dense_v = dense_k, dense_v
+    ctx.sync(stream())
+
+
+@pytest.mark.parametrize("long", [False, True])
+def test_as_many_sequences_as_there_may_be(b2d, ctx, long):
+    """8192 sequences, some without rows or keys, with and without one long chunk among them: written, read back, attended."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rng = np.random.default_rng(1)
+    new = [int(x) for x in rng.integers(0, 3, 8192)]
+    context = [int(x) for x in np.maximum(new, rng.integers(0, 24, 8192))]
+    if long:
+        new[5000], context[5000] = 300, 900
+    s = Setup(b2d, [], [], 2, 64, 16, "int8")  # only for its helpers' sake; the batch is built here
+    page, kv, hd = 16, 2, 64
+    need = [-(-c // page) for c in context]
+    first = np.cumsum([0] + need)
+    pages = int(first[-1])
+    order = torch.randperm(pages, generator=g, device=DEV).int()
+    table = torch.full((8192, max(need)), -7, dtype=torch.int32, device=DEV)
+    rows = torch.from_numpy(np.repeat(np.arange(8192), need)).to(DEV)
+    col = torch.from_numpy(np.arange(pages) - np.repeat(first[:-1], need)).to(DEV)
+    table[rows, col] = order
+    pools = [torch.zeros(pages, kv, page, hd, dtype=torch.int8, device=DEV) for _ in range(2)]
+    scales = [torch.zeros(pages, kv, page, device=DEV) for _ in range(2)]
+    cache = b2d.PagedCache(*pools, *scales)
+    i32 = dict(dtype=torch.int32, device=DEV)
+
+    def batch(counts):
+        start = torch.tensor(np.cumsum([0] + counts), **i32)
+        return b2d.PagedBatch(start, torch.tensor(context, **i32), table, sum(counts), max(counts), max(context))
+    whole = batch(context)  # every context is written, and read back
+    k, v = (torch.randn(sum(context), kv, hd, generator=g, device=DEV) for _ in range(2))
+    ctx.kv_append(cache, whole, k, v, stream=stream())
+    back = [torch.empty_like(k) for _ in range(2)]
+    ctx.kv_gather(cache, whole, back[0], back[1], stream=stream())
+    ctx.sync(stream())
+    held = [quantise(x, torch.int8)[0].to(DEV) for x in (k, v)]
+    assert torch.equal(back[0], held[0]) and torch.equal(back[1], held[1])
+    some = batch(new)
+    q = torch.randn(sum(new), 4, hd, generator=g, device=DEV).half()
+    out = torch.full_like(q, 77.0)
+    work = torch.empty(ctx.paged_attention_workspace(cache, some, 4), dtype=torch.uint8, device=DEV)
+    ctx.paged_attention(q, cache, some, out, workspace=work, stream=stream())
+    ctx.sync(stream())
+    at = np.cumsum([0] + context)
+    s.dense_k, s.dense_v = ([x[at[i]:at[i + 1]].double() for i in range(8192)] for x in held)
+    s.new, s.context, s.start, s.dtype = new, context, [int(x) for x in np.cumsum([0] + new)], torch.int8
+    check_attention(s, q, out)
