@@ -228,7 +228,7 @@ __device__ __forceinline__ int64_t scale_index(const KvView& kv, int page, int h
 // New rows into the cache.  Bound by HBM: each source element is read once and each pool element written once.  One
 // vector (one head of one row, of K or of V) belongs to head_dim / 8 lanes, eight elements a lane: 16-byte loads of
 // 16-bit sources (two of fp32), 8-byte stores of 8-bit pools, the largest magnitude found by shuffles, nothing
-// staged in shared memory but the batch description.  65537 rows of 4 x 128 fp32 to int8 and back to fp32: 153 us, 4.4 TB/s
+// staged in shared memory but the batch description.  65537 rows of 4 x 128 fp32 to int8 and back to fp32: 152 us, 4.4 TB/s
 // of the 675 MB that both calls have to move.
 template <typename Src, int POOL>
 __global__ void __launch_bounds__(256, 8) kv_append_kernel(KvView kv, BatchView b, const Src* __restrict__ k,

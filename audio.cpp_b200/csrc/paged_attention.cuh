@@ -13,9 +13,13 @@
 // their way).  8-bit pools have half the bytes a step, too few on their way from registers alone (4.1 TB/s): each lane
 // copies its own pieces three steps ahead into a ring in shared memory with cp.async and reads back what it copied.
 //
-// 8-bit pools: codes are exact in fp16, so both products run on bare codes in fp16 and nothing is rounded but P.  The
-// key's scale multiplies the finished score; bf16 queries are brought to fp16 by a power of two per row that makes
-// their largest entry lie in [1, 2) (entries below 2^-14 of it lose bits far under the bf16 rounding of the others).
+// What is held in fewer than 32 bits: P, since a tensor product's operands are 16-bit and of one type (V's).  Against 64 bits
+// that is 2.3e-3 of the output's norm with bf16 caches and 2.4e-4 with fp16, where rounding the output alone is 1.7e-3 and
+// 2.1e-4; scores, the maximum, the sums of p and of p v are fp32.
+//
+// 8-bit pools: codes are exact in fp16, so both products run on bare codes in fp16 and nothing is rounded but P (to fp16:
+// 1.7e-3 with bf16 queries).  The key's scale multiplies the finished score; bf16 queries are brought to fp16 by a power of
+// two per row that makes their largest entry lie in [1, 2) (entries below 2^-14 of it are rounded to 2^-25 of it).
 // The value's scale multiplies the probability, t = p vs, before it is rounded to fp16; the running maximum is that
 // of s + log2 vs, so the largest t of a row is near 1 whatever the scales are and what fp16 flushes is below 2^-24
 // of it.  (Expanding V to round(code x scale) instead doubled the error against 64 bits, 0.0029 to 0.0017 of the
@@ -25,8 +29,9 @@
 // SM alike whatever the lengths.  A run that holds only part of a unit leaves (O, m, l) in the workspace and
 // paged_merge_kernel joins the parts in their order in the list, so results do not depend on timing.
 //
-// 3 sequences of up to 131071 keys, bf16, 28 / 4 heads of 128: 103 us, 6.1 TB/s (94 % of a copy's rate).  64 of up to 8190,
-// int8: 91 us, 3.8 TB/s, bound by issue (half of the slots) and latency: some 490 instructions for 16 keys, three CTAs an SM.
+// 3 sequences of up to 131071 keys, bf16, 28 / 4 heads of 128: 101 us, 6.3 TB/s (96 % of a copy's rate).  64 of up to 8190,
+// int8: 90 us, 3.8 TB/s; neither issue (51 % of the slots) nor HBM (52 %) is full: some 490 instructions for 16 keys in
+// dependent steps, and twelve warps an SM to hide them behind one another.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -254,7 +259,8 @@ struct PagedShape {
     static constexpr int kVPiece = (kVw < 4 ? kVw : 4) * 4;
     static constexpr int kDepth = 4;  // 8-bit: steps in the ring
     static constexpr int kRingWords = 32 * (2 * kKw + 4 * kVw + 1);  // of one step of a warp: K, V, a scale a lane
-    // CTAs an SM holds: what the registers allow without spilling (the O accumulators of 16 rows of 128 take 64)
+    // CTAs an SM holds: what the registers allow (the O accumulators of 16 rows of 128 take 64).  Nothing spills but 4 to 12
+    // bytes of 16 rows of 64 over 8-bit pools, which stay within 128 registers.
     static constexpr int kMinBlocks = HD == 128 ? (NT == 1 ? 3 : 2) : kWide ? 3 : 4;
     static constexpr size_t kJoin = size_t(kPaWarps) * kRows * (HD + 2) * 4;
     static constexpr size_t kRing = kWide ? 0 : size_t(kPaWarps) * kDepth * kRingWords * 4;

@@ -17,9 +17,12 @@
 //   8-bit caches: three pairs of warps read the codes and write them as fp16, which is exact, in the same layout.  Scales
 //     are applied as in paged_stream_kernel: y = s + log2 vs is the logarithm of t = p vs, m follows y, t = 2^(y - m) is
 //     what is rounded and multiplied with the codes, and the row's sum adds t / vs.  (fp16 values of code x scale, with one
-//     power of two for 32 keys, spare the softmax 48 shared loads a half: 2.37 in place of 2.71 ms for four int8 prompts.
+//     power of two for 32 keys, spare the softmax 48 shared loads a half: 2.45 in place of 2.79 ms for four int8 prompts.
 //     But a row then loses bits to a key beside those it sees, even one that is masked, whose scale is far above theirs,
-//     and keys off by 2^-11 change which of two large scores is the larger.)
+//     and keys off by 2^-11 change which of two large scores is the larger.)  With 512 threads a thread has 128 registers,
+//     and the softmax of 8-bit caches spills some of its 64 scores' companions: 40 to 64 bytes stored.
+// 4 x up to 4096 rows over up to 16384 keys, 28 / 4 heads of 128: int8 2.79 ms with bf16 queries, 2.73 with fp16, e4m3 2.71;
+// 2 x up to 2047 over up to 8191, 12 / 2 heads, bf16: 131 us.
 // K and V have a ring of two blocks each.  TMEM (512 columns): S (and P) of tile t, half h at 128 t + 64 h, O_t at
 // 256 + 128 t.
 // Few units are spread over more CTAs by cutting the key range into `splits`; paged_join_kernel joins the parts.
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(PagedTcShape<POOL, HD>::kThreads, 1)
                     y1 = kWide ? fma_x2(y1, rf2, base2) : add_x2(y1, base2);
                     y0.x = ex2_approx(y0.x), y0.y = ex2_approx(y0.y);
                     // A quarter of them off MUFU: 145 -> 131 us for 2047 + 1098 rows of 12 / 2 heads over 8191 keys.  Not with
-                    // 8-bit caches, whose code warps want the issue slots (2.35 -> 2.54 ms for four int8 prompts).
+                    // 8-bit caches, whose code warps want the issue slots (four int8 prompts were a twelfth slower).
                     if (kWide && (e & 4)) y1 = ex2_fma_x2(y1);
                     else y1.x = ex2_approx(y1.x), y1.y = ex2_approx(y1.y);
                     if constexpr (!kWide) {

@@ -16,7 +16,8 @@
 // -> 48k clocks).
 // One row of 32003 fp32 entries takes 15 us, its cluster's barriers and passes one after the other; 64 x 128256 of mixed
 // requests 91 us (0.4 TB/s): the passes that weigh entries in fp64, 33k clocks of the 120k that a row with top-p alone
-// takes, and its second round.
+// takes, and its second round.  (64 registers keep two CTAs an SM; find_cut costs the fp32 and fp16 forms 72 bytes of spills,
+// and in the bf16 form it is not inlined and takes what it captures from a stack frame.)
 // Which token comes out depends on sums of up to 2^18 terms and on comparisons next to a border, so the weights are
 // computed in fp64 and added as integers (units of 2^-45 of the largest weight): sums of integers do not depend on
 // the order of threads, warps or CTAs, so neither does the token.

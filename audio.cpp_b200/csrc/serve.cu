@@ -206,10 +206,14 @@ int stream_rows(const BatchView& b, int group) { return int64_t(b.max_new) * gro
 
 // Packed rows (tokens x heads per kv head) up to which a sequence goes through the stream kernel.  Its cost grows with
 // every tile of 16 rows that reads the keys again, the tensor-tile kernel's with every pair of 128; with 8-bit caches that
-// one also waits for its codes, whatever the rows.  64 sequences of up to 3 tokens over up to 8192 keys, 28 / 4 heads of
-// 128 (21 packed rows at most): stream 253 us, tensor tiles 187 with bf16 caches, 207 and 345 with int8; of up to 5 over
-// 2048 (35 rows): 138 and 64, 132 and 106.  A few ragged int8 sequences on both sides of the border pay for two kernels:
-// 8 of up to 9 tokens over 4096 take 35 us, with a border of 16 rows 27.  head_dim 32 has no tensor-tile kernel.
+// one also waits for its codes, whatever the rows.  64 sequences, 28 / 4 heads, stream and tensor tiles in us, bf16 queries:
+//                                             bf16 x 128    int8 x 128    bf16 x 64     int8 x 64
+//   up to 3 tokens over 8192 (21 rows)        253, 189      209, 356      157, 159      142, 301
+//   up to 4 over 4096 (28 rows)               154, 107      137, 191      103, 89       97, 161
+//   up to 5 over 2048 (35 rows)               139, 65       134, 110      93, 54        93, 92
+// (fp16 queries over int8 take 1 to 6 % less in either.)  A few ragged int8 sequences on both sides of the border pay for two
+// kernels: 8 of up to 9 tokens over 4096 take 37 us, all of them in either kernel 26 to 28.  head_dim 32 has no
+// tensor-tile kernel.
 int stream_most_rows(const KvView& kv) { return kv.head_dim == 32 ? 0x7fffffff : kv.ks ? 32 : 16; }
 
 int64_t batch_packed_rows(const BatchView& b, int group) { return int64_t(std::min(b.max_new, b.rows)) * group; }
@@ -414,8 +418,13 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
 }
 
 // -------------------------------------------------------------------------------------------------- sampling
-// bf16 rows from which a CTA each, counting values, is faster than a cluster each, weighing entries: 8 rows of 128256 take
-// 96 and 124 us with top-p, 75 and 53 with top-k; 16 rows 97 and 153, 76 and 72; 64 rows 99 and 356, 77 and 149.
+// bf16 rows from which a CTA each, counting values, is the better of a cluster each, weighing entries.  Values and cluster
+// in us, with top-p, top-k and no cut:
+//                 vocabulary 300              4096                        32003                      128256
+//   8 rows        25, 28; 18, 30; 19, 15      26, 40; 19, 35; 19, 16      42, 60; 32, 36; 35, 19     97, 124; 76, 54; 88, 27
+//   16            25, 28; 19, 30; 19, 15      27, 46; 19, 38; 19, 16      43, 73; 32, 50; 35, 25     98, 153; 76, 72; 88, 37
+//   64            26, 30; 19, 31; 19, 15      28, 52; 19, 43; 20, 17      44, 167; 33, 104; 36, 59   99, 354; 77, 150; 90, 85
+// (Which cuts a row makes is known on the device alone.)
 constexpr int64_t kValueRows = 16;
 
 void sample_tokens(const ServeDevice&, const b2d_sample_request* rq, cudaStream_t st) {

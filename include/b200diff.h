@@ -494,7 +494,8 @@ B2D_API size_t b2d_paged_attention_workspace(b2d_ctx* ctx, const b2d_kv_cache* c
  * table entry.  Value scales of one context lie within 2^100 of each other; beside all-zero value vectors, which count
  * as 2^-60, from 2^-60 to 2^41.  Scores, softmax sums and the output's sums are fp32; probabilities enter the second
  * product rounded to the queries' type, or, times the value's scale, to fp16 for an 8-bit cache, whose codes are
- * multiplied as they are.  The same batch gives the same bits whenever it runs.
+ * multiplied as they are (by bf16 queries in fp16, a power of two a row: entries below 2^-14 of a row's largest are rounded
+ * to 2^-25 of it).  The same batch gives the same bits whenever it runs.
  * workspace: 16-byte aligned, contents neither read nor kept; calls that may overlap (two streams, two graphs) need
  * one each. */
 B2D_API b2d_status b2d_paged_attention(b2d_ctx* ctx, const b2d_kv_cache* cache, const b2d_kv_batch* batch, int32_t bf16,
