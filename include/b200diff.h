@@ -528,7 +528,7 @@ B2D_API b2d_status b2d_vvlm_forward_paged(b2d_ctx* ctx, const b2d_kv_cache* cach
  * temperature <= 0 (or NaN) takes the best entry.  A NaN logit counts as -infinity, +infinity as certain; a row without an
  * entry above -infinity gives token -1.  Weights are computed in fp64 to within 2^-44 of the largest and summed
  * exactly in units of 2^-45 of it (an entry below half a unit is never drawn), so the token depends on nothing but the
- * arguments. */
+ * arguments.  tokens and probs overlap none of the other arrays. */
 typedef struct {
     int32_t logits_type;        /* B2D_TYPE_F32, B2D_TYPE_F16 or B2D_TYPE_BF16 */
     int64_t rows, vocab;        /* vocab 1 to 262144 */

@@ -10,8 +10,8 @@ u |o|.  Probabilities are rounded to fp16 for fp16 queries and for every 8-bit c
 integer codes).  An fp16 number below 2^-14 is off by 2^-25 absolute instead of u of itself.  The key that set the
 running maximum has t = 1, so with n keys the sum of t code is off by at most n 2^-25 max|code|, and the sum of p is at
 least 1 / (that key's value scale): the output is off by at most n 2^-25 max|code| x scale <= n 2^-25 max|v|.  bf16
-queries on an 8-bit cache: chunks multiply keys rounded to fp16, each off by 2^-11 of itself (or 2^-25 of the largest of
-its neighbours), which moves a score by at most 2^-11 sum |q k| scale."""
+queries on an 8-bit cache: attention_bound also allows keys off by 2^-11 of themselves, which move a score by at most
+2^-11 sum |q k| scale; the kernels multiply exact codes, and check_uneven below holds them to that."""
 import numpy as np
 import pytest
 
