@@ -424,7 +424,7 @@ void paged_attention(const ServeDevice& dev, const b2d_kv_cache* cache, const b2
 //   8 rows        25, 28; 18, 30; 19, 15      26, 40; 19, 35; 19, 16      42, 60; 32, 36; 35, 19     97, 124; 76, 54; 88, 27
 //   16            25, 28; 19, 30; 19, 15      27, 46; 19, 38; 19, 16      43, 73; 32, 50; 35, 25     98, 153; 76, 72; 88, 37
 //   64            26, 30; 19, 31; 19, 15      28, 52; 19, 43; 20, 17      44, 167; 33, 104; 36, 59   99, 354; 77, 150; 90, 85
-// (Which cuts a row makes is known on the device alone.)
+// (Which cuts a row makes is known on the device; the rule looks at sizes.)
 constexpr int64_t kValueRows = 16;
 
 void sample_tokens(const ServeDevice&, const b2d_sample_request* rq, cudaStream_t st) {
